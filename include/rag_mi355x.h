@@ -319,6 +319,61 @@ int rag_hybrid_rrf_mmr(rag_csc_t* tfidf, rag_flat_t* flat, int n_dense, const in
  * budgets with (:437,:458).  Both NULL drops the tables.  Copied to HBM; refused while a query is begun. */
 int rag_csc_set_doc_tables(rag_csc_t* h, const int64_t* flat_row, const int64_t* text_bytes);
 
+/* ---- query adapters and distillation ----------------------------------- */
+
+/* Low-rank adapters of many requests at once beside a shared projection: what turns the embedding model's vector
+ * (embedding_manager.py:88-98, search_engine.py:141) into the vector the index is searched with, per store, user or
+ * task.  No counterpart in the reference, which searches with the model's vector itself.
+ *     y_t = W x_t + scale[s] B[s] (A[s] x_t),     s = slots[t];  -1: no adapter, y_t = W x_t
+ * x n x d_in (rows ldx apart), W d_out x d_in, A n_slots x rank x d_in, B n_slots x d_out x rank (dense, row-major),
+ * scale n_slots float32, slots n int64, y n x d_out (rows ldy apart).  x, W, A, B and y are of `dtype`; sums are
+ * float32 and y is rounded once.  A request whose slot is outside [-1, n_slots) gets NaN.  A shorter adapter is
+ * one whose last rows of A and columns of B are zero (its gradients are zero there too).  Any alignment of the
+ * rows of x / y; y must not overlap the inputs.  `ws_dev`: rag_adapter_ws_bytes bytes, 256-byte aligned, the
+ * caller's until the call's work on `stream` is done (calls that may overlap need one each).  Asynchronous on
+ * `stream`, nothing is allocated, may be captured into a graph. */
+#define RAG_ADAPTER_MAX_N (1 << 24)
+#define RAG_ADAPTER_MAX_SLOTS 4096
+#define RAG_ADAPTER_MAX_RANK 128
+int rag_adapter_ws_bytes(int dtype, int64_t n, int d_in, int d_out, int n_slots, int rank, int want_grad, int64_t* bytes);
+int rag_adapter_apply_dev(int dtype, int64_t n, int d_in, int d_out, int n_slots, int rank, const void* x_dev, int64_t ldx,
+                          const void* w_dev, const void* a_dev, const void* b_dev, const float* scale_dev,
+                          const int64_t* slots_dev, void* y_dev, int64_t ldy, void* ws_dev, int64_t ws_bytes, void* stream);
+/* Its backward: dy n x d_out -> dx = dy W + scale A^T (B^T dy) (of `dtype`; NULL: not wanted) and the bank's
+ * gradients dA n_slots x rank x d_in, dB n_slots x d_out x rank, float32, written whole (zeros for slots that no
+ * request has).  W is frozen.  A request outside the bank gets a NaN dx and adds nothing to dA / dB.  The sums
+ * over requests run in a fixed order: equal calls give equal bits.  ws: want_grad = 1. */
+int rag_adapter_grad_dev(int dtype, int64_t n, int d_in, int d_out, int n_slots, int rank, const void* x_dev, int64_t ldx,
+                         const void* w_dev, const void* a_dev, const void* b_dev, const float* scale_dev,
+                         const int64_t* slots_dev, const void* dy_dev, int64_t lddy, void* dx_dev, int64_t lddx,
+                         float* da_dev, float* db_dev, void* ws_dev, int64_t ws_bytes, void* stream);
+
+/* Distillation of a ranker's top list, forward and backward.  The teacher is what search_engine.py:362-394 asks for a
+ * second opinion (cross_encoder.predict over the hits of :141); the student is the dense score itself.  No counterpart
+ * in the reference, which does not train.
+ * Query i, rows x_j of the index: s_ij = <q_i, x_j> / temperature (inner product) or -||q_i - x_j||^2 / temperature
+ * (L2).  ids / scores (nq x k): the teacher's list per query, row numbers of this index (-1: no entry, as a search
+ * pads) and scores; p = softmax(scores / teacher_temperature) over the entries.  A row twice in a list counts twice.
+ *     over = RAG_OVER_INDEX:  loss_i = sum_k p_k (log p_k - s_k) + log sum_j exp(s_ij), j over EVERY row of the index
+ *     over = RAG_OVER_LIST:   ..., j over the entries of the list (a score of -inf is an entry with p = 0)
+ *     dq_i = weights_i d loss_i / d q_i      (weights NULL: 1; dq_dev NULL: the loss alone)
+ * q and dq (rows ldq / lddq apart) have the index' storage type, loss float32.  A query without an entry of finite
+ * score has loss 0 and dq 0; one with a row number outside [-1, ntotal) gets NaN.  Any alignment.
+ * `ws_dev`: rag_flat_distill_ws_bytes bytes (it does not depend on the number of rows; 0 for the list), 256-byte
+ * aligned, the caller's until the call's work on `stream` is done.  Asynchronous on `stream`; equal calls give equal
+ * bits.  May be captured into a graph once no added row is staged on the host (L2: once the norms exist), that is
+ * after any one call; the graph keeps the rows it was captured with (rows added later are not seen, rows replaced
+ * behind rag_flat_reset are) and must not outlive the handle. */
+#define RAG_OVER_INDEX 0
+#define RAG_OVER_LIST 1
+#define RAG_DISTILL_MAX_NQ 65535
+#define RAG_DISTILL_MAX_K 1024
+int rag_flat_distill_ws_bytes(rag_flat_t* h, int64_t nq, int k, int over, int want_grad, int64_t* bytes);
+int rag_flat_distill_dev(rag_flat_t* h, int64_t nq, const void* q_dev, int64_t ldq, int k, const int64_t* ids_dev,
+                         const float* scores_dev, double temperature, double teacher_temperature, int over,
+                         const float* weights_dev, float* loss_dev, void* dq_dev, int64_t lddq, void* ws_dev,
+                         int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

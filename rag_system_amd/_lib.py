@@ -26,6 +26,8 @@ METRIC_L2 = 1
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 MAX_K = 256
+OVER_INDEX = 0
+OVER_LIST = 1
 
 
 class EngineError(RuntimeError):
@@ -95,6 +97,14 @@ SIGNATURES = {
     "rag_hybrid_rrf_mmr": (C.c_int, [_p, _p, C.c_int, _p, C.c_int, _p, C.c_double, C.c_int, C.c_double, C.c_int, _p,
                                      C.c_double, _i64, _p, _p, _p, _p, _p, _p, _p]),
     "rag_csc_set_doc_tables": (C.c_int, [_p, _p, _p]),
+    "rag_adapter_ws_bytes": (C.c_int, [C.c_int, _i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _i64p]),
+    "rag_adapter_apply_dev": (C.c_int, [C.c_int, _i64, C.c_int, C.c_int, C.c_int, C.c_int, _p, _i64, _p, _p, _p, _p, _p, _p,
+                                        _i64, _p, _i64, _p]),
+    "rag_adapter_grad_dev": (C.c_int, [C.c_int, _i64, C.c_int, C.c_int, C.c_int, C.c_int, _p, _i64, _p, _p, _p, _p, _p, _p,
+                                       _i64, _p, _i64, _p, _p, _p, _i64, _p]),
+    "rag_flat_distill_ws_bytes": (C.c_int, [_p, _i64, C.c_int, C.c_int, C.c_int, _i64p]),
+    "rag_flat_distill_dev": (C.c_int, [_p, _i64, _p, _i64, C.c_int, _p, _p, C.c_double, C.c_double, C.c_int, _p, _p, _p,
+                                       _i64, _p, _i64, _p]),
 }
 
 _lock = threading.Lock()
@@ -186,6 +196,11 @@ def engine(device=None):
         elif _inited_device != int(device):
             raise ValueError("engine already initialised on device %d" % _inited_device)
     return lib
+
+
+def device():
+    """HIP ordinal the engine runs on (None before engine())."""
+    return _inited_device
 
 
 def lib_stream():

@@ -57,6 +57,39 @@ struct FlatView {
     int64_t n_rows;
 };
 int flat_with_view(rag_flat_t* h, int (*use)(const FlatView&, void*), void* ctx);
+// flat.hip: the rows of a flat index for a kernel that runs on the caller's stream and keeps no state in the
+// handle (rag_flat_distill_dev).  Staged rows are flushed and, with want_norms, the squared row norms are
+// complete before `use` runs, WITH THE HANDLE'S MUTEX HELD.  While `st` is being captured nothing may be flushed,
+// computed or waited for: then rows still staged or norms still missing are refused, and the handle keeps the
+// arrays that the graph names for as long as it lives (a later add that grows the arena leaves the old one to it).
+struct FlatRows {
+    const void* arena;     // n_rows x ld, fp32 or bfloat16, pad columns zero
+    const float* norms;    // ||x||^2 per row (want_norms), else NULL
+    int ld, d, bf16, metric;
+    int64_t n_rows;
+};
+int flat_rows_on_stream(rag_flat_t* h, bool want_norms, hipStream_t st, const char* who,
+                        int (*use)(const FlatRows&, void*), void* ctx);
+// rows of an index without touching the device (argument checks)
+struct FlatShape { int d, bf16, metric; };
+FlatShape flat_shape(const rag_flat_t* h);
+// Device of this process made current for the scope; the caller's comes back behind it.
+class DeviceScope {
+  public:
+    DeviceScope() {
+        if (hipGetDevice(&was_) != hipSuccess) was_ = -1;
+        if (was_ != device_id()) changed_ = hipSetDevice(device_id()) == hipSuccess;
+    }
+    ~DeviceScope() {
+        if (changed_ && was_ >= 0) (void)hipSetDevice(was_);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+
+  private:
+    int was_ = -1;
+    bool changed_ = false;
+};
 // sparse.hip: a begun TF-IDF query (rag_tfidf_query_begin) seen by rag_hybrid_rrf_mmr (cand.hip)
 struct CscBegunView {
     hipStream_t st;                   // the handle's own stream: scoring + selection are enqueued there

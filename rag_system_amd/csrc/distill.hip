@@ -1,0 +1,473 @@
+// distill.hip -- distillation of a ranker's top list over a flat index, forward and backward (rag_flat_distill_dev).
+//
+// Query q_i (d values), rows x_j of the index, beta = 1 / temperature.  Student logits
+//     s_ij = beta <q_i, x_j>  (inner product)     or     -beta ||q_i - x_j||^2  (L2).
+// Teacher: k row numbers t_ik (-1: no entry) with scores z_ik; p_i = softmax(z_i / teacher temperature) over the
+// entries.  P_i = softmax(s_i) over every row of the index ("index") or over the entries of the list ("list").
+//     loss_i = sum_k p_ik (log p_ik - s_i,t_ik) + log sum_j exp(s_ij)
+//     dq_i   = w_i g beta (sum_j P_ij x_j - sum_k p_ik x_t_ik)          g = 1 (inner product), 2 (L2)
+// (L2: the term in q_i has the factor sum_j P_ij - sum_k p_ik = 0.)  Gradient and loss need the same weights of the
+// same rows, so both come out of ONE pass: a running maximum m, the sum l of exp(s - m) and the row sum
+// o = sum_j exp(s_ij - m) x_j, rescaled when m grows.  The index is split over workgroups; a join kernel adds the parts.
+// All sums, statistics and the row sum are fp32; dq is rounded once, to the type of q.
+#include "common.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+namespace {
+
+using namespace rag;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int MAX_LIST = RAG_DISTILL_MAX_K;
+constexpr int THREADS = 256;
+constexpr int WAVES = THREADS / 64;
+
+__device__ __forceinline__ float bf_to_f(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
+// round to nearest even; NaN stays NaN
+__device__ __forceinline__ unsigned short f_to_bf(float f) {
+    const unsigned u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40);
+    return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
+}
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const unsigned short* p) { return bf_to_f(*p); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(unsigned short* p, float v) { *p = f_to_bf(v); }
+
+// A 16-byte piece of a row: E = 4 floats or 8 bfloat16.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ void load(const float* p, float* v) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(p);
+        for (int i = 0; i < 4; ++i) v[i] = t[i];
+    }
+};
+template <> struct Piece<unsigned short> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ void load(const unsigned short* p, float* v) {
+        const u16x8 t = *reinterpret_cast<const u16x8*>(p);
+        for (int i = 0; i < 8; ++i) v[i] = bf_to_f(t[i]);
+    }
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+// over the workgroup, for every thread; `red` holds WAVES floats
+__device__ __forceinline__ float block_sum(float v, float* red) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int w = 0; w < WAVES; ++w) s += red[w];
+    return s;
+}
+__device__ __forceinline__ float block_max(float v, float* red) {
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = red[0];
+    for (int w = 1; w < WAVES; ++w) s = fmaxf(s, red[w]);
+    return s;
+}
+
+struct Call {
+    const void* x;            // rows, n x ld
+    const float* norms;       // L2, over the index
+    long long n, m;
+    int ld, d, k, l2;
+    const void* q;
+    long long ldq;
+    const long long* ids;     // m x k
+    const float* scores;
+    float beta, beta_t;
+    const float* weights;     // m or NULL (1)
+    float* loss;
+    void* dq;                 // m x d or NULL
+    long long lddq;
+    // workspace of the "index" form
+    float* list_part;         // m x ld: sum_k p_k x_k
+    float* list_head;         // m x 2: [0] sum_k p_k (log p_k - s_k); [1] 1, 0 (empty list) or NaN (a bad row number)
+    float* part_ml;           // splits x m x 2: m, l
+    float* part_o;            // splits x m x ld
+    int splits;
+    long long rows_per_split;
+};
+
+// One workgroup per query: the list's entries.  LIST: the whole operator over the list; else list_part / list_head.
+template <typename T, bool LIST>
+__global__ __launch_bounds__(THREADS) void list_kernel(Call c) {
+    constexpr int E = Piece<T>::E;
+    extern __shared__ float sh[];
+    float* qs = sh;               // ld
+    float* s_of = qs + c.ld;      // k
+    float* p_of = s_of + c.k;     // k
+    __shared__ float red[WAVES];
+    const long long i = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const T* x = static_cast<const T*>(c.x);
+    const long long* ids = c.ids + i * c.k;
+    const float* z = c.scores + i * c.k;
+    const T* q = static_cast<const T*>(c.q) + i * c.ldq;
+    for (int j = tid; j < c.ld; j += THREADS) qs[j] = j < c.d ? load1(q + j) : 0.f;
+    float zmax = -INFINITY, any = 0.f, bad = 0.f;
+    for (int k = tid; k < c.k; k += THREADS) {
+        const long long id = ids[k];
+        if (id < -1 || id >= c.n) bad = 1.f;
+        else if (id >= 0) {
+            const float v = z[k] * c.beta_t;
+            zmax = fmaxf(zmax, v);
+            if (!(v == -INFINITY)) any = 1.f;
+        }
+    }
+    zmax = block_max(zmax, red);
+    any = block_max(any, red);
+    bad = block_max(bad, red);
+    if (bad != 0.f || any == 0.f) {       // (uniform) nothing to learn from, or a row number outside the index
+        const float v = bad != 0.f ? NAN : 0.f;
+        if (LIST) {
+            if (tid == 0) c.loss[i] = v;
+            if (c.dq)
+                for (int j = tid; j < c.d; j += THREADS) store1(static_cast<T*>(c.dq) + i * c.lddq + j, v);
+        } else if (tid == 0) {
+            c.list_head[2 * i] = v;
+            c.list_head[2 * i + 1] = v;
+        }
+        return;
+    }
+    float zsum = 0.f;
+    for (int k = tid; k < c.k; k += THREADS)
+        if (ids[k] >= 0) zsum += expf(z[k] * c.beta_t - zmax);
+    zsum = block_sum(zsum, red);          // (its barriers also publish qs)
+    for (int k = wave; k < c.k; k += WAVES) {
+        const long long id = ids[k];
+        if (id < 0) continue;
+        const T* row = x + id * c.ld;
+        float acc = 0.f;
+        for (int j = lane * E; j < c.ld; j += 64 * E) {
+            float v[E];
+            Piece<T>::load(row + j, v);
+            for (int e = 0; e < E; ++e) {
+                if (c.l2) {
+                    const float t = qs[j + e] - v[e];
+                    acc = fmaf(t, t, acc);
+                } else {
+                    acc = fmaf(qs[j + e], v[e], acc);
+                }
+            }
+        }
+        acc = wave_sum(acc);
+        if (lane == 0) s_of[k] = c.l2 ? -c.beta * acc : c.beta * acc;
+    }
+    __syncthreads();
+    float smax = -INFINITY;
+    for (int k = tid; k < c.k; k += THREADS)
+        if (ids[k] >= 0) smax = fmaxf(smax, s_of[k]);
+    smax = block_max(smax, red);
+    const float log_zsum = logf(zsum);
+    float head = 0.f, mass = 0.f;
+    for (int k = tid; k < c.k; k += THREADS) {
+        float p = 0.f;
+        if (ids[k] >= 0) {
+            const float a = z[k] * c.beta_t - zmax;
+            p = expf(a) / zsum;
+            if (p != 0.f) head += p * (a - log_zsum - s_of[k]);   // (NaN enters)
+            mass += expf(s_of[k] - smax);
+        }
+        p_of[k] = p;
+    }
+    head = block_sum(head, red);
+    mass = block_sum(mass, red);
+    if (LIST) {
+        if (tid == 0) c.loss[i] = head + smax + logf(mass);
+        if (!c.dq) return;
+        for (int k = tid; k < c.k; k += THREADS)
+            if (ids[k] >= 0) p_of[k] = expf(s_of[k] - smax) / mass - p_of[k];
+        __syncthreads();
+    } else {
+        if (tid == 0) {
+            c.list_head[2 * i] = head;
+            c.list_head[2 * i + 1] = 1.f;
+        }
+        if (!c.dq) return;
+    }
+    const float f = LIST ? (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f) : 1.f;
+    for (int j = tid * E; j < c.ld; j += THREADS * E) {
+        float acc[E] = {};
+        for (int k = 0; k < c.k; ++k) {
+            const long long id = ids[k];
+            if (id < 0) continue;
+            float v[E];
+            Piece<T>::load(x + id * c.ld + j, v);
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(p_of[k], v[e], acc[e]);
+        }
+        for (int e = 0; e < E; ++e) {
+            if (!LIST) c.list_part[i * c.ld + j + e] = acc[e];
+            else if (j + e < c.d) store1(static_cast<T*>(c.dq) + i * c.lddq + j + e, f * acc[e]);
+        }
+    }
+}
+
+// Any row length: one workgroup per (split of the rows, query), 32 rows at a time; a wave computes eight dot products,
+// then every thread adds its columns of the 32 rows.
+constexpr int ANY_ROWS = 32;
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
+    constexpr int E = Piece<T>::E, COLS = (8192 / E + THREADS - 1) / THREADS;
+    extern __shared__ float qs[];   // ld
+    __shared__ float s_of[ANY_ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const long long i = blockIdx.y, r0 = blockIdx.x * c.rows_per_split, r1 = min(c.n, r0 + c.rows_per_split);
+    const T* x = static_cast<const T*>(c.x);
+    const T* q = static_cast<const T*>(c.q) + i * c.ldq;
+    for (int j = tid; j < c.ld; j += THREADS) qs[j] = j < c.d ? load1(q + j) : 0.f;
+    __syncthreads();
+    float m = -INFINITY, l = 0.f, o[COLS][E] = {};
+    for (long long r = r0; r < r1; r += ANY_ROWS) {
+        for (int a = wave; a < ANY_ROWS; a += WAVES) {
+            float acc = 0.f;
+            if (r + a < r1) {
+                const T* row = x + (r + a) * c.ld;
+                for (int j = lane * E; j < c.ld; j += 64 * E) {
+                    float v[E];
+                    Piece<T>::load(row + j, v);
+                    for (int e = 0; e < E; ++e) acc = fmaf(qs[j + e], v[e], acc);
+                }
+                acc = wave_sum(acc);
+                acc = c.beta * (c.l2 ? 2.f * acc - c.norms[r + a] : acc);
+            } else {
+                acc = -INFINITY;
+            }
+            if (lane == 0) s_of[a] = acc;
+        }
+        __syncthreads();
+        float t = m;
+        for (int a = 0; a < ANY_ROWS; ++a) t = fmaxf(t, s_of[a]);
+        const float scale = t == -INFINITY ? 1.f : expf(m - t);
+        m = t;
+        l *= scale;
+        if (GRAD)
+            for (int b = 0; b < COLS; ++b)
+                for (int e = 0; e < E; ++e) o[b][e] *= scale;
+        for (int a = 0; a < ANY_ROWS && r + a < r1; ++a) {
+            const float p = s_of[a] == -INFINITY ? 0.f : expf(s_of[a] - m);
+            l += p;
+            if (!GRAD) continue;
+            for (int b = 0; b < COLS; ++b) {
+                const int j = (b * THREADS + tid) * E;
+                if (j >= c.ld) break;
+                float v[E];
+                Piece<T>::load(x + (r + a) * c.ld + j, v);
+                for (int e = 0; e < E; ++e) o[b][e] = fmaf(p, v[e], o[b][e]);
+            }
+        }
+        __syncthreads();
+    }
+    const long long at = blockIdx.x * c.m + i;
+    if (tid == 0) {
+        c.part_ml[2 * at] = m;
+        c.part_ml[2 * at + 1] = l;
+    }
+    if (!GRAD) return;
+    for (int b = 0; b < COLS; ++b) {
+        const int j = (b * THREADS + tid) * E;
+        if (j < c.ld)
+            for (int e = 0; e < E; ++e) c.part_o[at * c.ld + j + e] = o[b][e];
+    }
+}
+
+// Adds the splits' parts: one workgroup per query.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void join_kernel(Call c) {
+    extern __shared__ float w_of[];   // splits
+    __shared__ float red[WAVES];
+    const long long i = blockIdx.x;
+    const int tid = threadIdx.x;
+    T* dq = c.dq ? static_cast<T*>(c.dq) + i * c.lddq : nullptr;
+    const float live = c.list_head[2 * i + 1];
+    if (!(live == 1.f)) {
+        if (tid == 0) c.loss[i] = live;
+        if (dq)
+            for (int j = tid; j < c.d; j += THREADS) store1(dq + j, live);
+        return;
+    }
+    float m = -INFINITY;
+    for (int s = tid; s < c.splits; s += THREADS) m = fmaxf(m, c.part_ml[2 * (s * c.m + i)]);
+    m = block_max(m, red);
+    float l = 0.f;
+    for (int s = tid; s < c.splits; s += THREADS) {
+        const float ms = c.part_ml[2 * (s * c.m + i)];
+        const float w = ms == -INFINITY ? 0.f : expf(ms - m);
+        w_of[s] = w;
+        const float ls = c.part_ml[2 * (s * c.m + i) + 1];
+        l += w == 0.f && !(ls != ls) ? 0.f : w * ls;
+    }
+    l = block_sum(l, red);
+    float qq = 0.f;
+    if (c.l2) {
+        const T* q = static_cast<const T*>(c.q) + i * c.ldq;
+        for (int j = tid; j < c.d; j += THREADS) qq = fmaf(load1(q + j), load1(q + j), qq);
+        qq = block_sum(qq, red);
+    }
+    if (tid == 0) c.loss[i] = c.list_head[2 * i] + (m - c.beta * qq) + logf(l);
+    if (!dq) return;
+    const float f = (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f);
+    for (int j = tid; j < c.d; j += THREADS) {
+        float o = 0.f;
+        for (int s = 0; s < c.splits; ++s) o = fmaf(w_of[s], c.part_o[(s * c.m + i) * c.ld + j], o);
+        store1(dq + j, f * (o / l - c.list_part[i * c.ld + j]));
+    }
+}
+
+// How a call is split; depends on the number of queries and the row length, not on the number of rows (the
+// workspace may be allocated before rows are added).
+struct Plan {
+    int splits;
+    size_t head_off, list_off, ml_off, o_off, bytes;
+};
+
+int elem_ld(int d, int bf16) { return bf16 ? (d + 7) & ~7 : (d + 3) & ~3; }
+
+Plan make_plan(long long m, int d, int bf16, int over, bool grad) {
+    Plan p{};
+    if (over == RAG_OVER_LIST || m == 0) return p;
+    const size_t ld = elem_ld(d, bf16);
+    p.splits = (int)std::max<long long>(1, std::min<long long>(1024, 2048 / m));
+    auto take = [&](size_t floats) {
+        const size_t at = p.bytes;
+        p.bytes += (floats * sizeof(float) + 255) & ~(size_t)255;
+        return at;
+    };
+    p.head_off = take(2 * m);
+    p.list_off = take(grad ? m * ld : 0);
+    p.ml_off = take((size_t)p.splits * m * 2);
+    p.o_off = take(grad ? (size_t)p.splits * m * ld : 0);
+    return p;
+}
+
+struct Ctx {
+    Call c;
+    Plan p;
+    int over;
+    char* ws;
+    hipStream_t st;
+};
+
+template <typename T>
+int launch(Ctx& x) {
+    Call& c = x.c;
+    const size_t list_lds = ((size_t)c.ld + 2 * c.k) * sizeof(float);
+    if (x.over == RAG_OVER_LIST) {
+        list_kernel<T, true><<<(unsigned)c.m, THREADS, list_lds, x.st>>>(c);
+        RAG_HIP(hipGetLastError());
+        return RAG_OK;
+    }
+    c.splits = x.p.splits;
+    c.rows_per_split = std::max<long long>(ANY_ROWS, (c.n + c.splits - 1) / c.splits);
+    c.list_head = reinterpret_cast<float*>(x.ws + x.p.head_off);
+    c.list_part = reinterpret_cast<float*>(x.ws + x.p.list_off);
+    c.part_ml = reinterpret_cast<float*>(x.ws + x.p.ml_off);
+    c.part_o = reinterpret_cast<float*>(x.ws + x.p.o_off);
+    list_kernel<T, false><<<(unsigned)c.m, THREADS, list_lds, x.st>>>(c);
+    RAG_HIP(hipGetLastError());
+    const dim3 grid((unsigned)c.splits, (unsigned)c.m);
+    if (c.dq) index_any_kernel<T, true><<<grid, THREADS, c.ld * sizeof(float), x.st>>>(c);
+    else index_any_kernel<T, false><<<grid, THREADS, c.ld * sizeof(float), x.st>>>(c);
+    RAG_HIP(hipGetLastError());
+    join_kernel<T><<<(unsigned)c.m, THREADS, c.splits * sizeof(float), x.st>>>(c);
+    RAG_HIP(hipGetLastError());
+    return RAG_OK;
+}
+
+int with_rows(const FlatRows& r, void* ctx) {
+    Ctx& x = *static_cast<Ctx*>(ctx);
+    x.c.x = r.arena;
+    x.c.norms = r.norms;
+    x.c.n = r.n_rows;
+    x.c.ld = r.ld;
+    x.c.d = r.d;
+    x.c.l2 = r.metric == RAG_METRIC_L2;
+    return r.bf16 ? launch<unsigned short>(x) : launch<float>(x);
+}
+
+int check_shape(const char* who, rag_flat_t* h, int64_t nq, int k, int over) {
+    if (!h) return fail(RAG_ERR_INVALID_ARG, "%s: bad handle", who);
+    if (nq < 0 || nq > RAG_DISTILL_MAX_NQ)
+        return fail(RAG_ERR_INVALID_ARG, "%s: nq=%lld out of range [0,%d]", who, (long long)nq, RAG_DISTILL_MAX_NQ);
+    if (k < 0 || k > RAG_DISTILL_MAX_K)
+        return fail(RAG_ERR_INVALID_ARG, "%s: k=%d out of range [0,%d]", who, k, RAG_DISTILL_MAX_K);
+    if (over != RAG_OVER_INDEX && over != RAG_OVER_LIST)
+        return fail(RAG_ERR_INVALID_ARG, "%s: over=%d is neither RAG_OVER_INDEX(0) nor RAG_OVER_LIST(1)", who, over);
+    return RAG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rag_flat_distill_ws_bytes(rag_flat_t* h, int64_t nq, int k, int over, int want_grad, int64_t* bytes) {
+    RAG_REQUIRE_INIT();
+    const int rc = check_shape("rag_flat_distill_ws_bytes", h, nq, k, over);
+    if (rc) return rc;
+    if (!bytes) return fail(RAG_ERR_INVALID_ARG, "rag_flat_distill_ws_bytes: bytes is NULL");
+    const FlatShape s = flat_shape(h);
+    *bytes = (int64_t)make_plan(nq, s.d, s.bf16, over, want_grad != 0).bytes;
+    return RAG_OK;
+}
+
+int rag_flat_distill_dev(rag_flat_t* h, int64_t nq, const void* q_dev, int64_t ldq, int k, const int64_t* ids_dev,
+                         const float* scores_dev, double temperature, double teacher_temperature, int over,
+                         const float* weights_dev, float* loss_dev, void* dq_dev, int64_t lddq, void* ws_dev,
+                         int64_t ws_bytes, void* stream) {
+    const char* who = "rag_flat_distill_dev";
+    RAG_REQUIRE_INIT();
+    int rc = check_shape(who, h, nq, k, over);
+    if (rc) return rc;
+    if (!(temperature > 0) || !(teacher_temperature > 0) || !std::isfinite(temperature) || !std::isfinite(teacher_temperature) ||
+        !std::isfinite((float)(1.0 / temperature)) || !std::isfinite((float)(1.0 / teacher_temperature)))
+        return fail(RAG_ERR_INVALID_ARG, "%s: temperatures must be positive and finite (%g, %g)", who, temperature,
+                    teacher_temperature);
+    if (nq == 0) return RAG_OK;
+    const FlatShape s = flat_shape(h);
+    if (!q_dev || !loss_dev || (k > 0 && (!ids_dev || !scores_dev)))
+        return fail(RAG_ERR_INVALID_ARG, "%s: NULL buffer", who);
+    if (ldq < s.d || (dq_dev && lddq < s.d))
+        return fail(RAG_ERR_INVALID_ARG, "%s: row strides %lld / %lld are below d=%d", who, (long long)ldq, (long long)lddq, s.d);
+    Ctx x{};
+    x.p = make_plan(nq, s.d, s.bf16, over, dq_dev != nullptr);
+    if (x.p.bytes > 0 && (!ws_dev || ws_bytes < (int64_t)x.p.bytes || ((uintptr_t)ws_dev & 255)))
+        return fail(RAG_ERR_INVALID_ARG, "%s: needs a workspace of %lld bytes, aligned to 256 (rag_flat_distill_ws_bytes)", who,
+                    (long long)x.p.bytes);
+    x.over = over;
+    x.ws = static_cast<char*>(ws_dev);
+    x.st = (hipStream_t)stream;
+    x.c.m = nq;
+    x.c.k = k;
+    x.c.q = q_dev;
+    x.c.ldq = ldq;
+    x.c.ids = reinterpret_cast<const long long*>(ids_dev);
+    x.c.scores = scores_dev;
+    x.c.beta = (float)(1.0 / temperature);
+    x.c.beta_t = (float)(1.0 / teacher_temperature);
+    x.c.weights = weights_dev;
+    x.c.loss = loss_dev;
+    x.c.dq = dq_dev;
+    x.c.lddq = lddq;
+    DeviceScope dev;
+    return flat_rows_on_stream(h, s.metric == RAG_METRIC_L2 && over == RAG_OVER_INDEX, x.st, who, with_rows, &x);
+}
+
+}  // extern "C"

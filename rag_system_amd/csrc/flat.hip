@@ -858,6 +858,9 @@ struct rag_flat {
     float* zero16 = nullptr;                           // 64 B of zeros (MFMA tile padding source)
     float* xnorm = nullptr;  int64_t xnorm_cap = 0;    // ||x||^2 per row (L2, MFMA path), lazily filled
     int64_t norm_valid = 0;
+    int64_t norm_done = 0;                             // ... of which the device is known to have finished (flat_rows_on_stream)
+    bool captured = false;                             // a captured graph names x / xnorm: replaced arrays go to `retired`
+    std::vector<void*> retired;
     float* ws_hq = nullptr;  int64_t ws_hq_cap = 0;    // host-variant device copies
     float* ws_D = nullptr; long long* ws_I = nullptr; int64_t ws_out_cap = 0;
     char* pin = nullptr; size_t pin_cap = 0;            // pinned staging of the host variant (small batches)
@@ -906,7 +909,8 @@ int ensure_capacity(rag_flat* h, int64_t rows) {
     if (h->ndev > 0)
         RAG_HIP(hipMemcpyAsync(nx, h->x, (size_t)h->ndev * rb, hipMemcpyDeviceToDevice, st));
     RAG_HIP(hipStreamSynchronize(st));
-    if (h->x) RAG_HIP(hipFree(h->x));
+    if (h->x && h->captured) h->retired.push_back(h->x);
+    else if (h->x) RAG_HIP(hipFree(h->x));
     h->x = nx;
     h->cap = want;
     return RAG_OK;
@@ -1118,7 +1122,8 @@ int ensure_norm_array(rag_flat* h, hipStream_t st) {
     if (h->norm_valid > 0)
         RAG_HIP(hipMemcpyAsync(nn, h->xnorm, (size_t)h->norm_valid * sizeof(float), hipMemcpyDeviceToDevice, st));
     RAG_HIP(hipStreamSynchronize(st));
-    if (h->xnorm) RAG_HIP(hipFree(h->xnorm));
+    if (h->xnorm && h->captured) h->retired.push_back(h->xnorm);
+    else if (h->xnorm) RAG_HIP(hipFree(h->xnorm));
     h->xnorm = nn;
     h->xnorm_cap = h->cap;
     return RAG_OK;
@@ -1694,6 +1699,44 @@ int flat_with_view(rag_flat_t* h, int (*use)(const FlatView&, void*), void* ctx)
     const FlatView v{h->x, h->ld, h->d, h->dtype == RAG_DTYPE_BF16 ? 1 : 0, h->ndev};
     return use(v, ctx);
 }
+FlatShape flat_shape(const rag_flat_t* h) { return FlatShape{h->d, h->dtype == RAG_DTYPE_BF16 ? 1 : 0, h->metric}; }
+
+int flat_rows_on_stream(rag_flat_t* h, bool want_norms, hipStream_t st, const char* who,
+                        int (*use)(const FlatRows&, void*), void* ctx) {
+    std::lock_guard<std::mutex> lk(h->mu);
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &cs) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(RAG_ERR_UNSUPPORTED, "%s: the null stream cannot be used while another stream is captured", who);
+    }
+    if (cs != hipStreamCaptureStatusNone) {
+        if (!h->staged.empty())
+            return fail(RAG_ERR_UNSUPPORTED, "%s under capture: %lld added rows are still staged on the host; call once "
+                        "before the capture", who, (long long)(h->staged.size() / h->d));
+        if (want_norms && h->norm_done < h->ndev)
+            return fail(RAG_ERR_UNSUPPORTED, "%s under capture: the norms of %lld rows are not computed yet; call once "
+                        "before the capture", who, (long long)(h->ndev - h->norm_done));
+        h->captured = true;
+    } else {
+        int rc = flush_staged(h);
+        if (rc) return rc;
+        if (want_norms && h->norm_done < h->ndev) {
+            rc = ensure_norm_array(h, lib_stream());
+            if (rc) return rc;
+            if (h->norm_valid < h->ndev) {
+                rc = mfma_row_norms(h->x, h->ld, h->dtype == RAG_DTYPE_BF16, h->norm_valid, h->ndev - h->norm_valid,
+                                    h->xnorm, lib_stream());
+                if (rc) return rc;
+            }
+            RAG_HIP(hipDeviceSynchronize());  // once per add: also what a search began on a stream of its own
+            h->norm_valid = h->norm_done = h->ndev;
+        }
+    }
+    const FlatRows v{h->x, want_norms ? h->xnorm : nullptr, h->ld, h->d, h->dtype == RAG_DTYPE_BF16 ? 1 : 0, h->metric,
+                     h->ndev};
+    return use(v, ctx);
+}
+
 // Called by rag_init() with the selected device current, once per process (one process per GPU).
 int flat_init_scratch() {
     int dev = -1;
@@ -1764,6 +1807,7 @@ void rag_flat_free(rag_flat_t* h) {
         (void)hipFree(h->ws_fk);
         (void)hipFree(h->ws_fi);
         (void)hipFree(h->xnorm);
+        for (void* p : h->retired) (void)hipFree(p);
         (void)hipFree(h->ws_D);
         (void)hipFree(h->ws_I);
         if (h->pin) (void)hipHostFree(h->pin);
@@ -1902,6 +1946,7 @@ int rag_flat_reset(rag_flat_t* h) {
     h->ntotal = 0;
     h->ndev = 0;
     h->norm_valid = 0;
+    h->norm_done = 0;
     if (h->shadow) {  // refilled from row 0 by the next search (sync_shadow)
         h->shadow->ntotal = h->shadow->ndev = 0;
         h->shadow->norm_valid = 0;

@@ -18,7 +18,7 @@ import threading
 
 import numpy as np
 
-from . import _lib
+from . import _lib, device_tensors as dt
 
 METRIC_INNER_PRODUCT = 0
 METRIC_L2 = 1
@@ -51,6 +51,27 @@ class _HipFlatBackend:
 
     def add(self, x):
         _lib.check(self._lib.rag_flat_add(self._h, x.shape[0], _lib.ptr(x)), self._lib)
+
+    def add_dev(self, x):
+        """x: contiguous float32 torch tensor in HBM; on torch's current stream, complete on return."""
+        _lib.check(self._lib.rag_flat_add_dev(self._h, x.shape[0], C.c_void_p(x.data_ptr()), C.c_void_p(dt.stream_of(x))),
+                   self._lib)
+
+    def distill(self, q, ids, scores, temperature, teacher_temperature, over, weights, grad):
+        import torch
+        q, ldq = dt.rows(q)
+        nq, k = ids.shape
+        need = C.c_int64()
+        _lib.check(self._lib.rag_flat_distill_ws_bytes(self._h, nq, k, over, 1 if grad else 0, C.byref(need)), self._lib)
+        loss = torch.empty(nq, dtype=torch.float32, device=q.device)
+        dq = torch.empty((nq, self.d), dtype=q.dtype, device=q.device) if grad else None
+        ws = dt.workspace(need.value, q)
+        _lib.check(self._lib.rag_flat_distill_dev(
+            self._h, nq, C.c_void_p(q.data_ptr()), ldq, k, C.c_void_p(ids.data_ptr()), C.c_void_p(scores.data_ptr()),
+            float(temperature), float(teacher_temperature), over, C.c_void_p(None if weights is None else weights.data_ptr()),
+            C.c_void_p(loss.data_ptr()), C.c_void_p(dq.data_ptr() if grad else None), self.d, C.c_void_p(ws.data_ptr()),
+            need.value, C.c_void_p(dt.stream_of(q))), self._lib)
+        return loss, dq
 
     def add_synthetic(self, n, seed, first_global_row):
         _lib.check(self._lib.rag_flat_add_synthetic(self._h, int(n), int(seed), int(first_global_row)), self._lib)
@@ -156,11 +177,52 @@ class IndexFlat:
         return self._b.ntotal
 
     def add(self, x):
+        """x: (n, d) float32 rows; a torch tensor in GPU memory (float32 or bfloat16) is added without a trip over the host."""
+        if dt.is_tensor(x):
+            import torch
+            dt.engine_for(x, "x")
+            if x.dim() != 2 or x.shape[1] != self.d or x.dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError("add expects a (n, %d) float32 or bfloat16 tensor, got %s of %s"
+                                 % (self.d, tuple(x.shape), x.dtype))
+            for part in torch.split(x.detach(), max(1, (1 << 28) // self.d)) if x.shape[0] else ():
+                self._b.add_dev(part.float().contiguous())
+            return
         x = np.ascontiguousarray(x, dtype=np.float32)
         if x.ndim != 2 or x.shape[1] != self.d:
             raise ValueError("add expects a (n, %d) float32 array, got %s" % (self.d, x.shape))
         if x.shape[0]:
             self._b.add(x)
+
+    def distill(self, q, ids, scores, temperature=0.05, teacher_temperature=1.0, over="index", weights=None, grad=True):
+        """Distillation of a ranker's top list into the queries, forward and backward (not in faiss; rag_flat_distill_dev).
+
+        q: (nq, d) in HBM, of the index' storage type (float32 / bfloat16): what a trained projection makes of the
+        model's vectors.  ids (int64) and scores (float32), (nq, k): the rows a teacher has scored per query, -1 = no
+        entry, as search() returns them.  Student logits are the index' scores / temperature (L2: minus the squared
+        distance), the teacher's probabilities softmax(scores / teacher_temperature) over its list:
+
+            loss_i = KL(teacher_i || student_i),  student = softmax over EVERY row (over="index") or the list ("list")
+            dq_i   = weights_i * d loss_i / d q_i
+
+        Returns (loss float32 (nq), dq of q's type, or None with grad=False).  One pass over the rows gives both; they
+        carry no autograd history: y.backward(dq), or adapters.QueryAdapters.grad(x, slots, dq).  A query without an
+        entry has loss 0 and dq 0, one with a row number outside the index NaN.  On torch's current stream; may be
+        captured into a graph behind any one call."""
+        import torch
+        if over not in ("index", "list"):
+            raise ValueError("over must be 'index' or 'list', got %r" % (over,))
+        if not hasattr(self._b, "distill"):
+            raise NotImplementedError("this index' backend has no distill()")
+        dt.engine_for(q, "q")
+        dt.check(q, "q", torch.bfloat16 if self.storage == "bf16" else torch.float32, (None, self.d))
+        nq = q.shape[0]
+        dt.check(ids, "ids", torch.int64, (nq, None), q)
+        dt.check(scores, "scores", torch.float32, tuple(ids.shape), q)
+        if weights is not None:
+            dt.check(weights, "weights", torch.float32, (nq,), q)
+            weights = weights.detach().contiguous()
+        return self._b.distill(q.detach(), ids.contiguous(), scores.detach().contiguous(), temperature, teacher_temperature,
+                               _lib.OVER_INDEX if over == "index" else _lib.OVER_LIST, weights, bool(grad))
 
     def search(self, x, k):
         x = np.ascontiguousarray(x, dtype=np.float32)

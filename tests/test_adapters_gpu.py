@@ -1,0 +1,257 @@
+"""adapters.QueryAdapters (rag_adapter_apply_dev, rag_adapter_grad_dev) against the formulas in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from _operators import adapters_grad_ref, adapters_ref, assert_within
+from rag_system_amd import _lib
+from rag_system_amd.adapters import QueryAdapters
+
+pytestmark = pytest.mark.gpu
+TYPE = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def make(n, d_in, d_out, S, R, dtype="f32", seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed * 1000 + n + 3 * d_in + 5 * d_out + 7 * S + R)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")     # noqa: E731
+    t = TYPE[dtype]
+    x, dy = r(n, d_in).to(t), r(n, d_out).to(t)
+    bank = QueryAdapters((r(d_out, d_in) * d_in ** -0.5).to(t), (r(S, R, d_in) * d_in ** -0.5).to(t),
+                         (r(S, d_out, R) * R ** -0.5).to(t), r(S))
+    slots = torch.randint(-1, S, (n,), generator=g, device="cuda")
+    return bank, x, slots, dy
+
+
+def refs(bank, x, slots, dy):
+    w = (bank.weight, bank.A, bank.B, bank.scale, slots.tolist())
+    return adapters_ref(x, *w), adapters_grad_ref(x, *w, dy)
+
+
+def check(bank, x, slots, dy):
+    (y_ref, y_allow), g_ref = refs(bank, x, slots, dy)
+    y = bank.apply(x, slots)
+    assert y.dtype == x.dtype
+    assert_within(y, y_ref, y_allow, "y")
+    dx, dA, dB = bank.grad(x, slots, dy)
+    assert dx.dtype == x.dtype and dA.dtype == dB.dtype == torch.float32
+    for name, got in (("dx", dx), ("dA", dA), ("dB", dB)):
+        assert_within(got, *g_ref[name], name)
+    return y, dx, dA, dB
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,d_in,d_out,S,R", [
+    (1, 1, 1, 1, 1), (1, 384, 384, 8, 16), (2, 5, 3, 2, 3), (1, 768, 384, 3, 64), (7, 33, 65, 4, 8), (15, 64, 64, 40, 4),
+    (16, 128, 128, 1, 16), (17, 100, 130, 5, 17), (33, 387, 129, 2, 12), (64, 256, 192, 64, 16), (65, 130, 260, 7, 33),
+    (129, 96, 384, 9, 5), (300, 200, 70, 3, 128), (511, 64, 40, 300, 2), (1000, 130, 66, 11, 9)])
+def test_small(n, d_in, d_out, S, R, dtype):
+    check(*make(n, d_in, d_out, S, R, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_wide(dtype):
+    check(*make(20, 2050, 1030, 3, 20, dtype))
+    check(*make(3, 8192, 16, 2, 4, dtype))
+    check(*make(3, 16, 8192, 2, 4, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how", ["one slot", "none", "sorted", "last slot only", "each its own"])
+def test_slot_patterns(how, dtype):
+    n, S = 200, 200
+    bank, x, slots, dy = make(n, 96, 80, S, 8, dtype, seed=2)
+    slots = {"one slot": torch.full((n,), 3), "none": torch.full((n,), -1), "sorted": torch.arange(n) // 7,
+             "last slot only": torch.where(torch.arange(n) == n - 1, S - 1, -1), "each its own": torch.randperm(n)}[how].cuda()
+    y, dx, dA, dB = check(bank, x, slots, dy)
+    met = torch.zeros(S, dtype=torch.bool, device="cuda")
+    met[slots[slots >= 0]] = True
+    assert not dA[~met].any() and not dB[~met].any()
+
+
+def test_long_batch():
+    """More requests than any tile or split holds, a few slots with nearly all of them."""
+    n, S = 40007, 5
+    bank, x, slots, dy = make(n, 24, 20, S, 6, seed=3)
+    slots = torch.where(torch.rand(n, device="cuda") < 0.9, 2, slots)
+    w = [t.double() for t in (bank.weight, bank.A, bank.B, bank.scale)]
+    dx, dA, dB = bank.grad(x, slots, dy)
+    y = bank.apply(x, slots)
+    xd, dyd = x.double(), dy.double()
+    for s in range(-1, S):
+        m = slots == s
+        e = w[0] if s < 0 else w[0] + w[3][s] * w[2][s] @ w[1][s]
+        mag = (w[0].abs() if s < 0 else w[0].abs() + w[3][s].abs() * w[2][s].abs() @ w[1][s].abs())
+        u = 2.0 ** -24
+        assert_within(y[m].cpu(), (xd[m] @ e.t()).cpu(), ((2 * 24 + 12) * u * (xd[m].abs() @ mag.t())).cpu(), "y")
+        assert_within(dx[m].cpu(), (dyd[m] @ e).cpu(), ((2 * 20 + 12) * u * (dyd[m].abs() @ mag)).cpu(), "dx")
+        if s >= 0:
+            outer, am = dyd[m].t() @ xd[m], dyd[m].abs().t() @ xd[m].abs()
+            c, k = w[3][s], int(m.sum()) + 30
+            assert_within(dA[s].cpu(), (c * w[2][s].t() @ outer).cpu(), (k * u * c.abs() * w[2][s].abs().t() @ am).cpu(), "dA")
+            assert_within(dB[s].cpu(), (c * outer @ w[1][s].t()).cpu(), (k * u * c.abs() * am @ w[1][s].abs().t()).cpu(), "dB")
+
+
+def test_slots_outside_the_bank():
+    bank, x, slots, dy = make(20, 40, 30, 4, 5, seed=4)
+    want = check(bank, x, slots.clamp(min=0), dy)                      # noqa: F841
+    s2 = slots.clamp(min=0).clone()
+    s2[3], s2[11], s2[12] = 4, -2, 1 << 40
+    out = [3, 11, 12]
+    keep = [i for i in range(20) if i not in out]
+    y = bank.apply(x, s2)
+    dx, dA, dB = bank.grad(x, s2, dy)
+    assert torch.isnan(y[out]).all() and torch.isnan(dx[out]).all()
+    s3 = s2.clone()
+    s3[out] = -1
+    assert torch.equal(y[keep], bank.apply(x, s3)[keep])
+    _, g = refs(bank, x, s3, dy)
+    assert_within(dA, *g["dA"], "dA")
+    assert_within(dB, *g["dB"], "dB")
+    assert torch.isfinite(dx[keep]).all()
+
+
+def test_values_of_other_requests_do_not_leak():
+    """An infinite or NaN embedding stays in its own row (and its own slot's gradients)."""
+    for n in (5, 70, 300):
+        bank, x, slots, dy = make(n, 64, 48, 3, 6, seed=5)
+        slots = torch.arange(n, device="cuda") % 3 - 1
+        x[1], dy[1] = float("nan"), float("inf")        # slot 0
+        y, (dx, dA, dB) = bank.apply(x, slots), bank.grad(x, slots, dy)
+        rest = [i for i in range(n) if i != 1]
+        assert torch.isfinite(y[rest]).all() and torch.isfinite(dx[rest]).all()
+        assert torch.isfinite(dA[1:]).all() and torch.isfinite(dB[1:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 9, 150])
+def test_strides_and_alignment(dtype, n):
+    bank, x, slots, dy = make(n, 64, 72, 4, 8, dtype, seed=6)
+    y, (dx, dA, dB) = bank.apply(x, slots), bank.grad(x, slots, dy)
+    wide = torch.zeros(n, 203, dtype=x.dtype, device="cuda")
+    wide[:, 1:65], wide[:, 101:173] = x, dy
+    for xs, dys in ((wide[:, 1:65], wide[:, 101:173]), (x.t().contiguous().t(), dy.t().contiguous().t())):
+        (y_ref, y_allow), g = refs(bank, x, slots, dy)
+        assert_within(bank.apply(xs, slots), y_ref, y_allow)
+        for name, got in zip(("dx", "dA", "dB"), bank.grad(xs, slots, dys)):
+            assert_within(got, *g[name], name)
+    one = x[:1].expand(n, 64)                          # every request the same vector
+    assert_within(bank.apply(one, slots), *adapters_ref(one, bank.weight, bank.A, bank.B, bank.scale, slots.tolist()))
+    assert torch.equal(bank.apply(x, slots.int()), y)
+
+
+def test_input_grad_is_optional():
+    bank, x, slots, dy = make(50, 64, 72, 4, 8)
+    dx, dA, dB = bank.grad(x, slots, dy)
+    none, dA2, dB2 = bank.grad(x, slots, dy, input_grad=False)
+    assert none is None and torch.equal(dA, dA2) and torch.equal(dB, dB2)
+
+
+def test_no_requests():
+    bank, x, slots, dy = make(3, 8, 9, 2, 4)
+    assert bank.apply(x[:0], slots[:0]).shape == (0, 9)
+    dx, dA, dB = bank.grad(x[:0], slots[:0], dy[:0])
+    assert dx.shape == (0, 8) and not dA.any() and not dB.any()
+
+
+def test_gradient_against_differences():
+    """Differences of sum(y * dy) in 64 bits are exact along a direction (y is linear in x, in A and in B)."""
+    bank, x, slots, dy = make(30, 40, 24, 3, 6, seed=7)
+    dx, dA, dB = (t.double().cpu() for t in bank.grad(x, slots, dy))
+    ls = slots.tolist()
+    f = lambda **kw: float((adapters_ref(kw.get("x", x), bank.weight, kw.get("A", bank.A), kw.get("B", bank.B),    # noqa: E731
+                                         bank.scale, ls)[0] * dy.double().cpu()).sum())
+    for name, t, got in (("x", x, dx), ("A", bank.A, dA), ("B", bank.B, dB)):
+        v = torch.randn_like(t)
+        a, b = t.double() + 0.5 * v.double(), t.double() - 0.5 * v.double()
+        diff, mine = f(**{name: a}) - f(**{name: b}), float((got * v.double().cpu()).sum())
+        assert abs(diff - mine) < 2e-5 * float((got * v.double().cpu()).abs().sum())
+
+
+def test_same_call_same_bits():
+    for n, S in ((1, 2), (64, 5), (3000, 3)):
+        bank, x, slots, dy = make(n, 128, 96, S, 16, seed=8)
+        a, b = bank.grad(x, slots, dy), bank.grad(x, slots, dy)
+        assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(bank.apply(x, slots), bank.apply(x, slots))
+
+
+@pytest.mark.parametrize("n", [1, 40, 2000])
+def test_graph_replays(n):
+    bank, x, slots, dy = make(n, 96, 64, 5, 8, seed=9)
+    bank.apply(x, slots), bank.grad(x, slots, dy)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = (bank.apply(x, slots),) + bank.grad(x, slots, dy)
+        graphs.append((g, out))
+    for it in range(4):
+        x.copy_(torch.randn_like(x))
+        slots.copy_(torch.randint(-1, 5, slots.shape, device="cuda"))
+        bank.A.add_(0.1)
+        for g, _ in graphs:
+            g.replay()
+        want = (bank.apply(x, slots),) + bank.grad(x, slots, dy)
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want)), it
+
+
+def test_other_streams():
+    bank, x, slots, dy = make(500, 128, 96, 6, 16, seed=10)
+    want = (bank.apply(x, slots),) + bank.grad(x, slots, dy)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((bank.apply(x, slots),) + bank.grad(x, slots, dy))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for out in got for p, q in zip(out, want))
+
+
+def test_refusals():
+    bank, x, slots, dy = make(6, 16, 24, 3, 4)
+    W, A, B, c = bank.weight, bank.A, bank.B, bank.scale
+    for args in ((W.cpu(), A, B), (W.double(), A, B), (W, A.bfloat16(), B), (W, A[:, :, :8], B), (W, A, B[:2]), (W, A, B, c.double()),
+                 (W, A, B, c[:2]), (W, A, B.transpose(1, 2).contiguous().transpose(1, 2)), (W, A[:0], B[:0], c[:0]),
+                 (W, A.repeat(1, 40, 1), B.repeat(1, 1, 40)), (W[0], A, B)):
+        with pytest.raises(ValueError):
+            QueryAdapters(*args)
+    for a in ((x.cpu(), slots), (x.bfloat16(), slots), (x[:, :8], slots), (x, slots[:5]), (x, slots.float()), (x, [0] * 5),
+              (x, [0, 1, 2, 0, 1, 3]), (x, [0, 1, 2, 0, 1, -2]), (x, [0, 1, 2, 0, 1, 0.5])):
+        with pytest.raises(ValueError):
+            bank.apply(*a)
+    for d in (dy[:5], dy.bfloat16(), dy[:, :8], dy.cpu()):
+        with pytest.raises(ValueError):
+            bank.grad(x, slots, d)
+    assert torch.equal(bank.apply(x, [0, 1, 2, None, -1, 0]), bank.apply(x, torch.tensor([0, 1, 2, -1, -1, 0], device="cuda")))
+
+
+def test_c_refusals():
+    import ctypes as C
+    bank, x, slots, dy = make(6, 16, 24, 3, 4)
+    lib, need = bank._lib, C.c_int64()
+    assert lib.rag_adapter_ws_bytes(0, 6, 16, 24, 3, 4, 1, C.byref(need)) == 0
+    ws = torch.empty(need.value + 256, dtype=torch.uint8, device="cuda")
+    p = lambda t: C.c_void_p(None if t is None else t.data_ptr())      # noqa: E731
+    y, dA, dB = (torch.full(s, 7.0, device="cuda") for s in ((6, 24), (3, 4, 16), (3, 24, 4)))
+
+    def call(dtype=0, n=6, d_in=16, d_out=24, S=3, R=4, xt=x, ldx=16, out=y, ldy=24, wst=ws, off=0, n_ws=need.value, slot=slots):
+        return lib.rag_adapter_apply_dev(dtype, n, d_in, d_out, S, R, p(xt), ldx, p(bank.weight), p(bank.A), p(bank.B),
+                                         p(bank.scale), p(slot), p(out), ldy, C.c_void_p(None if wst is None else wst.data_ptr() + off),
+                                         n_ws, C.c_void_p(0))
+    for kw in (dict(dtype=2), dict(n=-1), dict(n=(1 << 24) + 1), dict(d_in=0), dict(d_out=8193), dict(S=0), dict(S=4097), dict(R=0),
+               dict(R=129), dict(xt=None), dict(ldx=15), dict(out=None), dict(ldy=23), dict(wst=None), dict(off=8), dict(n_ws=1),
+               dict(slot=None)):
+        assert call(**kw) == _lib.RAG_ERR_INVALID_ARG, kw
+
+    def grad(da=dA, db=dB, n_ws=need.value, lddy=24, lddx=16):
+        return lib.rag_adapter_grad_dev(0, 6, 16, 24, 3, 4, p(x), 16, p(bank.weight), p(bank.A), p(bank.B), p(bank.scale), p(slots),
+                                        p(dy), lddy, p(x.clone()), lddx, p(da), p(db), p(ws), n_ws, C.c_void_p(0))
+    for kw in (dict(da=None), dict(db=None), dict(n_ws=1), dict(lddy=23), dict(lddx=15)):
+        assert grad(**kw) == _lib.RAG_ERR_INVALID_ARG, kw
+    torch.cuda.synchronize()
+    assert all(bool((t == 7).all()) for t in (y, dA, dB))
+    assert call() == 0 and grad() == 0
