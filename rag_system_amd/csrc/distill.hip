@@ -11,6 +11,7 @@
 // o = sum_j exp(s_ij - m) x_j, rescaled when m grows.  The index is split over workgroups; a join kernel adds the parts.
 // All sums, statistics and the row sum are fp32; dq is rounded once, to the type of q.
 #include "common.h"
+#include "distill_tile.h"
 
 #include <algorithm>
 #include <cmath>
@@ -20,10 +21,9 @@ namespace {
 
 using namespace rag;
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+using distill::f32x4;
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int MAX_LIST = RAG_DISTILL_MAX_K;
 constexpr int THREADS = 256;
 constexpr int WAVES = THREADS / 64;
 
@@ -64,23 +64,25 @@ __device__ __forceinline__ float wave_max(float v) {
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     return v;
 }
-// over the workgroup, for every thread; `red` holds WAVES floats
+// over a workgroup of W waves, for every thread; `red` holds W floats
+template <int W>
 __device__ __forceinline__ float block_sum(float v, float* red) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = 0.f;
-    for (int w = 0; w < WAVES; ++w) s += red[w];
+    for (int w = 0; w < W; ++w) s += red[w];
     return s;
 }
+template <int W>
 __device__ __forceinline__ float block_max(float v, float* red) {
     v = wave_max(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = red[0];
-    for (int w = 1; w < WAVES; ++w) s = fmaxf(s, red[w]);
+    for (int w = 1; w < W; ++w) s = fmaxf(s, red[w]);
     return s;
 }
 
@@ -98,33 +100,22 @@ struct Call {
     float* loss;
     void* dq;                 // m x d or NULL
     long long lddq;
-    // workspace of the "index" form
-    float* list_part;         // m x ld: sum_k p_k x_k
-    float* list_head;         // m x 2: [0] sum_k p_k (log p_k - s_k); [1] 1, 0 (empty list) or NaN (a bad row number)
-    float* part_ml;           // splits x m x 2: m, l
+    // workspace of the "index" form: the parts of the index' shares
+    float* part_ml;           // splits x m x 2: maximum in units of the product (L2: 2 <q,x> - ||x||^2), sum
     float* part_o;            // splits x m x ld
     int splits;
     long long rows_per_split;
 };
 
-// One workgroup per query: the list's entries.  LIST: the whole operator over the list; else list_part / list_head.
-template <typename T, bool LIST>
-__global__ __launch_bounds__(THREADS) void list_kernel(Call c) {
-    constexpr int E = Piece<T>::E;
-    extern __shared__ float sh[];
-    float* qs = sh;               // ld
-    float* s_of = qs + c.ld;      // k
-    float* p_of = s_of + c.k;     // k
-    __shared__ float red[WAVES];
-    const long long i = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const T* x = static_cast<const T*>(c.x);
+// The teacher's side of one query, by the whole workgroup: p_of[k] in LDS and the log of its normaliser.  Returns 1, or 0
+// (no entry of finite score) or NaN (a row number outside the index); the barriers inside publish p_of.
+template <int W>
+__device__ __forceinline__ float teacher(const Call& c, long long i, float* p_of, float* red, float* zmax_out, float* log_zsum) {
+    const int tid = threadIdx.x;
     const long long* ids = c.ids + i * c.k;
     const float* z = c.scores + i * c.k;
-    const T* q = static_cast<const T*>(c.q) + i * c.ldq;
-    for (int j = tid; j < c.ld; j += THREADS) qs[j] = j < c.d ? load1(q + j) : 0.f;
     float zmax = -INFINITY, any = 0.f, bad = 0.f;
-    for (int k = tid; k < c.k; k += THREADS) {
+    for (int k = tid; k < c.k; k += W * 64) {
         const long long id = ids[k];
         if (id < -1 || id >= c.n) bad = 1.f;
         else if (id >= 0) {
@@ -133,29 +124,34 @@ __global__ __launch_bounds__(THREADS) void list_kernel(Call c) {
             if (!(v == -INFINITY)) any = 1.f;
         }
     }
-    zmax = block_max(zmax, red);
-    any = block_max(any, red);
-    bad = block_max(bad, red);
-    if (bad != 0.f || any == 0.f) {       // (uniform) nothing to learn from, or a row number outside the index
-        const float v = bad != 0.f ? NAN : 0.f;
-        if (LIST) {
-            if (tid == 0) c.loss[i] = v;
-            if (c.dq)
-                for (int j = tid; j < c.d; j += THREADS) store1(static_cast<T*>(c.dq) + i * c.lddq + j, v);
-        } else if (tid == 0) {
-            c.list_head[2 * i] = v;
-            c.list_head[2 * i + 1] = v;
-        }
-        return;
-    }
+    zmax = block_max<W>(zmax, red);
+    any = block_max<W>(any, red);
+    bad = block_max<W>(bad, red);
+    if (bad != 0.f) return NAN;
+    if (any == 0.f) return 0.f;
     float zsum = 0.f;
-    for (int k = tid; k < c.k; k += THREADS)
-        if (ids[k] >= 0) zsum += expf(z[k] * c.beta_t - zmax);
-    zsum = block_sum(zsum, red);          // (its barriers also publish qs)
-    for (int k = wave; k < c.k; k += WAVES) {
+    for (int k = tid; k < c.k; k += W * 64) {
+        const float e = ids[k] >= 0 ? expf(z[k] * c.beta_t - zmax) : 0.f;
+        p_of[k] = e;
+        zsum += e;
+    }
+    zsum = block_sum<W>(zsum, red);
+    for (int k = tid; k < c.k; k += W * 64) p_of[k] /= zsum;   // (each thread its own)
+    __syncthreads();
+    *zmax_out = zmax;
+    *log_zsum = logf(zsum);
+    return 1.f;
+}
+
+// s_of[k]: the student's logits of the list's entries, a wave per entry; qs holds the query.
+template <typename T, int W>
+__device__ __forceinline__ void list_logits(const Call& c, const long long* ids, const float* qs, float* s_of) {
+    constexpr int E = Piece<T>::E;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int k = wave; k < c.k; k += W) {
         const long long id = ids[k];
         if (id < 0) continue;
-        const T* row = x + id * c.ld;
+        const T* row = static_cast<const T*>(c.x) + id * c.ld;
         float acc = 0.f;
         for (int j = lane * E; j < c.ld; j += 64 * E) {
             float v[E];
@@ -173,38 +169,57 @@ __global__ __launch_bounds__(THREADS) void list_kernel(Call c) {
         if (lane == 0) s_of[k] = c.l2 ? -c.beta * acc : c.beta * acc;
     }
     __syncthreads();
-    float smax = -INFINITY;
+}
+
+// sum_k p_k (log p_k - s_k)
+template <int W>
+__device__ __forceinline__ float list_head(const Call& c, long long i, const float* p_of, const float* s_of, float zmax, float log_zsum,
+                                           float* red) {
+    float head = 0.f;
+    for (int k = threadIdx.x; k < c.k; k += W * 64)
+        if (p_of[k] != 0.f) head += p_of[k] * (c.scores[i * c.k + k] * c.beta_t - zmax - log_zsum - s_of[k]);   // (NaN enters)
+    return block_sum<W>(head, red);
+}
+
+// over = the list: one workgroup per query does it all.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void list_kernel(Call c) {
+    constexpr int E = Piece<T>::E;
+    extern __shared__ float sh[];
+    float* qs = sh;               // ld
+    float* s_of = qs + c.ld;      // k
+    float* p_of = s_of + c.k;     // k
+    __shared__ float red[WAVES];
+    const long long i = blockIdx.x;
+    const int tid = threadIdx.x;
+    const T* x = static_cast<const T*>(c.x);
+    const long long* ids = c.ids + i * c.k;
+    const T* q = static_cast<const T*>(c.q) + i * c.ldq;
+    T* dq = c.dq ? static_cast<T*>(c.dq) + i * c.lddq : nullptr;
+    for (int j = tid; j < c.ld; j += THREADS) qs[j] = j < c.d ? load1(q + j) : 0.f;
+    float zmax, log_zsum;
+    const float live = teacher<WAVES>(c, i, p_of, red, &zmax, &log_zsum);   // (its barriers also publish qs)
+    if (!(live == 1.f)) {         // (uniform) nothing to learn from, or a row number outside the index
+        if (tid == 0) c.loss[i] = live;
+        if (dq)
+            for (int j = tid; j < c.d; j += THREADS) store1(dq + j, live);
+        return;
+    }
+    list_logits<T, WAVES>(c, ids, qs, s_of);
+    float smax = -INFINITY, mass = 0.f;
     for (int k = tid; k < c.k; k += THREADS)
         if (ids[k] >= 0) smax = fmaxf(smax, s_of[k]);
-    smax = block_max(smax, red);
-    const float log_zsum = logf(zsum);
-    float head = 0.f, mass = 0.f;
-    for (int k = tid; k < c.k; k += THREADS) {
-        float p = 0.f;
-        if (ids[k] >= 0) {
-            const float a = z[k] * c.beta_t - zmax;
-            p = expf(a) / zsum;
-            if (p != 0.f) head += p * (a - log_zsum - s_of[k]);   // (NaN enters)
-            mass += expf(s_of[k] - smax);
-        }
-        p_of[k] = p;
-    }
-    head = block_sum(head, red);
-    mass = block_sum(mass, red);
-    if (LIST) {
-        if (tid == 0) c.loss[i] = head + smax + logf(mass);
-        if (!c.dq) return;
-        for (int k = tid; k < c.k; k += THREADS)
-            if (ids[k] >= 0) p_of[k] = expf(s_of[k] - smax) / mass - p_of[k];
-        __syncthreads();
-    } else {
-        if (tid == 0) {
-            c.list_head[2 * i] = head;
-            c.list_head[2 * i + 1] = 1.f;
-        }
-        if (!c.dq) return;
-    }
-    const float f = LIST ? (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f) : 1.f;
+    smax = block_max<WAVES>(smax, red);
+    for (int k = tid; k < c.k; k += THREADS)
+        if (ids[k] >= 0) mass += expf(s_of[k] - smax);
+    mass = block_sum<WAVES>(mass, red);
+    const float head = list_head<WAVES>(c, i, p_of, s_of, zmax, log_zsum, red);
+    if (tid == 0) c.loss[i] = head + smax + logf(mass);
+    if (!dq) return;
+    for (int k = tid; k < c.k; k += THREADS)
+        if (ids[k] >= 0) p_of[k] = expf(s_of[k] - smax) / mass - p_of[k];
+    __syncthreads();
+    const float f = (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f);
     for (int j = tid * E; j < c.ld; j += THREADS * E) {
         float acc[E] = {};
         for (int k = 0; k < c.k; ++k) {
@@ -214,10 +229,8 @@ __global__ __launch_bounds__(THREADS) void list_kernel(Call c) {
             Piece<T>::load(x + id * c.ld + j, v);
             for (int e = 0; e < E; ++e) acc[e] = fmaf(p_of[k], v[e], acc[e]);
         }
-        for (int e = 0; e < E; ++e) {
-            if (!LIST) c.list_part[i * c.ld + j + e] = acc[e];
-            else if (j + e < c.d) store1(static_cast<T*>(c.dq) + i * c.lddq + j + e, f * acc[e]);
-        }
+        for (int e = 0; e < E; ++e)
+            if (j + e < c.d) store1(dq + j + e, f * acc[e]);
     }
 }
 
@@ -247,7 +260,7 @@ __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
                     for (int e = 0; e < E; ++e) acc = fmaf(qs[j + e], v[e], acc);
                 }
                 acc = wave_sum(acc);
-                acc = c.beta * (c.l2 ? 2.f * acc - c.norms[r + a] : acc);
+                if (c.l2) acc = fmaf(2.f, acc, -c.norms[r + a]);
             } else {
                 acc = -INFINITY;
             }
@@ -256,14 +269,14 @@ __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
         __syncthreads();
         float t = m;
         for (int a = 0; a < ANY_ROWS; ++a) t = fmaxf(t, s_of[a]);
-        const float scale = t == -INFINITY ? 1.f : expf(m - t);
+        const float scale = t == -INFINITY ? 1.f : expf((m - t) * c.beta);
         m = t;
         l *= scale;
         if (GRAD)
             for (int b = 0; b < COLS; ++b)
                 for (int e = 0; e < E; ++e) o[b][e] *= scale;
         for (int a = 0; a < ANY_ROWS && r + a < r1; ++a) {
-            const float p = s_of[a] == -INFINITY ? 0.f : expf(s_of[a] - m);
+            const float p = s_of[a] == -INFINITY ? 0.f : expf((s_of[a] - m) * c.beta);
             l += p;
             if (!GRAD) continue;
             for (int b = 0; b < COLS; ++b) {
@@ -289,54 +302,80 @@ __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
     }
 }
 
-// Adds the splits' parts: one workgroup per query.
+// Adds the shares' parts and takes the teacher's side off: one workgroup per query and 64 columns, each wave adds every
+// eighth share (list entry); the first of a query's workgroups computes the loss.
+constexpr int JOIN_WAVES = 8, JOIN_THREADS = 64 * JOIN_WAVES;
 template <typename T>
-__global__ __launch_bounds__(THREADS) void join_kernel(Call c) {
-    extern __shared__ float w_of[];   // splits
-    __shared__ float red[WAVES];
+__global__ __launch_bounds__(JOIN_THREADS) void join_kernel(Call c) {
+    extern __shared__ float sh[];
+    __shared__ float red[JOIN_WAVES];
+    __shared__ float cols[2][JOIN_WAVES][64];
+    float* w_of = sh;                 // splits
+    float* p_of = w_of + c.splits;    // k
+    float* s_of = p_of + c.k;         // k
+    float* qs = s_of + c.k;           // ld
     const long long i = blockIdx.x;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     T* dq = c.dq ? static_cast<T*>(c.dq) + i * c.lddq : nullptr;
-    const float live = c.list_head[2 * i + 1];
-    if (!(live == 1.f)) {
-        if (tid == 0) c.loss[i] = live;
-        if (dq)
-            for (int j = tid; j < c.d; j += THREADS) store1(dq + j, live);
+    const long long* ids = c.ids + i * c.k;
+    const int col = blockIdx.y * 64 + lane;
+    float zmax, log_zsum;
+    const float live = teacher<JOIN_WAVES>(c, i, p_of, red, &zmax, &log_zsum);
+    if (!(live == 1.f)) {             // (uniform)
+        if (tid == 0 && blockIdx.y == 0) c.loss[i] = live;
+        if (dq && wave == 0 && col < c.d) store1(dq + col, live);
         return;
     }
-    float m = -INFINITY;
-    for (int s = tid; s < c.splits; s += THREADS) m = fmaxf(m, c.part_ml[2 * (s * c.m + i)]);
-    m = block_max(m, red);
-    float l = 0.f;
-    for (int s = tid; s < c.splits; s += THREADS) {
-        const float ms = c.part_ml[2 * (s * c.m + i)];
-        const float w = ms == -INFINITY ? 0.f : expf(ms - m);
+    float m = -INFINITY, l = 0.f;
+    for (int s = tid; s < c.splits; s += JOIN_THREADS) m = fmaxf(m, c.part_ml[2 * (s * c.m + i)]);
+    m = block_max<JOIN_WAVES>(m, red);
+    for (int s = tid; s < c.splits; s += JOIN_THREADS) {
+        const float ms = c.part_ml[2 * (s * c.m + i)], ls = c.part_ml[2 * (s * c.m + i) + 1];
+        const float w = ms == -INFINITY ? 0.f : expf((ms - m) * c.beta);
         w_of[s] = w;
-        const float ls = c.part_ml[2 * (s * c.m + i) + 1];
-        l += w == 0.f && !(ls != ls) ? 0.f : w * ls;
+        l += w * ls;
     }
-    l = block_sum(l, red);
-    float qq = 0.f;
-    if (c.l2) {
+    l = block_sum<JOIN_WAVES>(l, red);   // (publishes w_of)
+    if (blockIdx.y == 0) {
         const T* q = static_cast<const T*>(c.q) + i * c.ldq;
-        for (int j = tid; j < c.d; j += THREADS) qq = fmaf(load1(q + j), load1(q + j), qq);
-        qq = block_sum(qq, red);
+        float qq = 0.f;
+        for (int j = tid; j < c.ld; j += JOIN_THREADS) {
+            const float v = j < c.d ? load1(q + j) : 0.f;
+            qs[j] = v;
+            qq = fmaf(v, v, qq);
+        }
+        qq = block_sum<JOIN_WAVES>(qq, red);
+        list_logits<T, JOIN_WAVES>(c, ids, qs, s_of);
+        const float head = list_head<JOIN_WAVES>(c, i, p_of, s_of, zmax, log_zsum, red);
+        if (tid == 0) c.loss[i] = head + c.beta * (c.l2 ? m - qq : m) + logf(l);
     }
-    if (tid == 0) c.loss[i] = c.list_head[2 * i] + (m - c.beta * qq) + logf(l);
     if (!dq) return;
-    const float f = (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f);
-    for (int j = tid; j < c.d; j += THREADS) {
-        float o = 0.f;
-        for (int s = 0; s < c.splits; ++s) o = fmaf(w_of[s], c.part_o[(s * c.m + i) * c.ld + j], o);
-        store1(dq + j, f * (o / l - c.list_part[i * c.ld + j]));
+    float o = 0.f, a = 0.f;
+    if (col < c.ld) {
+#pragma unroll 8
+        for (int s = wave; s < c.splits; s += JOIN_WAVES) o = fmaf(w_of[s], c.part_o[(s * c.m + i) * c.ld + col], o);
+#pragma unroll 4
+        for (int k = wave; k < c.k; k += JOIN_WAVES)
+            if (ids[k] >= 0) a = fmaf(p_of[k], load1(static_cast<const T*>(c.x) + ids[k] * c.ld + col), a);
     }
+    cols[0][wave][lane] = o;
+    cols[1][wave][lane] = a;
+    __syncthreads();
+    if (wave != 0 || col >= c.d) return;
+    o = a = 0.f;
+    for (int w = 0; w < JOIN_WAVES; ++w) {
+        o += cols[0][w][lane];
+        a += cols[1][w][lane];
+    }
+    store1(dq + col, (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f) * (o / l - a));
 }
 
 // How a call is split; depends on the number of queries and the row length, not on the number of rows (the
 // workspace may be allocated before rows are added).
 struct Plan {
+    distill::TilePlan tile;
     int splits;
-    size_t head_off, list_off, ml_off, o_off, bytes;
+    size_t ml_off, o_off, bytes;
 };
 
 int elem_ld(int d, int bf16) { return bf16 ? (d + 7) & ~7 : (d + 3) & ~3; }
@@ -345,14 +384,13 @@ Plan make_plan(long long m, int d, int bf16, int over, bool grad) {
     Plan p{};
     if (over == RAG_OVER_LIST || m == 0) return p;
     const size_t ld = elem_ld(d, bf16);
-    p.splits = (int)std::max<long long>(1, std::min<long long>(1024, 2048 / m));
+    if (distill::tile_plan(m, (int)ld, bf16 != 0, &p.tile)) p.splits = p.tile.splits;
+    else p.splits = (int)std::max<long long>(1, std::min<long long>(1024, 2048 / m));
     auto take = [&](size_t floats) {
         const size_t at = p.bytes;
         p.bytes += (floats * sizeof(float) + 255) & ~(size_t)255;
         return at;
     };
-    p.head_off = take(2 * m);
-    p.list_off = take(grad ? m * ld : 0);
     p.ml_off = take((size_t)p.splits * m * 2);
     p.o_off = take(grad ? (size_t)p.splits * m * ld : 0);
     return p;
@@ -369,25 +407,43 @@ struct Ctx {
 template <typename T>
 int launch(Ctx& x) {
     Call& c = x.c;
-    const size_t list_lds = ((size_t)c.ld + 2 * c.k) * sizeof(float);
     if (x.over == RAG_OVER_LIST) {
-        list_kernel<T, true><<<(unsigned)c.m, THREADS, list_lds, x.st>>>(c);
+        list_kernel<T><<<(unsigned)c.m, THREADS, ((size_t)c.ld + 2 * c.k) * sizeof(float), x.st>>>(c);
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
-    c.splits = x.p.splits;
-    c.rows_per_split = std::max<long long>(ANY_ROWS, (c.n + c.splits - 1) / c.splits);
-    c.list_head = reinterpret_cast<float*>(x.ws + x.p.head_off);
-    c.list_part = reinterpret_cast<float*>(x.ws + x.p.list_off);
+    const int step = x.p.tile.rows > 0 ? x.p.tile.rows : ANY_ROWS;     // shares are whole tiles; the last may be shorter
+    const long long per = (c.n + x.p.splits - 1) / x.p.splits;
+    c.rows_per_split = std::max<long long>(1, (per + step - 1) / step) * step;
+    c.splits = (int)((c.n + c.rows_per_split - 1) / c.rows_per_split);
     c.part_ml = reinterpret_cast<float*>(x.ws + x.p.ml_off);
     c.part_o = reinterpret_cast<float*>(x.ws + x.p.o_off);
-    list_kernel<T, false><<<(unsigned)c.m, THREADS, list_lds, x.st>>>(c);
-    RAG_HIP(hipGetLastError());
-    const dim3 grid((unsigned)c.splits, (unsigned)c.m);
-    if (c.dq) index_any_kernel<T, true><<<grid, THREADS, c.ld * sizeof(float), x.st>>>(c);
-    else index_any_kernel<T, false><<<grid, THREADS, c.ld * sizeof(float), x.st>>>(c);
-    RAG_HIP(hipGetLastError());
-    join_kernel<T><<<(unsigned)c.m, THREADS, c.splits * sizeof(float), x.st>>>(c);
+    if (c.splits > 0 && x.p.tile.rows > 0) {
+        distill::TileCall t{};
+        t.x = c.x;
+        t.norms = c.l2 ? c.norms : nullptr;
+        t.q = c.q;
+        t.part_ml = c.part_ml;
+        t.part_o = c.part_o;
+        t.n = c.n;
+        t.m = c.m;
+        t.ldq = c.ldq;
+        t.rows_per_split = c.rows_per_split;
+        t.ld = c.ld;
+        t.d = c.d;
+        t.splits = c.splits;
+        t.q_tiles = x.p.tile.q_tiles;
+        t.k2 = (float)((double)c.beta * 1.4426950408889634074);
+        const int rc = distill::tile_launch(x.p.tile, t, c.dq != nullptr, x.st);
+        if (rc) return rc;
+    } else if (c.splits > 0) {
+        const dim3 grid((unsigned)c.splits, (unsigned)c.m);
+        if (c.dq) index_any_kernel<T, true><<<grid, THREADS, c.ld * sizeof(float), x.st>>>(c);
+        else index_any_kernel<T, false><<<grid, THREADS, c.ld * sizeof(float), x.st>>>(c);
+        RAG_HIP(hipGetLastError());
+    }
+    const dim3 grid((unsigned)c.m, c.dq ? (unsigned)((c.ld + 63) / 64) : 1u);
+    join_kernel<T><<<grid, JOIN_THREADS, ((size_t)c.splits + 2 * c.k + c.ld) * sizeof(float), x.st>>>(c);
     RAG_HIP(hipGetLastError());
     return RAG_OK;
 }
