@@ -42,6 +42,7 @@ struct TileCall {
 // no tile kernel serves the row length.
 struct TilePlan {
     int kind;        // index of the variant, -1: none
+    bool few;        // ... among those for one to four queries (distill_rows.h)
     int rows;        // rows per tile
     int splits, q_tiles;
 };
@@ -180,16 +181,24 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
         for (int u = 0; u < SUBS; ++u)
 #pragma unroll
             for (int i = 0; i < ACC; ++i) s[u][i] = 0.f;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            f32x4 a[SUBS];
+        // (the next step's operands are read in front of a step's products: a wave has its SIMD to itself, nobody
+        // else fills the time an LDS read takes; sched_barrier keeps the order)
+        f32x4 a[2][SUBS];
+        auto read_s = [&](int g, f32x4* to) {
 #pragma unroll
             for (int u = 0; u < SUBS; ++u)
-                a[u] = *reinterpret_cast<const f32x4*>(xs + u * QT * 32 + off_s[g % GP] + (g / GP) * RT * 32);
+                to[u] = *reinterpret_cast<const f32x4*>(xs + u * QT * 32 + off_s[g % GP] + (g / GP) * RT * 32);
+        };
+        read_s(0, a[0]);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            if (g + 1 < NG) read_s(g + 1, a[(g + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) s[u] = M::mma(a[u][e], q[g][e], s[u]);
+                for (int u = 0; u < SUBS; ++u) s[u] = M::mma(a[g & 1][u][e], q[g][e], s[u]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         float p[SUBS][ACC];
 #pragma unroll
@@ -258,16 +267,29 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
             }
         l += sum;                               // this lane's rows; the lanes of a query are added at the end
         if (!GRAD) continue;
+        // a step: four rows of every lane, one column tile; STEPS of them are a column tile
+        constexpr int STEPS = SUBS * ACC / 4, AHEAD = QT == 32 ? 1 : 2;
+        float b[AHEAD + 1][4];
+        auto read_o = [&](int st, float* to) {
+            const int j = st / STEPS, u = st % STEPS / (ACC / 4), h = st % (ACC / 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i] = xs[(u * QT + 8 * h) * 32 + off_p[j % PP][i] + (j / PP) * RT * 32];
+        };
+#pragma unroll
+        for (int st = 0; st < AHEAD; ++st) read_o(st, b[st]);
 #pragma unroll
         for (int j = 0; j < NCT; ++j) {
             acc_t part;
 #pragma unroll
             for (int i = 0; i < ACC; ++i) part[i] = 0.f;
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u)
+            for (int k = 0; k < STEPS; ++k) {
+                const int st = j * STEPS + k;
+                if (st + AHEAD < NCT * STEPS) read_o(st + AHEAD, b[(st + AHEAD) % (AHEAD + 1)]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < ACC; ++i)
-                    part = M::mma(xs[(u * QT + 8 * (i >> 2)) * 32 + off_p[j % PP][i & 3] + (j / PP) * RT * 32], p[u][i], part);
+                for (int i = 0; i < 4; ++i) part = M::mma(b[st % (AHEAD + 1)][i], p[k / (ACC / 4)][k % (ACC / 4) * 4 + i], part);
+            }
 #pragma unroll
             for (int i = 0; i < ACC; ++i) o[j][i] += part[i];
         }

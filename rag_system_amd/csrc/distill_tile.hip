@@ -1,4 +1,5 @@
 // distill_tile.hip -- variants of the pass over the index (distill_tile.h) and the rule that picks one.
+#include "distill_rows.h"
 #include "distill_tile.h"
 
 #include <algorithm>
@@ -47,10 +48,45 @@ const Variant VARIANTS[] = {
 };
 constexpr int N_VARIANTS = sizeof VARIANTS / sizeof VARIANTS[0];
 
+// One to four queries: [queries: 1, 2, 4][grad][l2]
+struct Few {
+    int bf16, lpr, np;
+    kernel_t fn[3][2][2];
+};
+template <typename T, int LPR, int NP, int MQ>
+void few_fn(kernel_t (*fn)[2]) {
+    fn[0][0] = rows_kernel<T, LPR, NP, MQ, false, false>;
+    fn[0][1] = rows_kernel<T, LPR, NP, MQ, false, true>;
+    fn[1][0] = rows_kernel<T, LPR, NP, MQ, true, false>;
+    fn[1][1] = rows_kernel<T, LPR, NP, MQ, true, true>;
+}
+template <typename T, int LPR, int NP>
+Few few() {
+    Few f{sizeof(T) == 2, LPR, NP, {}};
+    few_fn<T, LPR, NP, 1>(f.fn[0]);
+    few_fn<T, LPR, NP, 2>(f.fn[1]);
+    few_fn<T, LPR, NP, 4>(f.fn[2]);
+    return f;
+}
+// in order of the row length they serve: LPR x NP pieces of 16 bytes
+const Few FEW[] = {
+    few<float, 16, 1>(), few<float, 16, 2>(), few<float, 32, 2>(), few<float, 32, 3>(), few<float, 32, 4>(), few<float, 32, 6>(),
+    few<float, 32, 8>(),
+    few<unsigned short, 16, 1>(), few<unsigned short, 16, 2>(), few<unsigned short, 32, 2>(), few<unsigned short, 32, 3>(),
+    few<unsigned short, 32, 4>(),
+};
+constexpr int N_FEW = sizeof FEW / sizeof FEW[0];
+
 }  // namespace
 
 bool tile_plan(long long m, int ld, bool bf16, TilePlan* p) {
-    *p = TilePlan{-1, 0, 0, 0};
+    *p = TilePlan{-1, false, 0, 0, 0};
+    if (m <= 4)
+        for (int v = 0; v < N_FEW; ++v)
+            if ((FEW[v].bf16 != 0) == bf16 && FEW[v].lpr * FEW[v].np * (bf16 ? 8 : 4) >= ld) {
+                *p = TilePlan{v, true, 64 / FEW[v].lpr * ROWS_WAVES, num_cus() * 4, 1};
+                return true;
+            }
     if (bf16) return false;
     const int most = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;      // queries of a workgroup that are of use
     int best = -1;
@@ -85,6 +121,12 @@ bool tile_plan(long long m, int ld, bool bf16, TilePlan* p) {
 }
 
 int tile_launch(const TilePlan& p, const TileCall& c, bool grad, hipStream_t st) {
+    if (p.few) {
+        const kernel_t fn = FEW[p.kind].fn[c.m == 1 ? 0 : c.m == 2 ? 1 : 2][grad ? 1 : 0][c.norms ? 1 : 0];
+        fn<<<(unsigned)c.splits, 64 * ROWS_WAVES, grad ? (size_t)ROWS_WAVES * c.ld * sizeof(float) : 0, st>>>(c);
+        RAG_HIP(hipGetLastError());
+        return RAG_OK;
+    }
     const Variant& a = VARIANTS[p.kind];
     kernel_t fn = a.fn[grad ? 1 : 0][c.norms ? 1 : 0];
     if (a.lds > 48 * 1024)
