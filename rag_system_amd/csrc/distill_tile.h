@@ -1,28 +1,30 @@
-// distill_tile.h -- the pass over the index of rag_flat_distill_dev, float32 rows.
+// distill_tile.h -- the pass over the index of rag_flat_distill_dev with matrix instructions.
 //
-// A workgroup holds WQ x QT queries and streams its share of the rows through LDS, RT rows at a time.  Per tile
-//     S^T = X Q^T          (rows x queries)     MFMA 32x32x2 (QT = 32) or 16x16x4 (QT = 16), fp32
-//     P^T = exp(S^T - m)   running maximum m and sum l per query
+// A workgroup holds WQ x 16 queries and streams its share of the rows through LDS, RT rows at a time.  Per tile
+//     S^T = X Q^T          (rows x queries)     MFMA 16x16x4 (float32) / 16x16x32 (bfloat16)
+//     P^T = exp(S^T - m)   reference m and sum l per query
 //     O^T += X^T P^T       (columns x queries)
-// Writing both products transposed keeps a query in ONE lane of every result (lane & (QT-1)): maximum, sum and
-// rescaling are per-lane, and register i of S^T, whose lanes hold rows {r, r + 4, ..} of the query, already is the B
-// operand of the second product for exactly those rows -- the A operand takes the same rows of X^T.  P never
-// leaves its registers.
-// WD waves share a group of QT queries, each with CW of the columns (the row sum O and the queries of 384 columns
-// fill a wave's registers); their parts of S^T meet in LDS, added in the same order by each of them.
-// The products add to O two or four rows at a time, each rounded at O's last place; a sum over many rows of which one has
+// Writing both products transposed keeps a query in ONE lane of every result (lane & 15): maximum, sum and weights are
+// per-lane, and the registers of S^T already are the B operand of the second product -- register i of a lane group kl holds
+// row 4 kl + i of the query, so the A operand takes the same rows of X^T.  P never leaves its registers.  (bfloat16: 32
+// rows a product, eight of a lane: four of each half of the tile; X^T comes by the transposing LDS read.  The weights are
+// split into a bfloat16 and the bfloat16 of what is left, two products: one alone, 2^-9 off, is more than the gradient
+// keeps where student and teacher agree and sum_j P x and sum_k p x nearly cancel.)
+// WD waves share a group of 16 queries, each with CW of the columns (the row sum O and the queries of 384 columns
+// fill half of what a wave has with two on a SIMD); their parts of S^T meet in LDS, added in the same order by each.
+// The products add to O a few rows at a time, each rounded at O's last place; a sum over many rows of which one has
 // most of the weight would lose the others.  So every WINDOW tiles O is put down: added to the workgroup's part in HBM
 // and started again from zero.  (Summing each tile from zero and adding it to O in registers is as exact, but those
-// additions hold up the next products.)
+// additions hold up the next products: 13.4 against 11.2 ms for 1024 queries x 1M x 384.)
 // m is not the maximum but a reference that stays until a logit lies more than 2^LIFT above it: weights up to 2^LIFT and
-// their sums lose nothing in float32, and O, which fills the accumulation registers, is never rescaled there -- when the
-// reference does move, O is put down first.
+// their sums lose nothing in float32, and O is never rescaled in its registers -- when the reference does move, O is put
+// down first.
 //
-// Rows come by LDS-DMA (16 bytes a lane) into a ring of NB tiles, a tile as blocks of 32 columns: [DP / 32][RT][32].
-// One instruction fetches 128 bytes of each of eight rows, so a lane's row and piece are the same in all of them and its
-// address is one lane offset plus a uniform one.  The 16-byte pieces of a row's 128 bytes are stored at their place
-// xor (row & 7): both the 16-byte reads of S (8 rows, one piece) and the 4-byte reads of O (8 pieces of a row) touch
-// every bank once.
+// Rows come by LDS-DMA (16 bytes a lane) into a ring of NB tiles, a tile as blocks of 128 bytes of each row:
+// [blocks][RT][128 bytes].  One instruction fetches 128 bytes of each of eight rows, so a lane's row and piece are the same in
+// all of them.  The 16-byte pieces of a row's 128 bytes are stored at their place xor a permutation of (row & 7), so
+// that the 16-byte reads of S (8 rows, one piece) and the reads of O (float32: 4 pieces of rows r and r + 4; bfloat16: a pair
+// of pieces of four rows) touch every bank once.
 #pragma once
 #include "common.h"
 
@@ -30,7 +32,6 @@ namespace rag {
 namespace distill {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct TileCall {
     const void* x;             // n x ld
@@ -48,6 +49,7 @@ struct TileCall {
 struct TilePlan {
     int kind;        // index of the variant, -1: none
     bool few;        // ... among those for one to four queries (distill_rows.h)
+    bool bf16;
     int rows;        // rows per tile
     int splits, q_tiles;
 };
@@ -77,153 +79,156 @@ __device__ __forceinline__ bool place(const TileCall& c, int* split, int* q_tile
     return *split < c.splits;
 }
 
-template <int QT> struct Mma32;
-template <> struct Mma32<32> {
-    typedef f32x16 acc_t;
-    static constexpr int KL = 2, ACC = 16;
-    static __device__ __forceinline__ acc_t mma(float a, float b, acc_t c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
-};
-template <> struct Mma32<16> {
-    typedef f32x4 acc_t;
-    static constexpr int KL = 4, ACC = 4;
-    static __device__ __forceinline__ acc_t mma(float a, float b, acc_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-};
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int WINDOW = 64;      // tiles
 constexpr float LIFT = 40.f;    // powers of two
+// One group of queries, three tiles: the variant whose four waves are alone on the CU and bound by HBM.
+constexpr bool pipelined(int wq, int wd, int cw, int rt, int nb) { return wq == 1 && nb == 3 && rt == 32 && cw <= 96; }
 
-template <int QT, int WQ, int WD, int CW, int RT, int NB, bool GRAD, bool L2>
-__global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
-    typedef Mma32<QT> M;
-    typedef typename M::acc_t acc_t;
-    constexpr int KL = M::KL, ACC = M::ACC, NW = WQ * WD, DP = CW * WD;
-    constexpr int SUBS = RT / QT;              // MFMA tiles along the rows
-    constexpr int NG = CW / (4 * KL);          // 16-byte pieces of a lane along the columns (S)
-    constexpr int GP = 8 / KL;                 // ... of which GP within 128 bytes
-    constexpr int NCT = CW / QT;               // column tiles (O)
-    constexpr int PP = 32 / QT;                // ... of which PP within 128 bytes
-    constexpr int LOADS = RT * DP / 256 / NW;  // LDS-DMA instructions (1 KiB) per wave and tile
-    static_assert(CW % 32 == 0 && RT % QT == 0 && RT % 8 == 0 && RT * DP % (256 * NW) == 0, "tile shape");
-    constexpr int TILE = RT * DP;              // floats
-    extern __shared__ __align__(16) float lds[];
-    float* exch = lds + NB * TILE;             // WD > 1: NW x SUBS x ACC x 64
+template <typename T, int WQ, int WD, int CW, int RT, int NB, bool GRAD, bool L2>
+__global__ __launch_bounds__(64 * WQ * WD, 1) void tile_kernel(TileCall c) {
+    constexpr bool BF = sizeof(T) == 2;
+    constexpr int ESZ = sizeof(T), PIECE = 16 / ESZ;      // elements of a 16-byte piece
+    constexpr int NW = WQ * WD, DP = CW * WD, BLOCK = RT * 128;      // bytes of a block of columns
+    constexpr int SUBS = RT / 16;                         // MFMA tiles along the rows
+    constexpr int NG = CW / (4 * PIECE);                  // steps of S: 64 bytes of a row
+    constexpr int NCT = CW / 16;                          // column tiles of O
+    constexpr int PP = 8 * PIECE / 16;                    // ... of which PP within 128 bytes
+    constexpr int TILE = RT * DP * ESZ;                   // bytes
+    constexpr int LOADS = TILE / 1024 / NW;               // LDS-DMA instructions per wave and tile
+    static_assert(CW % (8 * PIECE) == 0 && RT % (BF ? 32 : 16) == 0 && TILE % (1024 * NW) == 0, "tile shape");
+    extern __shared__ __align__(16) char lds[];
+    float* exch = reinterpret_cast<float*>(lds + NB * TILE);   // WD > 1: NW x SUBS x 64 x 4
 
     int split, q_tile;
     if (!place(c, &split, &q_tile)) return;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int li = lane & (QT - 1), kl = lane / QT, wd = wid % WD, wq = wid / WD;
+    const int li = lane & 15, kl = lane >> 4, wd = wid % WD, wq = wid / WD;
     const long long r0 = split * c.rows_per_split, r1 = min(c.n, r0 + c.rows_per_split);
     const int tiles = (int)((r1 - r0 + RT - 1) / RT);
-    const long long qi = ((long long)q_tile * WQ + wq) * QT + li;
-    const float* x = static_cast<const float*>(c.x);
+    const long long qi = ((long long)q_tile * WQ + wq) * 16 + li;
+    const T* x = static_cast<const T*>(c.x);
+    // where a row's pieces are: place of piece p of row r = p ^ turn(r)
+    auto turn = [](int r) __attribute__((always_inline)) { return BF ? ((r & 3) << 1) | ((r >> 2) & 1) : r & 7; };
 
-    // queries: B operand of S^T, pieces kl of every 4 KL columns (a lane without a query takes the first one's: its
-    // results are not stored); zero behind the row's end
-    f32x4 q[NG];
+    // queries: B operand of S^T, piece kl of every four (a lane without a query takes the first one's: its results are
+    // not stored); zero behind the row's end
+    u32x4 q[NG];
     {
-        const float* qp = static_cast<const float*>(c.q) + (qi < c.m ? qi : 0) * c.ldq;
+        const T* qp = static_cast<const T*>(c.q) + (qi < c.m ? qi : 0) * c.ldq;
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < NG; ++g) {
+            T v[PIECE];
+#pragma unroll
+            for (int e = 0; e < PIECE; ++e) {
+                const int col = wd * CW + (g * 4 + kl) * PIECE + e;
+                v[e] = qp[min(col, c.d - 1)];
+            }
+            __builtin_memcpy(&q[g], v, 16);
+            const int end = c.d - (wd * CW + (g * 4 + kl) * PIECE);      // values of this piece that the row has
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int col = wd * CW + g * 4 * KL + kl * 4 + e;
-                q[g][e] = __uint_as_float(__float_as_uint(qp[min(col, c.d - 1)]) & (col < c.d ? ~0u : 0u));
+                if (BF) q[g][e] &= (2 * e < end ? 0xffffu : 0u) | (2 * e + 1 < end ? 0xffff0000u : 0u);
+                else q[g][e] &= e < end ? ~0u : 0u;
             }
+        }
     }
-    // places in a tile, in floats
-    int off_s[GP], off_p[PP][4];
+    // places in a tile, in bytes
+    int off_s[2], off_p[PP][BF ? 1 : 4];
 #pragma unroll
-    for (int g = 0; g < GP; ++g) off_s[g] = wd * CW * RT + li * 32 + (((g * KL + kl) ^ (li & 7)) << 2);
+    for (int g = 0; g < 2; ++g) off_s[g] = wd * (CW / (8 * PIECE)) * BLOCK + li * 128 + (((g * 4 + kl) ^ turn(li)) << 4);
 #pragma unroll
     for (int j = 0; j < PP; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            off_p[j][i] = wd * CW * RT + (4 * kl + i) * 32 + (((j * (QT / 4) + (li >> 2)) ^ ((4 * kl + i) & 7)) << 2) + (li & 3);
+        for (int i = 0; i < (BF ? 1 : 4); ++i) {
+            // float32: row 4 kl + i, column li of the tile.  bfloat16: this lane's part of the transposing read, row 4 kl + li / 4,
+            // columns li % 4 * 4 and on
+            const int row = 4 * kl + (BF ? li >> 2 : i), byte = BF ? (li & 3) * 8 : li * 4;
+            off_p[j][i] = wd * (CW / (8 * PIECE)) * BLOCK + row * 128 + (((j * (16 / PIECE) + (byte >> 4)) ^ turn(row)) << 4) + (byte & 15);
+        }
 
     // Columns behind the row's end come from its last piece (their queries are zero, their sums are not stored), rows
     // behind the index' end from its last row (they are given no weight).
-    const int lr = lane >> 3, lc = ((lane & 7) ^ lr) << 2;
-    auto fetch1 = [&](int t, int b, int a) __attribute__((always_inline)) {    // the a-th of this wave's instructions for tile t, into ring place b
+    const int lr = lane >> 3, lc = ((lane & 7) ^ turn(lr)) * PIECE;
+    auto fetch1 = [&](int t, int b, int a) __attribute__((always_inline)) {   // the a-th of this wave's instructions for tile t, into ring place b
         const long long first = r0 + (long long)t * RT;
         const int at = a * NW + wid, blk = at / (RT / 8), rg = at % (RT / 8) * 8;
-        const int rows = (int)min((long long)RT, c.n - first), row = min(rg + lr, rows - 1), col = min(blk * 32 + lc, c.ld - 4);
-        lds_dma16(x + first * c.ld, (unsigned)(rows * c.ld) * 4, (row * c.ld + col) * 4, lds + b * TILE + at * 256);
+        const int rows = (int)min((long long)RT, c.n - first), row = min(rg + lr, rows - 1), col = min(blk * 8 * PIECE + lc, c.ld - PIECE);
+        lds_dma16(x + first * c.ld, (unsigned)(rows * c.ld) * ESZ, (row * c.ld + col) * ESZ, lds + b * TILE + at * 1024);
     };
-    acc_t o[GRAD ? NCT : 1];
+    f32x4 o[GRAD ? NCT : 1];
     if (GRAD)
 #pragma unroll
-        for (int j = 0; j < NCT; ++j)
-#pragma unroll
-            for (int i = 0; i < ACC; ++i) o[j][i] = 0.f;
+        for (int j = 0; j < NCT; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, m_next = -INFINITY, l = 0.f;
     bool lifted = false;
-    acc_t s[SUBS];                              // S^T of the newest tile, then its weights
-    float nrm[L2 ? SUBS : 1][L2 ? ACC : 1];
+    f32x4 s[SUBS];                              // S^T of the newest tile, then its weights
+    f32x4 nrm[L2 ? SUBS : 1];
 
     auto norms = [&](int t) __attribute__((always_inline)) {
         const long long first = r0 + (long long)t * RT;
 #pragma unroll
         for (int u = 0; u < SUBS; ++u)
 #pragma unroll
-            for (int i = 0; i < ACC; ++i)
-                nrm[L2 ? u : 0][L2 ? i : 0] = c.norms[min(first + u * QT + 8 * (i >> 2) + (i & 3) + 4 * kl, c.n - 1)];
+            for (int i = 0; i < 4; ++i) nrm[L2 ? u : 0][i] = c.norms[min(first + u * 16 + 4 * kl + i, c.n - 1)];
     };
-    // S^T of the tile at xs.  The next step's operands are read in front of a step's products (a wave has its SIMD to itself:
-    // nobody else fills the time an LDS read takes; sched_barrier keeps the order), and the wave's LDS-DMA instructions for
-    // tile t are spread over the steps: each holds the wave for 60 to 180 cycles.
-    auto product = [&](const float* xs, int t, int b) __attribute__((always_inline)) {
+    // S^T of the tile at xs.  The next step's operands are read in front of a step's products (sched_barrier keeps the order),
+    // and the wave's LDS-DMA instructions for tile t are spread over the steps: each holds the wave for 60 to 180 cycles.
+    auto product = [&](const char* xs, int t, int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u)
-#pragma unroll
-            for (int i = 0; i < ACC; ++i) s[u][i] = 0.f;
-        f32x4 a[2][SUBS];
-        auto read = [&](int g, f32x4* to) __attribute__((always_inline)) {
+        for (int u = 0; u < SUBS; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        u32x4 a[2][SUBS];
+        auto read = [&](int g, u32x4* to) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < SUBS; ++u)
-                to[u] = *reinterpret_cast<const f32x4*>(xs + u * QT * 32 + off_s[g % GP] + (g / GP) * RT * 32);
+                to[u] = *reinterpret_cast<const u32x4*>(xs + off_s[g & 1] + u * 16 * 128 + (g >> 1) * BLOCK);
         };
         read(0, a[0]);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             if (g + 1 < NG) read(g + 1, a[(g + 1) & 1]);
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (BF) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+                for (int u = 0; u < SUBS; ++u)
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[g & 1][u]), __builtin_bit_cast(bf16x8, q[g]), s[u], 0, 0, 0);
+            } else {
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) s[u] = M::mma(a[g & 1][u][e], q[g][e], s[u]);
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int u = 0; u < SUBS; ++u)
+                        s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[g & 1][u][e]), __uint_as_float(q[g][e]), s[u], 0, 0, 0);
+            }
             if (NB > 1)
 #pragma unroll
                 for (int f = g * LOADS / NG; f < (g + 1) * LOADS / NG; ++f) fetch1(t, b, f);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    float* mine = exch + wid * SUBS * ACC * 64;
+    float* mine = exch + wid * SUBS * 256;
     auto give = [&]() __attribute__((always_inline)) {                         // this wave's part of S^T
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u)
-#pragma unroll
-            for (int i = 0; i < ACC; i += 4)
-                *reinterpret_cast<f32x4*>(mine + (u * ACC + i) * 64 + lane * 4) = f32x4{s[u][i], s[u][i + 1], s[u][i + 2], s[u][i + 3]};
+        for (int u = 0; u < SUBS; ++u) *reinterpret_cast<f32x4*>(mine + u * 256 + lane * 4) = s[u];
     };
     auto take = [&]() __attribute__((always_inline)) {                         // the sum of the WD parts, in the same order in each of the waves
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u)
+        for (int u = 0; u < SUBS; ++u) {
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < ACC; i += 4) {
-                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < WD; ++w)
-                    sum += *reinterpret_cast<const f32x4*>(exch + ((wq * WD + w) * SUBS * ACC + u * ACC + i) * 64 + lane * 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[u][i + e] = sum[e];
-            }
+            for (int w = 0; w < WD; ++w) sum += *reinterpret_cast<const f32x4*>(exch + ((wq * WD + w) * SUBS + u) * 256 + lane * 4);
+            s[u] = sum;
+        }
     };
     // The softmax of the newest tile, in pieces that the products of the tile before it can hide: 0 the logits and the lane's
     // maximum, 1 the query's maximum, then a weight of each sub-tile at a time.
-    constexpr int PIECES = 2 + ACC;
+    constexpr int PIECES = 2 + 4;
     float top = -INFINITY, base = 0.f, sum = 0.f;
     auto softmax = [&](int t, int piece) __attribute__((always_inline)) {
         if (piece == 0) {
@@ -232,14 +237,14 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
 #pragma unroll
             for (int u = 0; u < SUBS; ++u)
 #pragma unroll
-                for (int i = 0; i < ACC; ++i) {
-                    if (L2) s[u][i] = fmaf(2.f, s[u][i], -nrm[L2 ? u : 0][L2 ? i : 0]);
-                    s[u][i] = u * QT + 8 * (i >> 2) + (i & 3) < left ? s[u][i] : -INFINITY;
+                for (int i = 0; i < 4; ++i) {
+                    if (L2) s[u][i] = fmaf(2.f, s[u][i], -nrm[L2 ? u : 0][i]);
+                    s[u][i] = u * 16 + i < left ? s[u][i] : -INFINITY;
                     top = fmaxf(top, s[u][i]);
                 }
         } else if (piece == 1) {
-#pragma unroll
-            for (int w = QT; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
             const bool lift = (top - m) * c.k2 > LIFT;         // (m = -inf: nothing but zeros has been added)
             lifted = lift && m != -INFINITY;
             m_next = lift ? top : m;
@@ -254,26 +259,56 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
             }
         }
     };
-    // O^T += of the tile at xs with the weights p; beside it the softmax of tile t (next).  A step is four rows of every
-    // lane and one column tile.
-    constexpr int STEPS = SUBS * ACC / 4, AHEAD = QT == 32 ? 1 : 2, MID = WD > 1 ? NCT / 2 * STEPS : 0;
-    auto add_rows = [&](const float* xs, const acc_t* p, int t, bool next) __attribute__((always_inline)) {
-        float b[AHEAD + 1][4];
-        auto read = [&](int st, float* to) __attribute__((always_inline)) {
-            const int j = st / STEPS, u = st % STEPS / (ACC / 4), h = st % (ACC / 4);
+    // O^T += of the tile at xs with the weights p; beside it the softmax of tile t (next).  A step is a column tile and
+    // sixteen rows (bfloat16: 32).
+    constexpr int STEPS = BF ? SUBS / 2 : SUBS, AHEAD = 2, MID = WD > 1 ? NCT / 2 * STEPS : 0;
+    auto add_rows = [&](const char* xs, const f32x4* p, int t, bool next) __attribute__((always_inline)) {
+        u32x4 b[AHEAD + 1], hi[BF ? STEPS : 1], lo[BF ? STEPS : 1];
+        if constexpr (BF) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[i] = xs[(u * QT + 8 * h) * 32 + off_p[j % PP][i] + (j / PP) * RT * 32];
+            for (int k = 0; k < STEPS; ++k) {
+                bf16x8 h, r;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float v = p[2 * k + (e >> 2)][e & 3];
+                    h[e] = (__bf16)v;
+                    r[e] = (__bf16)(v - (float)h[e]);
+                }
+                hi[k] = __builtin_bit_cast(u32x4, h);
+                lo[k] = __builtin_bit_cast(u32x4, r);
+            }
+        }
+        auto read = [&](int st, u32x4* to) __attribute__((always_inline)) {
+            const int j = st / STEPS, k = st % STEPS;
+            const char* from = xs + (j / PP) * BLOCK;
+            if constexpr (BF) {
+                s16x4 v[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4*)(from + off_p[j % PP][0] + (2 * k + h) * 16 * 128));
+                *to = __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) (*to)[i] = *reinterpret_cast<const unsigned*>(from + off_p[j % PP][BF ? 0 : i] + k * 16 * 128);
+            }
         };
 #pragma unroll
-        for (int st = 0; st < AHEAD; ++st) read(st, b[st]);
+        for (int st = 0; st < AHEAD; ++st) read(st < NCT * STEPS ? st : 0, &b[st]);
 #pragma unroll
         for (int st = 0; st < NCT * STEPS; ++st) {
             const int j = st / STEPS, k = st % STEPS;
             if (WD > 1 && st == MID && next) take();
-            if (st + AHEAD < NCT * STEPS) read(st + AHEAD, b[(st + AHEAD) % (AHEAD + 1)]);
+            if (st + AHEAD < NCT * STEPS) read(st + AHEAD, &b[(st + AHEAD) % (AHEAD + 1)]);
             __builtin_amdgcn_sched_barrier(0);
+            const u32x4 a = b[st % (AHEAD + 1)];
+            if constexpr (BF) {
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, lo[k]), o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, hi[k]), o[j], 0, 0, 0);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[j] = M::mma(b[st % (AHEAD + 1)][i], p[k / (ACC / 4)][k % (ACC / 4) * 4 + i], o[j]);
+                for (int i = 0; i < 4; ++i) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), p[k][i], o[j], 0, 0, 0);
+            }
             if (next && st >= MID && st - MID < PIECES) softmax(t, st - MID);
         }
         if (next)
@@ -293,20 +328,17 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
         if (GRAD) {
             float* to = c.part_o + at * c.ld;
             int col0 = wd * CW + 4 * kl, end = qi < c.m ? c.ld : 0;
-            asm volatile("" : "+v"(col0), "+v"(end));    // (else 48 addresses are kept in registers over the whole loop)
+            asm volatile("" : "+v"(col0), "+v"(end));    // (else the addresses are kept in registers over the whole loop)
 #pragma unroll
-            for (int j = 0; j < NCT; ++j)
-#pragma unroll
-                for (int i = 0; i < ACC; i += 4) {
-                    const int col = col0 + j * QT + 8 * (i >> 2);
-                    if (col < end) {
-                        f32x4 v = {o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
-                        if (!fresh) v += *reinterpret_cast<const f32x4*>(to + col) * before;
-                        *reinterpret_cast<f32x4*>(to + col) = v;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][i + e] = 0.f;
+            for (int j = 0; j < NCT; ++j) {
+                const int col = col0 + j * 16;
+                if (col < end) {
+                    f32x4 v = o[j];
+                    if (!fresh) v += *reinterpret_cast<const f32x4*>(to + col) * before;
+                    *reinterpret_cast<f32x4*>(to + col) = v;
                 }
+                o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
         }
         fresh = false;
     };
@@ -317,10 +349,10 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
         l += sum;                               // this lane's rows; the lanes of a query are added at the end
     };
 
-    constexpr bool PIPE = NB == 3 && GRAD && QT * CW <= 32 * 256;
+    constexpr bool PIPE = pipelined(WQ, WD, CW, RT, NB) && GRAD;
     if (PIPE) {
-        // Tile t's products for O run beside the softmax of tile t + 1, whose S came first: three tiles in the ring (t, t + 1,
-        // and t + 2 on its way).
+        // Few waves on a CU: tile t's products for O run beside the softmax of tile t + 1, whose S came first (three tiles in
+        // the ring: t, t + 1, and t + 2 on its way).
 #pragma unroll
         for (int a = 0; a < LOADS; ++a) fetch1(0, 0, a);
         wait_meet<0>();
@@ -336,11 +368,10 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
         int slot = 0;                           // t % NB
         for (int t = 0; t < tiles; ++t) {
             const int slot1 = slot + 1 < NB ? slot + 1 : 0, slot2 = slot1 + 1 < NB ? slot1 + 1 : 0;
-            acc_t p[SUBS];
+            f32x4 p[SUBS];
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) p[u] = s[u];
-            const bool more = t + 1 < tiles;
-            if (more) {
+            if (t + 1 < tiles) {
                 wait_meet<0>();                 // tile t + 1 is there, nobody reads tile t - 1 any more
                 if (L2) norms(t + 1);
                 product(lds + slot1 * TILE, t + 2 < tiles ? t + 2 : 0, slot2);
@@ -353,20 +384,21 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
             slot = slot1;
         }
     } else {
-        int slot = 0;
-        if (NB > 1)
+        // NB == 2, 3: tiles t and, on its way, t + NB - 1; NB == 1: no room for another
 #pragma unroll
-            for (int a = 0; a < LOADS; ++a) fetch1(0, 0, a);
+        for (int b = 0; b < NB - 1; ++b)
+#pragma unroll
+            for (int a = 0; a < LOADS; ++a) fetch1(b < tiles ? b : 0, b, a);
+        int slot = 0;
         for (int t = 0; t < tiles; ++t) {
-            wait_meet<0>();                     // NB > 1: tile t is there; nobody reads the tile before any more
+            wait_meet<(NB > 1 ? (NB - 2) * LOADS : 0)>();   // NB > 1: tile t is there; nobody reads the tile before any more
             if (NB == 1) {
 #pragma unroll
                 for (int a = 0; a < LOADS; ++a) fetch1(t, 0, a);
                 wait_meet<0>();
             }
             if (L2) norms(t);
-            const int next = NB > 1 && slot + 1 < NB ? slot + 1 : 0;
-            product(lds + slot * TILE, t + 1 < tiles ? t + 1 : 0, next);
+            product(lds + slot * TILE, t + NB - 1 < tiles ? t + NB - 1 : 0, slot > 0 ? slot - 1 : NB - 1);
             if (WD > 1) {
                 give();
                 take();
@@ -375,13 +407,13 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_f32_kernel(TileCall c) {
             for (int piece = 0; piece < PIECES; ++piece) softmax(t, piece);
             advance(t);
             if (GRAD) add_rows(lds + slot * TILE, s, t, false);
-            slot = next;
+            slot = slot + 1 < NB ? slot + 1 : 0;
         }
     }
     put_down();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no LDS-DMA outlives the workgroup
-#pragma unroll
-    for (int w = QT; w < 64; w *= 2) l_part += __shfl_xor(l_part, w);
+    l_part += __shfl_xor(l_part, 16);
+    l_part += __shfl_xor(l_part, 32);
     if (qi < c.m && kl == 0 && wd == 0) {
         c.part_ml[2 * at] = m_part;
         c.part_ml[2 * at + 1] = l_part;

@@ -1,0 +1,37 @@
+// distill_variants.h -- the instances of tile_kernel (distill_tile.h) for one storage type (distill_tile_f32.hip, _bf16.hip).
+#pragma once
+#include "distill_tile.h"
+
+#include <algorithm>
+
+namespace rag {
+namespace distill {
+
+typedef void (*kernel_t)(TileCall);
+struct Variant {
+    int wq, wd, cw, rt, lds;
+    kernel_t fn[2][2];   // [grad][l2]
+};
+extern const Variant* const VARIANTS_F32;
+extern const int N_VARIANTS_F32;
+extern const Variant* const VARIANTS_BF16;
+extern const int N_VARIANTS_BF16;
+
+constexpr int LDS_MAX = 160 * 1024;
+constexpr int exch_bytes(int wq, int wd, int rt) { return wd > 1 ? wq * wd * (rt / 16) * 1024 : 0; }
+// tiles of the ring: three where they fit, else what does
+constexpr int ring(int wq, int wd, int cw, int rt, int esz) {
+    return std::min(3, (LDS_MAX - exch_bytes(wq, wd, rt)) / (rt * cw * wd * esz));
+}
+
+template <typename T, int WQ, int WD, int CW, int RT>
+Variant variant() {
+    constexpr int E = sizeof(T), NB = ring(WQ, WD, CW, RT, E);
+    static_assert(NB >= 1, "tile does not fit");
+    return Variant{WQ, WD, CW, RT, NB * RT * CW * WD * E + exch_bytes(WQ, WD, RT),
+                   {{tile_kernel<T, WQ, WD, CW, RT, NB, false, false>, tile_kernel<T, WQ, WD, CW, RT, NB, false, true>},
+                    {tile_kernel<T, WQ, WD, CW, RT, NB, true, false>, tile_kernel<T, WQ, WD, CW, RT, NB, true, true>}}};
+}
+
+}  // namespace distill
+}  // namespace rag
