@@ -11,11 +11,12 @@
 // o = sum_j exp(s_ij - m) x_j, rescaled when m grows.  The index is split over workgroups; a join kernel adds the parts.
 // All sums, statistics and the row sum are fp32; dq is rounded once, to the type of q.
 #include "common.h"
-#include "distill_tile.h"
+#include "distill_rows.h"
 
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace {
 
@@ -107,127 +108,277 @@ struct Call {
     long long rows_per_split;
 };
 
-// The teacher's side of one query, by the whole workgroup: p_of[k] in LDS and the log of its normaliser.  Returns 1, or 0
-// (no entry of finite score) or NaN (a row number outside the index); the barriers inside publish p_of.
-template <int W>
-__device__ __forceinline__ float teacher(const Call& c, long long i, float* p_of, float* red, float* zmax_out, float* log_zsum) {
-    const int tid = threadIdx.x;
-    const long long* ids = c.ids + i * c.k;
-    const float* z = c.scores + i * c.k;
-    float zmax = -INFINITY, any = 0.f, bad = 0.f;
-    for (int k = tid; k < c.k; k += W * 64) {
+// The teacher's side of one query, by each wave for itself (lists are short, a barrier costs more): the maximum and the sum
+// of its softmax.  Returns 1, or 0 (no entry of finite score) or NaN (a row number outside the index).
+__device__ __forceinline__ float teacher(const Call& c, const long long* ids, const float* z, float* zmax, float* zsum) {
+    const int lane = threadIdx.x & 63;
+    float top = -INFINITY;
+    bool any = false, bad = false;
+    for (int k = lane; k < c.k; k += 64) {
         const long long id = ids[k];
-        if (id < -1 || id >= c.n) bad = 1.f;
-        else if (id >= 0) {
-            const float v = z[k] * c.beta_t;
-            zmax = fmaxf(zmax, v);
-            if (!(v == -INFINITY)) any = 1.f;
+        const float v = z[k] * c.beta_t;
+        bad |= id < -1 || id >= c.n;
+        if (id >= 0) {
+            top = fmaxf(top, v);
+            any |= !(v == -INFINITY);
         }
     }
-    zmax = block_max<W>(zmax, red);
-    any = block_max<W>(any, red);
-    bad = block_max<W>(bad, red);
-    if (bad != 0.f) return NAN;
-    if (any == 0.f) return 0.f;
-    float zsum = 0.f;
-    for (int k = tid; k < c.k; k += W * 64) {
-        const float e = ids[k] >= 0 ? expf(z[k] * c.beta_t - zmax) : 0.f;
-        p_of[k] = e;
-        zsum += e;
-    }
-    zsum = block_sum<W>(zsum, red);
-    for (int k = tid; k < c.k; k += W * 64) p_of[k] /= zsum;   // (each thread its own)
-    __syncthreads();
-    *zmax_out = zmax;
-    *log_zsum = logf(zsum);
+    if (__any(bad)) return NAN;
+    if (!__any(any)) return 0.f;
+    top = wave_max(top);
+    float sum = 0.f;
+    for (int k = lane; k < c.k; k += 64) sum += ids[k] >= 0 ? expf(z[k] * c.beta_t - top) : 0.f;
+    *zmax = top;
+    *zsum = wave_sum(sum);
     return 1.f;
 }
+// p and p (log p - s) of an entry
+__device__ __forceinline__ float prob(const Call& c, float z, float zmax, float zsum) { return expf(z * c.beta_t - zmax) / zsum; }
+__device__ __forceinline__ float cross(const Call& c, float z, float p, float s, float zmax, float log_zsum) {
+    return p != 0.f ? p * (z * c.beta_t - zmax - log_zsum - s) : 0.f;   // (NaN enters)
+}
 
-// s_of[k]: the student's logits of the list's entries, a wave per entry; qs holds the query.
+// over = the list: one workgroup per query.  LPR lanes hold a row (NP pieces of 16 bytes each) and their columns of the query and of
+// two sums, sum exp(s - m) x and sum p x: every row is read once, the next two are on their way while one is used.
+template <typename T, int LPR, int NP, bool GRAD>
+__global__ __launch_bounds__(512) void list_rows_kernel(Call c) {
+    typedef distill::RowPiece<T> P;
+    typedef typename P::raw raw;
+    constexpr int E = P::E, RPW = 64 / LPR;
+    extern __shared__ __align__(16) char raw_lds[];
+    long long* ids = reinterpret_cast<long long*>(raw_lds);         // k
+    float* z = reinterpret_cast<float*>(ids + c.k);            // k
+    float* p_of = z + c.k;                                     // k
+    float* lds = p_of + c.k;                                   // GRAD: waves x ld
+    __shared__ float mlh[8][3];
+    const long long i = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6, li = lane % LPR;
+    const int group = wave * RPW + lane / LPR, groups = waves * RPW;
+    const T* x = static_cast<const T*>(c.x);
+    const T* qp = static_cast<const T*>(c.q) + i * c.ldq;
+    for (int k = tid; k < c.k; k += blockDim.x) {
+        ids[k] = c.ids[i * c.k + k];
+        z[k] = c.scores[i * c.k + k];
+    }
+    T* dq = GRAD ? static_cast<T*>(c.dq) + i * c.lddq : nullptr;
+    int col[NP];
+    bool mine[NP];
+#pragma unroll
+    for (int a = 0; a < NP; ++a) {
+        col[a] = (li + LPR * a) * E;
+        mine[a] = col[a] < c.ld;
+        if (!mine[a]) col[a] = c.ld - E;
+    }
+    raw next[2][NP];
+    auto fetch = [&](int k, raw* to) {        // (an entry that is none takes row 0, if there is one; it is not used)
+        long long id = k < c.k ? ids[k] : 0;
+        id = id >= 0 && id < c.n ? id : 0;
+#pragma unroll
+        for (int a = 0; a < NP; ++a) to[a] = *reinterpret_cast<const raw*>(x + id * c.ld + col[a]);
+    };
+    __syncthreads();
+    if (c.n > 0) {
+        fetch(group, next[0]);
+        fetch(group + groups, next[1]);
+    }
+    float zmax, zsum;
+    const float live = teacher(c, ids, z, &zmax, &zsum);
+    if (!(live == 1.f)) {                     // (uniform) nothing to learn from, or a row number outside the index
+        if (tid == 0) c.loss[i] = live;
+        if (GRAD)
+            for (int j = tid; j < c.d; j += blockDim.x) store1(dq + j, live);
+        return;
+    }
+    const float log_zsum = logf(zsum);
+    for (int k = tid; k < c.k; k += blockDim.x) p_of[k] = ids[k] >= 0 ? prob(c, z[k], zmax, zsum) : 0.f;
+    float q[NP * E];
+#pragma unroll
+    for (int a = 0; a < NP; ++a)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float v = load1(qp + min(col[a] + e, c.d - 1));
+            q[a * E + e] = mine[a] && col[a] + e < c.d ? v : 0.f;
+        }
+    __syncthreads();
+    // m is a reference that moves when a logit lies more than 2^40 above it (weights up to there lose nothing)
+    const float k2 = 1.44269504f;
+    float m = -INFINITY, l = 0.f, head = 0.f, o[GRAD ? NP * E : 1] = {}, w[GRAD ? NP * E : 1] = {};
+    for (int k = group; k - group < c.k; k += groups) {      // (every group goes round equally often)
+        raw now[NP];
+#pragma unroll
+        for (int a = 0; a < NP; ++a) {
+            now[a] = next[0][a];
+            next[0][a] = next[1][a];
+        }
+        if (k - group + 2 * groups < c.k) fetch(k + 2 * groups, next[1]);
+        const int at = k < c.k ? k : 0;
+        const bool real = k < c.k && ids[at] >= 0;
+        const float p = p_of[at];
+        float v[NP * E], part[2] = {0.f, 0.f};
+#pragma unroll
+        for (int a = 0; a < NP; ++a) P::widen(now[a], v + a * E);
+#pragma unroll
+        for (int j = 0; j < NP * E; ++j) {
+            if (c.l2) {
+                const float t = mine[j / E] ? q[j] - v[j] : 0.f;     // (pad columns are zero on both sides)
+                part[j & 1] = fmaf(t, t, part[j & 1]);
+            } else {
+                part[j & 1] = fmaf(q[j], v[j], part[j & 1]);
+            }
+        }
+        const float dot = distill::group_sum<LPR>(part[0] + part[1]);
+        const float s = real ? (c.l2 ? -c.beta * dot : c.beta * dot) : -INFINITY;
+        if (real) head += cross(c, z[at], p, s, zmax, log_zsum);
+        const bool lift = (s - m) * k2 > 40.f;
+        if (__any(lift)) {
+            const float scale = lift ? __builtin_amdgcn_exp2f((m - s) * k2) : 1.f;
+            m = lift ? s : m;
+            l *= scale;
+            if (GRAD)
+#pragma unroll
+                for (int j = 0; j < NP * E; ++j) o[j] *= scale;
+        }
+        if (real) {
+            const float e = __builtin_amdgcn_exp2f((s - (m == -INFINITY ? 0.f : m)) * k2);
+            l += e;
+            if (GRAD)
+#pragma unroll
+                for (int j = 0; j < NP * E; ++j) {
+                    o[j] = fmaf(e, v[j], o[j]);
+                    w[j] = fmaf(p, v[j], w[j]);
+                }
+        }
+    }
+    // the groups of a wave, then the waves
+    float all = m;
+#pragma unroll
+    for (int d = LPR; d < 64; d *= 2) all = fmaxf(all, __shfl_xor(all, d));
+    float mass = l * expf(m - (all == -INFINITY ? 0.f : all));
+#pragma unroll
+    for (int d = LPR; d < 64; d *= 2) {
+        mass += __shfl_xor(mass, d);
+        head += __shfl_xor(head, d);
+    }
+    if (lane == 0) {
+        mlh[wave][0] = all;
+        mlh[wave][1] = mass;
+        mlh[wave][2] = head;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int a = 0; a < waves; ++a) top = fmaxf(top, mlh[a][0]);
+    const float base = top == -INFINITY ? 0.f : top;
+    mass = head = 0.f;
+    for (int a = 0; a < waves; ++a) {
+        mass = fmaf(mlh[a][1], expf(mlh[a][0] - base), mass);
+        head += mlh[a][2];
+    }
+    if (tid == 0) c.loss[i] = head + top + logf(mass);
+    if (!GRAD) return;
+    const float share = expf(m - base) / mass;
+#pragma unroll
+    for (int j = 0; j < NP * E; ++j) {
+        o[GRAD ? j : 0] = fmaf(o[GRAD ? j : 0], share, -w[GRAD ? j : 0]);
+#pragma unroll
+        for (int d = LPR; d < 64; d *= 2) o[GRAD ? j : 0] += __shfl_xor(o[GRAD ? j : 0], d);
+    }
+    if (lane < LPR)
+#pragma unroll
+        for (int a = 0; a < NP; ++a)
+            if (mine[a])
+#pragma unroll
+                for (int e = 0; e < E; ++e) lds[wave * c.ld + col[a] + e] = o[GRAD ? a * E + e : 0];
+    __syncthreads();
+    const float f = (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f);
+    for (int j = tid; j < c.d; j += blockDim.x) {
+        float sum = 0.f;
+        for (int a = 0; a < waves; ++a) sum += lds[a * c.ld + j];
+        store1(dq + j, f * sum);
+    }
+}
+
+// s_of[k]: the student's logits of the list's entries, four entries a wave; qs holds the query.
 template <typename T, int W>
 __device__ __forceinline__ void list_logits(const Call& c, const long long* ids, const float* qs, float* s_of) {
     constexpr int E = Piece<T>::E;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int k = wave; k < c.k; k += W) {
-        const long long id = ids[k];
-        if (id < 0) continue;
-        const T* row = static_cast<const T*>(c.x) + id * c.ld;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15;
+    for (int k = wave * 4 + (lane >> 4); k - (lane >> 4) < c.k; k += 4 * W) {
+        const long long id = k < c.k ? ids[k] : -1;
+        const T* row = static_cast<const T*>(c.x) + (id >= 0 ? id : 0) * c.ld;
         float acc = 0.f;
-        for (int j = lane * E; j < c.ld; j += 64 * E) {
-            float v[E];
-            Piece<T>::load(row + j, v);
-            for (int e = 0; e < E; ++e) {
-                if (c.l2) {
-                    const float t = qs[j + e] - v[e];
-                    acc = fmaf(t, t, acc);
-                } else {
-                    acc = fmaf(qs[j + e], v[e], acc);
+        if (id >= 0)
+#pragma unroll 8
+            for (int j = li * E; j < c.ld; j += 16 * E) {
+                float v[E];
+                Piece<T>::load(row + j, v);
+                for (int e = 0; e < E; ++e) {
+                    if (c.l2) {
+                        const float t = qs[j + e] - v[e];
+                        acc = fmaf(t, t, acc);
+                    } else {
+                        acc = fmaf(qs[j + e], v[e], acc);
+                    }
                 }
             }
-        }
-        acc = wave_sum(acc);
-        if (lane == 0) s_of[k] = c.l2 ? -c.beta * acc : c.beta * acc;
+        acc = distill::group_sum<16>(acc);
+        if (li == 0 && k < c.k) s_of[k] = c.l2 ? -c.beta * acc : c.beta * acc;
     }
     __syncthreads();
 }
 
-// sum_k p_k (log p_k - s_k)
-template <int W>
-__device__ __forceinline__ float list_head(const Call& c, long long i, const float* p_of, const float* s_of, float zmax, float log_zsum,
-                                           float* red) {
-    float head = 0.f;
-    for (int k = threadIdx.x; k < c.k; k += W * 64)
-        if (p_of[k] != 0.f) head += p_of[k] * (c.scores[i * c.k + k] * c.beta_t - zmax - log_zsum - s_of[k]);   // (NaN enters)
-    return block_sum<W>(head, red);
-}
-
-// over = the list: one workgroup per query does it all.
+// over = the list, any row length: one workgroup per query; the rows are read twice.
 template <typename T>
-__global__ __launch_bounds__(THREADS) void list_kernel(Call c) {
+__global__ __launch_bounds__(THREADS) void list_any_kernel(Call c) {
     constexpr int E = Piece<T>::E;
     extern __shared__ float sh[];
     float* qs = sh;               // ld
     float* s_of = qs + c.ld;      // k
-    float* p_of = s_of + c.k;     // k
+    float* w_of = s_of + c.k;     // k
     __shared__ float red[WAVES];
     const long long i = blockIdx.x;
     const int tid = threadIdx.x;
     const T* x = static_cast<const T*>(c.x);
     const long long* ids = c.ids + i * c.k;
+    const float* z = c.scores + i * c.k;
     const T* q = static_cast<const T*>(c.q) + i * c.ldq;
     T* dq = c.dq ? static_cast<T*>(c.dq) + i * c.lddq : nullptr;
-    for (int j = tid; j < c.ld; j += THREADS) qs[j] = j < c.d ? load1(q + j) : 0.f;
-    float zmax, log_zsum;
-    const float live = teacher<WAVES>(c, i, p_of, red, &zmax, &log_zsum);   // (its barriers also publish qs)
-    if (!(live == 1.f)) {         // (uniform) nothing to learn from, or a row number outside the index
+    float zmax, zsum;
+    const float live = teacher(c, ids, z, &zmax, &zsum);
+    if (!(live == 1.f)) {         // (uniform)
         if (tid == 0) c.loss[i] = live;
         if (dq)
             for (int j = tid; j < c.d; j += THREADS) store1(dq + j, live);
         return;
     }
+    for (int j = tid; j < c.ld; j += THREADS) qs[j] = j < c.d ? load1(q + j) : 0.f;
+    __syncthreads();
     list_logits<T, WAVES>(c, ids, qs, s_of);
-    float smax = -INFINITY, mass = 0.f;
+    float smax = -INFINITY, mass = 0.f, head = 0.f;
     for (int k = tid; k < c.k; k += THREADS)
         if (ids[k] >= 0) smax = fmaxf(smax, s_of[k]);
     smax = block_max<WAVES>(smax, red);
     for (int k = tid; k < c.k; k += THREADS)
-        if (ids[k] >= 0) mass += expf(s_of[k] - smax);
+        if (ids[k] >= 0) {
+            mass += expf(s_of[k] - smax);
+            head += cross(c, z[k], prob(c, z[k], zmax, zsum), s_of[k], zmax, logf(zsum));
+        }
     mass = block_sum<WAVES>(mass, red);
-    const float head = list_head<WAVES>(c, i, p_of, s_of, zmax, log_zsum, red);
+    head = block_sum<WAVES>(head, red);
     if (tid == 0) c.loss[i] = head + smax + logf(mass);
     if (!dq) return;
     for (int k = tid; k < c.k; k += THREADS)
-        if (ids[k] >= 0) p_of[k] = expf(s_of[k] - smax) / mass - p_of[k];
+        w_of[k] = ids[k] >= 0 ? expf(s_of[k] - smax) / mass - prob(c, z[k], zmax, zsum) : 0.f;
     __syncthreads();
     const float f = (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f);
     for (int j = tid * E; j < c.ld; j += THREADS * E) {
         float acc[E] = {};
+#pragma unroll 4
         for (int k = 0; k < c.k; ++k) {
             const long long id = ids[k];
             if (id < 0) continue;
             float v[E];
             Piece<T>::load(x + id * c.ld + j, v);
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(p_of[k], v[e], acc[e]);
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(w_of[k], v[e], acc[e]);
         }
         for (int e = 0; e < E; ++e)
             if (j + e < c.d) store1(dq + j + e, f * acc[e]);
@@ -303,42 +454,43 @@ __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
 }
 
 // Adds the shares' parts and takes the teacher's side off: one workgroup per query and 64 columns, each wave adds every
-// eighth share (list entry); the first of a query's workgroups computes the loss.
-constexpr int JOIN_WAVES = 8, JOIN_THREADS = 64 * JOIN_WAVES;
-template <typename T>
-__global__ __launch_bounds__(JOIN_THREADS) void join_kernel(Call c) {
+// JOIN_WAVES-th share and list entry; one more workgroup per query computes the loss.
+template <typename T, int JOIN_WAVES, int CPL>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void join_kernel(Call c) {
+    constexpr int JOIN_THREADS = 64 * JOIN_WAVES;
     extern __shared__ float sh[];
     __shared__ float red[JOIN_WAVES];
-    __shared__ float cols[2][JOIN_WAVES][64];
-    float* w_of = sh;                 // splits
-    float* p_of = w_of + c.splits;    // k
-    float* s_of = p_of + c.k;         // k
-    float* qs = s_of + c.k;           // ld
+    __shared__ float cols[JOIN_WAVES][64 * CPL][2];
     const long long i = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    T* dq = c.dq ? static_cast<T*>(c.dq) + i * c.lddq : nullptr;
+    const bool loss = blockIdx.y == 0;
     const long long* ids = c.ids + i * c.k;
-    const int col = blockIdx.y * 64 + lane;
-    float zmax, log_zsum;
-    const float live = teacher<JOIN_WAVES>(c, i, p_of, red, &zmax, &log_zsum);
+    const float* z = c.scores + i * c.k;
+    const T* q = static_cast<const T*>(c.q) + i * c.ldq;
+    T* dq = c.dq ? static_cast<T*>(c.dq) + i * c.lddq : nullptr;
+    const int col = (((int)blockIdx.y - 1) * 64 + lane) * CPL;
+    float zmax, zsum;
+    const float live = teacher(c, ids, z, &zmax, &zsum);
     if (!(live == 1.f)) {             // (uniform)
-        if (tid == 0 && blockIdx.y == 0) c.loss[i] = live;
-        if (dq && wave == 0 && col < c.d) store1(dq + col, live);
+        if (tid == 0 && loss) c.loss[i] = live;
+        if (!loss && wave == 0)
+            for (int e = 0; e < CPL; ++e)
+                if (col + e < c.d) store1(dq + col + e, live);
         return;
     }
+    // the shares' references and sums, by each wave for itself
     float m = -INFINITY, l = 0.f;
-    for (int s = tid; s < c.splits; s += JOIN_THREADS) m = fmaxf(m, c.part_ml[2 * (s * c.m + i)]);
-    m = block_max<JOIN_WAVES>(m, red);
-    for (int s = tid; s < c.splits; s += JOIN_THREADS) {
+    for (int s = lane; s < c.splits; s += 64) m = fmaxf(m, c.part_ml[2 * (s * c.m + i)]);
+    m = wave_max(m);
+    for (int s = lane; s < c.splits; s += 64) {
         const float ms = c.part_ml[2 * (s * c.m + i)], ls = c.part_ml[2 * (s * c.m + i) + 1];
-        const float w = ms == -INFINITY ? 0.f : expf((ms - m) * c.beta);
-        w_of[s] = w;
-        l += w * ls;
+        l += (ms == -INFINITY ? 0.f : expf((ms - m) * c.beta)) * ls;
     }
-    l = block_sum<JOIN_WAVES>(l, red);   // (publishes w_of)
-    if (blockIdx.y == 0) {
-        const T* q = static_cast<const T*>(c.q) + i * c.ldq;
-        float qq = 0.f;
+    l = wave_sum(l);
+    if (loss) {
+        float* s_of = sh;                 // k
+        float* qs = s_of + c.k;           // ld
+        float qq = 0.f, head = 0.f;
         for (int j = tid; j < c.ld; j += JOIN_THREADS) {
             const float v = j < c.d ? load1(q + j) : 0.f;
             qs[j] = v;
@@ -346,28 +498,49 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(Call c) {
         }
         qq = block_sum<JOIN_WAVES>(qq, red);
         list_logits<T, JOIN_WAVES>(c, ids, qs, s_of);
-        const float head = list_head<JOIN_WAVES>(c, i, p_of, s_of, zmax, log_zsum, red);
+        const float log_zsum = logf(zsum);
+        for (int k = tid; k < c.k; k += JOIN_THREADS)
+            if (ids[k] >= 0) head += cross(c, z[k], prob(c, z[k], zmax, zsum), s_of[k], zmax, log_zsum);
+        head = block_sum<JOIN_WAVES>(head, red);
         if (tid == 0) c.loss[i] = head + c.beta * (c.l2 ? m - qq : m) + logf(l);
+        return;
     }
-    if (!dq) return;
-    float o = 0.f, a = 0.f;
-    if (col < c.ld) {
+    float o[CPL] = {}, a[CPL] = {};
+    const int at = min(col, c.ld - CPL);     // (rows are padded to 16 bytes; columns behind the end are not stored)
 #pragma unroll 8
-        for (int s = wave; s < c.splits; s += JOIN_WAVES) o = fmaf(w_of[s], c.part_o[(s * c.m + i) * c.ld + col], o);
-#pragma unroll 4
-        for (int k = wave; k < c.k; k += JOIN_WAVES)
-            if (ids[k] >= 0) a = fmaf(p_of[k], load1(static_cast<const T*>(c.x) + ids[k] * c.ld + col), a);
+    for (int s = wave; s < c.splits; s += JOIN_WAVES) {
+        const float ms = c.part_ml[2 * (s * c.m + i)], f = ms == -INFINITY ? 0.f : expf((ms - m) * c.beta);
+        float v[CPL];
+        __builtin_memcpy(v, __builtin_assume_aligned(c.part_o + (s * c.m + i) * c.ld + at, CPL * 4), CPL * 4);
+#pragma unroll
+        for (int e = 0; e < CPL; ++e) o[e] = fmaf(f, v[e], o[e]);
     }
-    cols[0][wave][lane] = o;
-    cols[1][wave][lane] = a;
+#pragma unroll 8
+    for (int k = wave; k < c.k; k += JOIN_WAVES) {
+        const long long id = ids[k];
+        T v[CPL];
+        __builtin_memcpy(v, __builtin_assume_aligned(static_cast<const T*>(c.x) + max(id, 0ll) * c.ld + at, CPL * sizeof(T)), CPL * sizeof(T));
+        const float p = id >= 0 ? prob(c, z[k], zmax, zsum) : 0.f;
+#pragma unroll
+        for (int e = 0; e < CPL; ++e) a[e] = fmaf(p, id >= 0 ? load1(v + e) : 0.f, a[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < CPL; ++e) {
+        cols[wave][lane * CPL + e][0] = o[e];
+        cols[wave][lane * CPL + e][1] = a[e];
+    }
     __syncthreads();
-    if (wave != 0 || col >= c.d) return;
-    o = a = 0.f;
-    for (int w = 0; w < JOIN_WAVES; ++w) {
-        o += cols[0][w][lane];
-        a += cols[1][w][lane];
+    const float f = (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f);
+    for (int j = tid; j < 64 * CPL; j += JOIN_THREADS) {
+        const int to = ((int)blockIdx.y - 1) * 64 * CPL + j;
+        if (to >= c.d) break;
+        float so = 0.f, sa = 0.f;
+        for (int w = 0; w < JOIN_WAVES; ++w) {
+            so += cols[w][j][0];
+            sa += cols[w][j][1];
+        }
+        store1(dq + to, f * (so / l - sa));
     }
-    store1(dq + col, (c.weights ? c.weights[i] : 1.f) * c.beta * (c.l2 ? 2.f : 1.f) * (o / l - a));
 }
 
 // How a call is split; depends on the number of queries and the row length, not on the number of rows (the
@@ -404,11 +577,26 @@ struct Ctx {
     hipStream_t st;
 };
 
+template <int V> using Int = std::integral_constant<int, V>;
+
 template <typename T>
 int launch(Ctx& x) {
     Call& c = x.c;
     if (x.over == RAG_OVER_LIST) {
-        list_kernel<T><<<(unsigned)c.m, THREADS, ((size_t)c.ld + 2 * c.k) * sizeof(float), x.st>>>(c);
+        constexpr int E = Piece<T>::E;
+        auto rows = [&](auto lpr, auto np) {
+            if (lpr.value * np.value * E < c.ld) return false;
+            // waves: enough for the list's rows, but fewer (two rows or more each) where the queries fill the card
+            const int need = (c.k * lpr.value + 63) / 64, waves = std::max(1, std::min(c.m >= 1024 ? 4 : 8, need));
+            const size_t bytes = (size_t)c.k * 16 + (c.dq ? (size_t)waves * c.ld * sizeof(float) : 0);
+            if (c.dq) list_rows_kernel<T, lpr.value, np.value, true><<<(unsigned)c.m, 64 * waves, bytes, x.st>>>(c);
+            else list_rows_kernel<T, lpr.value, np.value, false><<<(unsigned)c.m, 64 * waves, bytes, x.st>>>(c);
+            return true;
+        };
+        const bool served = rows(Int<16>(), Int<1>()) || rows(Int<16>(), Int<2>()) || rows(Int<32>(), Int<2>()) ||
+                            rows(Int<32>(), Int<3>()) || rows(Int<32>(), Int<4>()) ||
+                            (E == 4 && (rows(Int<32>(), Int<6>()) || rows(Int<32>(), Int<8>())));
+        if (!served) list_any_kernel<T><<<(unsigned)c.m, THREADS, ((size_t)c.ld + 2 * c.k) * sizeof(float), x.st>>>(c);
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
@@ -442,8 +630,11 @@ int launch(Ctx& x) {
         else index_any_kernel<T, false><<<grid, THREADS, c.ld * sizeof(float), x.st>>>(c);
         RAG_HIP(hipGetLastError());
     }
-    const dim3 grid((unsigned)c.m, c.dq ? (unsigned)((c.ld + 63) / 64) : 1u);
-    join_kernel<T><<<grid, JOIN_THREADS, ((size_t)c.splits + 2 * c.k + c.ld) * sizeof(float), x.st>>>(c);
+    // (few queries have many shares each, and leave the card to them; many share a workgroup's chain of loads over more columns)
+    const size_t bytes = ((size_t)c.k + c.ld) * sizeof(float);
+    auto grid = [&](int cols) { return dim3((unsigned)c.m, c.dq ? 1u + (unsigned)((c.d + cols - 1) / cols) : 1u); };
+    if (c.m <= 64) join_kernel<T, 16, 1><<<grid(64), 64 * 16, bytes, x.st>>>(c);
+    else join_kernel<T, 8, 4><<<grid(256), 64 * 8, bytes, x.st>>>(c);
     RAG_HIP(hipGetLastError());
     return RAG_OK;
 }

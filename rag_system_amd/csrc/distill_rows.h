@@ -54,7 +54,7 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-constexpr int ROWS_WAVES = 4;
+constexpr int ROWS_WAVES = 8;
 
 template <typename T, int LPR, int NP, int MQ, bool GRAD, bool L2>
 __global__ __launch_bounds__(64 * ROWS_WAVES) void rows_kernel(TileCall c) {

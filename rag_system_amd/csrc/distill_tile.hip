@@ -66,7 +66,7 @@ bool tile_plan(long long m, int ld, bool bf16, TilePlan* p) {
     if (m <= 4)
         for (int v = 0; v < N_FEW; ++v)
             if ((FEW[v].bf16 != 0) == bf16 && FEW[v].lpr * FEW[v].np * (bf16 ? 8 : 4) >= ld) {
-                *p = TilePlan{v, true, bf16, 64 / FEW[v].lpr * ROWS_WAVES, num_cus() * 4, 1};
+                *p = TilePlan{v, true, bf16, 64 / FEW[v].lpr * ROWS_WAVES, num_cus() * 2, 1};
                 return true;
             }
     // The variant with the least work for these queries: whole groups of them, whole columns, over the rate its groups reach
