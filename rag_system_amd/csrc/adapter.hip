@@ -7,177 +7,494 @@
 //     v_t = c_s B_s^T dy_t              dx_t = W^T dy_t + A_s^T v_t
 //     dA_s = sum_t v_t x_t^T            dB_s = sum_t dy_t u_t^T      over the requests of slot s.
 // u, v, dA, dB and every sum are fp32; y and dx are rounded once, to the type of x.
-#include "common.h"
+#include "adapter_gemm.h"
 
 #include <algorithm>
 
 namespace {
 
 using namespace rag;
+using namespace rag::adapter;
 
-constexpr int THREADS = 256;
-
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ float load1(const unsigned short* p) { return __uint_as_float((unsigned)*p << 16); }
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store1(unsigned short* p, float f) {
-    const unsigned u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) *p = (unsigned short)((u >> 16) | 0x40);   // NaN stays NaN
-    else *p = (unsigned short)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
-}
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-struct Call {
-    long long n, ldx, ldy, lddy, lddx;
-    int d_in, d_out, slots_n, rank;
-    const void *x, *w, *a, *b, *dy;
-    const float* scale;
+// ---- order: requests sorted by slot, in the order they came within a slot ------------------------------------------
+//
+// A counting sort over bins 0 .. slots - 1, slots (none), slots + 1 (outside the bank).  A wave counts a chunk of requests,
+// every bin's counts are summed over the chunks, and the wave puts its requests where the sums say: no atomics, so equal
+// calls give equal orders.  For the gradients a slot's requests are dealt out as items of `len` (an empty slot is one item,
+// which writes zeros).
+struct Item {
+    int slot, begin, end, part;   // part: -1, or the partial sum it writes (its slot has several items)
+};
+struct Sort {
     const long long* slots;
-    void *y, *dx;
-    float *da, *db;
-    float *u, *v;   // n x R
+    int n, n_slots, chunk, chunks, len;
+    int *perm, *slot_at, *counts, *start;   // counts: chunks x (slots + 2); start: slots + 3
+    int2* parts;                            // per slot: first partial, number of partials (0: none)
+    int* n_items;
+    Item* items;
 };
-
-// slot of a request: >= 0, -1 (none) or -2 (outside the bank: its results are NaN)
-__device__ __forceinline__ int slot_of(const Call& c, long long t) {
-    const long long s = c.slots[t];
-    return s >= -1 && s < c.slots_n ? (int)s : -2;
+__device__ __forceinline__ int bin_of(const Sort& s, int t) {
+    const long long v = s.slots[t];
+    return v >= 0 && v < s.n_slots ? (int)v : v == -1 ? s.n_slots : s.n_slots + 1;
 }
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void down_kernel(Call c) {
-    const long long t = blockIdx.x;
-    const int s = slot_of(c, t), lane = threadIdx.x & 63;
-    const T* x = static_cast<const T*>(c.x) + t * c.ldx;
-    for (int r = threadIdx.x >> 6; r < c.rank; r += THREADS / 64) {
-        float acc = 0.f;
-        if (s >= 0) {
-            const T* a = static_cast<const T*>(c.a) + ((long long)s * c.rank + r) * c.d_in;
-            for (int j = lane; j < c.d_in; j += 64) acc = fmaf(load1(a + j), load1(x + j), acc);
-            acc = wave_sum(acc) * c.scale[s];
+// lane's place among the lanes of its bin, and their number
+__device__ __forceinline__ int place_in_wave(int bin, bool live, int* of) {
+    const int lane = threadIdx.x & 63;
+    unsigned long long todo = __ballot(live);
+    int at = 0;
+    while (todo) {
+        const int b = __shfl(bin, __ffsll((long long)todo) - 1);
+        const unsigned long long with = __ballot(live && bin == b);
+        if (live && bin == b) {
+            at = __popcll(with & ((1ull << lane) - 1));
+            *of = __popcll(with);
         }
-        if (lane == 0) c.u[t * c.rank + r] = s == -2 ? NAN : acc;
+        todo &= ~with;
+    }
+    return at;
+}
+// counts[] += this wave's chunk; the last lane of a bin adds for all of them (one writer, no atomics)
+__device__ __forceinline__ void count_chunk(const Sort& s, int c, int* counts) {
+    const int lane = threadIdx.x & 63, end = min(s.n, (c + 1) * s.chunk);
+    for (int t0 = c * s.chunk; t0 < end; t0 += 64) {
+        const bool live = t0 + lane < end;
+        const int bin = live ? bin_of(s, t0 + lane) : -1;
+        int of = 0;
+        const int at = place_in_wave(bin, live, &of);
+        if (live && at == of - 1) counts[bin] += of;
     }
 }
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void apply_kernel(Call c) {
-    const long long t = blockIdx.x;
-    const int s = slot_of(c, t), lane = threadIdx.x & 63;
-    const T* x = static_cast<const T*>(c.x) + t * c.ldx;
-    for (int o = threadIdx.x >> 6; o < c.d_out; o += THREADS / 64) {
-        const T* w = static_cast<const T*>(c.w) + (long long)o * c.d_in;
-        float acc = 0.f;
-        for (int j = lane; j < c.d_in; j += 64) acc = fmaf(load1(w + j), load1(x + j), acc);
-        if (s >= 0) {
-            const T* b = static_cast<const T*>(c.b) + ((long long)s * c.d_out + o) * c.rank;
-            for (int r = lane; r < c.rank; r += 64) acc = fmaf(load1(b + r), c.u[t * c.rank + r], acc);
+__device__ __forceinline__ void place_chunk(const Sort& s, int c, int* next) {
+    const int lane = threadIdx.x & 63, end = min(s.n, (c + 1) * s.chunk);
+    for (int t0 = c * s.chunk; t0 < end; t0 += 64) {
+        const bool live = t0 + lane < end;
+        const int bin = live ? bin_of(s, t0 + lane) : -1;
+        int of = 0;
+        const int at = place_in_wave(bin, live, &of);
+        const int to = live ? next[bin] + at : 0;
+        if (live && at == of - 1) next[bin] = to + 1;
+        if (live) {
+            s.perm[to] = t0 + lane;
+            s.slot_at[to] = bin < s.n_slots ? bin : bin == s.n_slots ? -1 : -2;
         }
-        acc = wave_sum(acc);
-        if (lane == 0) store1(static_cast<T*>(c.y) + t * c.ldy + o, s == -2 ? NAN : acc);
     }
 }
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void up_grad_kernel(Call c) {
-    const long long t = blockIdx.x;
-    const int s = slot_of(c, t);
-    const T* dy = static_cast<const T*>(c.dy) + t * c.lddy;
-    for (int r = threadIdx.x; r < c.rank; r += THREADS) {
-        float acc = 0.f;
-        if (s >= 0) {
-            const T* b = static_cast<const T*>(c.b) + (long long)s * c.d_out * c.rank + r;
-            for (int o = 0; o < c.d_out; ++o) acc = fmaf(load1(b + (long long)o * c.rank), load1(dy + o), acc);
-            acc *= c.scale[s];
+// From the bins' totals (in LDS, destroyed): start[], and with items the list of items.  One workgroup of 1024.
+__device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int* tmp) {
+    const int bins = s.n_slots + 2, per = (bins + 1023) / 1024, b0 = threadIdx.x * per;
+    // three sums over the bins at a time: requests, items, partials
+    int sum[3] = {0, 0, 0};
+    auto items_of = [&](int b) { return b >= s.n_slots || !s.items ? 0 : max(1, (totals[b] + s.len - 1) / s.len); };
+    for (int b = b0; b < min(bins, b0 + per); ++b) {
+        const int it = items_of(b);
+        sum[0] += totals[b];
+        sum[1] += it;
+        sum[2] += it > 1 ? it : 0;
+    }
+    for (int a = 0; a < 3; ++a) tmp[a * 1024 + threadIdx.x] = sum[a];
+    __syncthreads();
+    for (int d = 1; d < 1024; d *= 2) {
+        int v[3];
+        for (int a = 0; a < 3; ++a) v[a] = threadIdx.x >= d ? tmp[a * 1024 + threadIdx.x - d] : 0;
+        __syncthreads();
+        for (int a = 0; a < 3; ++a) tmp[a * 1024 + threadIdx.x] += v[a];
+        __syncthreads();
+    }
+    int at = tmp[threadIdx.x] - sum[0], item = tmp[1024 + threadIdx.x] - sum[1], part = tmp[2048 + threadIdx.x] - sum[2];
+    if (threadIdx.x == 0) {
+        s.start[bins] = s.n;
+        if (s.items) *s.n_items = tmp[2047];
+    }
+    for (int b = b0; b < min(bins, b0 + per); ++b) {
+        const int total = totals[b], it = items_of(b);
+        s.start[b] = at;
+        totals[b] = at;
+        if (it > 0) {
+            s.parts[b] = int2{part, it > 1 ? it : 0};
+            for (int j = 0; j < it; ++j)
+                s.items[item + j] = Item{b, at + j * s.len, min(at + total, at + (j + 1) * s.len), it > 1 ? part + j : -1};
+            item += it;
+            part += it > 1 ? it : 0;
         }
-        c.v[t * c.rank + r] = s == -2 ? NAN : acc;
+        at += total;
     }
+    __syncthreads();
 }
 
+// All of it in one workgroup: sixteen waves, sixteen chunks, counts in LDS.
+constexpr int SMALL_BINS = 1026, SMALL_N = 16384;
+__global__ __launch_bounds__(1024) void order_small_kernel(Sort s) {
+    extern __shared__ int lds[];
+    const int bins = s.n_slots + 2, wave = threadIdx.x >> 6;
+    int* counts = lds;                 // 16 x bins
+    int* totals = counts + 16 * bins;  // bins
+    int* tmp = totals + bins;          // 3 x 1024
+    for (int j = threadIdx.x; j < 16 * bins; j += 1024) counts[j] = 0;
+    __syncthreads();
+    count_chunk(s, wave, counts + wave * bins);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += 1024) {
+        int sum = 0;
+        for (int w = 0; w < 16; ++w) {
+            const int v = counts[w * bins + b];
+            counts[w * bins + b] = sum;
+            sum += v;
+        }
+        totals[b] = sum;
+    }
+    __syncthreads();
+    starts_and_items(s, totals, tmp);
+    for (int j = threadIdx.x; j < 16 * bins; j += 1024) counts[j] += totals[j % bins];
+    __syncthreads();
+    place_chunk(s, wave, counts + wave * bins);
+}
+__global__ __launch_bounds__(64) void count_kernel(Sort s) {
+    extern __shared__ int lds[];
+    const int bins = s.n_slots + 2;
+    for (int b = threadIdx.x; b < bins; b += 64) lds[b] = 0;
+    __syncthreads();
+    count_chunk(s, blockIdx.x, lds);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += 64) s.counts[(long long)blockIdx.x * bins + b] = lds[b];
+}
+__global__ __launch_bounds__(1024) void scan_kernel(Sort s) {
+    extern __shared__ int lds[];
+    const int bins = s.n_slots + 2;
+    int* totals = lds;
+    int* tmp = totals + bins;
+    for (int b = threadIdx.x; b < bins; b += 1024) {
+        int sum = 0;
+#pragma unroll 16
+        for (int c = 0; c < s.chunks; ++c) {
+            int* at = s.counts + (long long)c * bins + b;
+            const int v = *at;
+            *at = sum;
+            sum += v;
+        }
+        totals[b] = sum;
+    }
+    __syncthreads();
+    starts_and_items(s, totals, tmp);
+}
+__global__ __launch_bounds__(64) void place_kernel(Sort s) {
+    extern __shared__ int lds[];
+    const int bins = s.n_slots + 2;
+    for (int b = threadIdx.x; b < bins; b += 64) lds[b] = s.counts[(long long)blockIdx.x * bins + b] + s.start[b];
+    __syncthreads();
+    place_chunk(s, blockIdx.x, lds);
+}
+
+// ---- transposes of the bank for the backward ---------------------------------------------------------------------------
+struct Turn {
+    const void* from[3];
+    void* to[3];
+    int rows[3], cols[3], count[3];   // count matrices of rows x cols, dense
+    int first[4];                     // first workgroup of each kind
+};
 template <typename T>
-__global__ __launch_bounds__(THREADS) void input_grad_kernel(Call c) {
-    const long long t = blockIdx.x;
-    const int s = slot_of(c, t);
-    const T* dy = static_cast<const T*>(c.dy) + t * c.lddy;
-    for (int j = threadIdx.x; j < c.d_in; j += THREADS) {
-        float acc = 0.f;
-        for (int o = 0; o < c.d_out; ++o)
-            acc = fmaf(load1(static_cast<const T*>(c.w) + (long long)o * c.d_in + j), load1(dy + o), acc);
-        if (s >= 0)
-            for (int r = 0; r < c.rank; ++r)
-                acc = fmaf(load1(static_cast<const T*>(c.a) + ((long long)s * c.rank + r) * c.d_in + j), c.v[t * c.rank + r], acc);
-        store1(static_cast<T*>(c.dx) + t * c.lddx + j, s == -2 ? NAN : acc);
+__global__ __launch_bounds__(256) void turn_kernel(Turn j) {
+    __shared__ T tile[64][66];
+    int kind = 0;
+    while (kind < 2 && (int)blockIdx.x >= j.first[kind + 1]) ++kind;
+    const int rows = j.rows[kind], cols = j.cols[kind], tr = (rows + 63) / 64, tc = (cols + 63) / 64;
+    const int b = blockIdx.x - j.first[kind], m = b / (tr * tc), r0 = b / tc % tr * 64, c0 = b % tc * 64;
+    const T* from = static_cast<const T*>(j.from[kind]) + (long long)m * rows * cols;
+    T* to = static_cast<T*>(j.to[kind]) + (long long)m * rows * cols;
+    const int lane = threadIdx.x & 63;
+    for (int r = threadIdx.x >> 6; r < 64; r += 4)
+        if (r0 + r < rows && c0 + lane < cols) tile[r][lane] = from[(long long)(r0 + r) * cols + c0 + lane];
+    __syncthreads();
+    for (int c = threadIdx.x >> 6; c < 64; c += 4)
+        if (c0 + c < cols && r0 + lane < rows) to[(long long)(c0 + c) * rows + r0 + lane] = tile[lane][c];
+}
+
+// ---- gradients of the bank -----------------------------------------------------------------------------------------------
+//
+// dA_s = sum_t v_t x_t^T and dB_s = sum_t dy_t u_t^T over the requests of an item.  MFMA 16x16x4 in float32 (u and v are float32,
+// and the sums are small beside W's products): the A operand is u or v (16 of the rank x 4 requests), the B operand x or dy.
+// A lane loads 16 bytes of a request's row, E columns, and gives one of them to each of E products: product e has the columns
+// li * E + e.  Nothing is staged; a wave has 16 E columns and up to 64 of the rank.
+struct SlotGrad {
+    Sort s;
+    const float *u, *v;
+    const void *x, *dy;
+    long long ldx, lddy;
+    float *da, *db, *part;   // part: partials x rank x (d_in + d_out)
+    int d_in, d_out, rank, rp;
+    bool vec_x, vec_dy;
+};
+template <typename T, int RT>
+__global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
+    constexpr int E = Mma<T>::E;
+    if ((int)blockIdx.x >= *g.s.n_items) return;
+    const Item it = g.s.items[blockIdx.x];
+    const int lane = threadIdx.x & 63, li = lane & 15, kl = lane >> 4;
+    const int rcs = (g.rank + RT * 16 - 1) / (RT * 16);
+    const int cols_a = (g.d_in + 16 * E - 1) / (16 * E), cols_b = (g.d_out + 16 * E - 1) / (16 * E);
+    int unit = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (unit >= (cols_a + cols_b) * rcs) return;      // (no barrier below)
+    const bool is_b = unit >= cols_a * rcs;
+    if (is_b) unit -= cols_a * rcs;
+    const int r0 = unit % rcs * RT * 16, c0 = unit / rcs * 16 * E + li * E, d = is_b ? g.d_out : g.d_in;
+    const T* src = static_cast<const T*>(is_b ? g.dy : g.x);
+    const long long ld = is_b ? g.lddy : g.ldx;
+    const float* cf = (is_b ? g.u : g.v) + r0;
+    const bool vec = is_b ? g.vec_dy : g.vec_x;
+    f32x4 acc[RT][E];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t0 = it.begin; t0 < it.end; t0 += 64) {
+        const int mine = g.s.perm[min(t0 + lane, it.end - 1)];
+        const int steps = (min(64, it.end - t0) + 3) / 4;
+#pragma unroll 4
+        for (int st = 0; st < steps; ++st) {
+            const int t = t0 + st * 4 + kl;
+            const T* row = src + (long long)__shfl(mine, st * 4 + kl) * ld;
+            const unsigned keep = t < it.end ? ~0u : 0u;
+            u32x4 xv = vec ? piece<true>(row, c0, d) : piece<false>(row, c0, d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) xv[e] &= keep;
+            float a[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const float f = cf[(long long)min(t, it.end - 1) * g.rp + min(r * 16 + li, g.rp - 1 - r0)];
+                a[r] = __uint_as_float(__float_as_uint(f) & keep);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float b = E == 4 ? __uint_as_float(xv[e & 3]) : __uint_as_float(e & 1 ? xv[e >> 1] & 0xffff0000u : xv[e >> 1] << 16);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b, acc[r][e], 0, 0, 0);
+            }
+        }
+    }
+    const long long size_a = (long long)g.rank * g.d_in, size_b = (long long)g.rank * g.d_out;
+    float* to = it.part >= 0 ? g.part + it.part * (size_a + size_b) + (is_b ? size_a : 0)
+                             : is_b ? g.db + it.slot * size_b : g.da + it.slot * size_a;
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int rr = r0 + r * 16 + 4 * kl + i, cc = c0 + e;
+                if (rr < g.rank && cc < d) to[is_b ? (long long)cc * g.rank + rr : (long long)rr * g.d_in + cc] = acc[r][e][i];
+            }
+}
+// The slots of several items: their partials, in order.
+__global__ __launch_bounds__(256) void slot_join_kernel(SlotGrad g) {
+    const int2 parts = g.s.parts[blockIdx.x];
+    if (parts.y == 0) return;
+    const long long size_a = (long long)g.rank * g.d_in, size = size_a + (long long)g.rank * g.d_out;
+    for (long long j = (long long)blockIdx.y * 256 + threadIdx.x; j < size; j += (long long)gridDim.y * 256) {
+        float sum = 0.f;
+#pragma unroll 8
+        for (int p = 0; p < parts.y; ++p) sum += g.part[(parts.x + p) * size + j];
+        if (j < size_a) g.da[blockIdx.x * size_a + j] = sum;
+        else g.db[blockIdx.x * (size - size_a) + j - size_a] = sum;
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void a_grad_kernel(Call c) {
-    const int s = blockIdx.x / c.rank, r = blockIdx.x % c.rank;
-    for (int j = threadIdx.x; j < c.d_in; j += THREADS) {
-        float acc = 0.f;
-        for (long long t = 0; t < c.n; ++t)
-            if (c.slots[t] == s) acc = fmaf(c.v[t * c.rank + r], load1(static_cast<const T*>(c.x) + t * c.ldx + j), acc);
-        c.da[((long long)s * c.rank + r) * c.d_in + j] = acc;
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void b_grad_kernel(Call c) {
-    const int s = blockIdx.x, o = blockIdx.y;
-    for (int r = threadIdx.x; r < c.rank; r += THREADS) {
-        float acc = 0.f;
-        for (long long t = 0; t < c.n; ++t)
-            if (c.slots[t] == s) acc = fmaf(load1(static_cast<const T*>(c.dy) + t * c.lddy + o), c.u[t * c.rank + r], acc);
-        c.db[((long long)s * c.d_out + o) * c.rank + r] = acc;
-    }
-}
-
+// ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    size_t u_off, v_off, bytes;
+    bool sorted;
+    int rp, chunk, chunks, len, max_items, max_parts;
+    size_t u, v, perm, slot_at, counts, start, parts, n_items, items, wt, at, bt, part, bytes;
 };
 
-Plan make_plan(long long n, int rank, bool grad) {
+Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int rank, bool grad) {
     Plan p{};
+    const size_t esz = dtype == RAG_DTYPE_BF16 ? 2 : 4;
+    const int unit = dtype == RAG_DTYPE_BF16 ? 32 : 16;
     auto take = [&](size_t bytes) {
         const size_t at = p.bytes;
         p.bytes += (bytes + 255) & ~(size_t)255;
         return at;
     };
-    p.u_off = take((size_t)n * rank * sizeof(float));
-    p.v_off = take(grad ? (size_t)n * rank * sizeof(float) : 0);
+    p.rp = (rank + unit - 1) / unit * unit;
+    // (few requests: sorting them costs a launch and saves little)
+    p.sorted = grad || n > 64;
+    p.u = take((size_t)n * p.rp * 4);
+    if (p.sorted) {
+        const bool small = n <= SMALL_N && n_slots + 2 <= SMALL_BINS;
+        p.chunk = small ? (int)((n + 16 * 64 - 1) / (16 * 64) * 64) : (int)std::max<long long>(512, ((n + 127) / 128 + 63) / 64 * 64);
+        p.chunks = small ? 0 : (int)((n + p.chunk - 1) / p.chunk);
+        p.perm = take((size_t)n * 4);
+        p.slot_at = take((size_t)n * 4);
+        p.counts = take((size_t)p.chunks * (n_slots + 2) * 4);
+        p.start = take((size_t)(n_slots + 3) * 4);
+    }
+    if (grad) {
+        p.len = (int)std::max<long long>(128, ((n + 255) / 256 + 3) / 4 * 4);
+        p.max_items = n_slots + (int)(n / p.len) + 1;
+        p.max_parts = 2 * (int)(n / p.len) + 2;
+        p.v = take((size_t)n * p.rp * 4);
+        p.parts = take((size_t)n_slots * sizeof(int2));
+        p.n_items = take(4);
+        p.items = take((size_t)p.max_items * sizeof(Item));
+        p.wt = take((size_t)d_in * d_out * esz);
+        p.at = take((size_t)n_slots * rank * d_in * esz);
+        p.bt = take((size_t)n_slots * rank * d_out * esz);
+        p.part = take((size_t)p.max_parts * rank * ((size_t)d_in + d_out) * 4);
+    }
     return p;
 }
 
-template <typename T>
-int run_apply(const Call& c, hipStream_t st) {
-    const unsigned n = (unsigned)c.n;
-    down_kernel<T><<<n, THREADS, 0, st>>>(c);
+struct Call {
+    int dtype, d_in, d_out, n_slots, rank;
+    long long n, ldx, ldy, lddy, lddx;
+    const void *x, *w, *a, *b, *dy;
+    const float* scale;
+    const long long* slots;
+    void *y, *dx;
+    float *da, *db;
+    char* ws;
+    hipStream_t st;
+};
+
+bool aligned16(const void* p, long long ld, size_t esz) { return ((uintptr_t)p & 15) == 0 && ld * (long long)esz % 16 == 0; }
+
+int run_order(const Call& c, const Plan& p, Sort* out, bool items) {
+    Sort s{};
+    s.slots = c.slots;
+    s.n = (int)c.n;
+    s.n_slots = c.n_slots;
+    s.chunk = p.chunk;
+    s.chunks = p.chunks;
+    s.len = p.len;
+    s.perm = reinterpret_cast<int*>(c.ws + p.perm);
+    s.slot_at = reinterpret_cast<int*>(c.ws + p.slot_at);
+    s.counts = reinterpret_cast<int*>(c.ws + p.counts);
+    s.start = reinterpret_cast<int*>(c.ws + p.start);
+    if (items) {
+        s.parts = reinterpret_cast<int2*>(c.ws + p.parts);
+        s.n_items = reinterpret_cast<int*>(c.ws + p.n_items);
+        s.items = reinterpret_cast<Item*>(c.ws + p.items);
+    }
+    *out = s;
+    const size_t bins = c.n_slots + 2;
+    if (p.chunks == 0) {
+        const size_t lds = (17 * bins + 3 * 1024) * 4;
+        if (lds > 48 * 1024)
+            RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(order_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        order_small_kernel<<<1, 1024, lds, c.st>>>(s);
+        RAG_HIP(hipGetLastError());
+        return RAG_OK;
+    }
+    count_kernel<<<(unsigned)p.chunks, 64, bins * 4, c.st>>>(s);
     RAG_HIP(hipGetLastError());
-    apply_kernel<T><<<n, THREADS, 0, st>>>(c);
+    scan_kernel<<<1, 1024, (bins + 3 * 1024) * 4, c.st>>>(s);
+    RAG_HIP(hipGetLastError());
+    place_kernel<<<(unsigned)p.chunks, 64, bins * 4, c.st>>>(s);
     RAG_HIP(hipGetLastError());
     return RAG_OK;
 }
 
+template <typename T, bool VEC>
+int launch_down(const Bank& k, const Order& o, const void* x, long long ldx, float* u, hipStream_t st) {
+    const unsigned groups = (unsigned)((o.n + DOWN_TOKENS - 1) / DOWN_TOKENS);
+    if (k.rp <= 16) down_kernel<T, 1, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
+    else if (k.rp <= 32) down_kernel<T, 2, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
+    else if (k.rp <= 64) down_kernel<T, 4, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
+    else down_kernel<T, 8, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
+    RAG_HIP(hipGetLastError());
+    return RAG_OK;
+}
+
+template <typename T, bool VEC>
+int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const float* u, void* y, long long ldy, hipStream_t st) {
+    const bool vec_out = ldy % 4 == 0 && ((uintptr_t)y & 15) == 0;
+    auto grid = [&](int ot, int tt) { return (unsigned)((k.d_out + 16 * ot - 1) / (16 * ot) * ((o.n + 16 * tt - 1) / (16 * tt))); };
+    const unsigned wide = grid(2, 4);
+    if (o.n <= 16) up_direct_kernel<T, 1, 1, 8, VEC><<<grid(1, 1), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    else if (o.n <= 32) up_direct_kernel<T, 1, 2, 8, VEC><<<grid(1, 2), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    else if (wide < 512) up_direct_kernel<T, 1, 4, 8, VEC><<<grid(1, 4), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    else up_direct_kernel<T, 2, 4, 4, VEC><<<wide, 256, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    RAG_HIP(hipGetLastError());
+    return RAG_OK;
+}
+
+// U and, with y, Y of a bank
 template <typename T>
-int run_grad(const Call& c, hipStream_t st) {
-    const unsigned n = (unsigned)c.n;
-    if (n > 0) {
-        down_kernel<T><<<n, THREADS, 0, st>>>(c);
-        RAG_HIP(hipGetLastError());
-        up_grad_kernel<T><<<n, THREADS, 0, st>>>(c);
-        RAG_HIP(hipGetLastError());
-        if (c.dx) {
-            input_grad_kernel<T><<<n, THREADS, 0, st>>>(c);
-            RAG_HIP(hipGetLastError());
-        }
+int run_product(const Bank& k, const Order& o, const void* x, long long ldx, float* u, void* y, long long ldy, hipStream_t st) {
+    const bool vec = k.vec_in && aligned16(x, ldx, sizeof(T));
+    int rc = vec ? launch_down<T, true>(k, o, x, ldx, u, st) : launch_down<T, false>(k, o, x, ldx, u, st);
+    if (rc || !y) return rc;
+    return vec ? launch_up<T, true>(k, o, x, ldx, u, y, ldy, st) : launch_up<T, false>(k, o, x, ldx, u, y, ldy, st);
+}
+
+Bank make_bank(const Call& c, const Plan& p, const void* w, const void* a, const void* b, int d_in, int d_out) {
+    const int e = c.dtype == RAG_DTYPE_BF16 ? 8 : 4;
+    Bank k{w, a, b, c.scale, d_in, d_out, c.n_slots, c.rank, p.rp, false, false};
+    k.vec_in = d_in % e == 0 && (((uintptr_t)w | (uintptr_t)a) & 15) == 0;
+    k.vec_rank = c.rank % e == 0 && ((uintptr_t)b & 15) == 0;
+    return k;
+}
+
+template <typename T>
+int run_apply(const Call& c, const Plan& p) {
+    Order o{nullptr, nullptr, c.slots, c.n, c.n_slots};
+    if (p.sorted) {
+        Sort s;
+        const int rc = run_order(c, p, &s, false);
+        if (rc) return rc;
+        o.perm = s.perm;
+        o.slot_at = s.slot_at;
     }
-    a_grad_kernel<T><<<(unsigned)(c.slots_n * c.rank), THREADS, 0, st>>>(c);
+    return run_product<T>(make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out), o, c.x, c.ldx, reinterpret_cast<float*>(c.ws + p.u), c.y, c.ldy, c.st);
+}
+
+template <typename T>
+int run_grad(const Call& c, const Plan& p) {
+    Sort s;
+    int rc = run_order(c, p, &s, true);
+    if (rc) return rc;
+    const Order o{s.perm, s.slot_at, c.slots, c.n, c.n_slots};
+    float* u = reinterpret_cast<float*>(c.ws + p.u);
+    float* v = reinterpret_cast<float*>(c.ws + p.v);
+    if (c.n > 0) {
+        // the transposed bank: B always (v), W and A for dx
+        Turn t{};
+        const void* from[3] = {c.b, c.w, c.a};
+        void* to[3] = {c.ws + p.bt, c.ws + p.wt, c.ws + p.at};
+        const int rows[3] = {c.d_out, c.d_out, c.rank}, cols[3] = {c.rank, c.d_in, c.d_in}, count[3] = {c.n_slots, 1, c.n_slots};
+        int at = 0;
+        for (int i = 0; i < 3; ++i) {
+            t.from[i] = from[i];
+            t.to[i] = to[i];
+            t.rows[i] = rows[i];
+            t.cols[i] = cols[i];
+            t.count[i] = i == 0 || c.dx ? count[i] : 0;
+            t.first[i] = at;
+            at += t.count[i] * ((rows[i] + 63) / 64) * ((cols[i] + 63) / 64);
+        }
+        t.first[3] = at;
+        turn_kernel<T><<<(unsigned)at, 256, 0, c.st>>>(t);
+        RAG_HIP(hipGetLastError());
+        rc = run_product<T>(make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out), o, c.x, c.ldx, u, nullptr, 0, c.st);
+        if (rc) return rc;
+        rc = run_product<T>(make_bank(c, p, to[1], to[0], to[2], c.d_out, c.d_in), o, c.dy, c.lddy, v, c.dx, c.lddx, c.st);
+        if (rc) return rc;
+    }
+    constexpr int E = Mma<T>::E;
+    SlotGrad g{s, u, v, c.x, c.dy, c.ldx, c.lddy, c.da, c.db, reinterpret_cast<float*>(c.ws + p.part), c.d_in, c.d_out, c.rank, p.rp,
+               c.d_in % E == 0 && aligned16(c.x, c.ldx, sizeof(T)), c.d_out % E == 0 && aligned16(c.dy, c.lddy, sizeof(T))};
+    auto launch = [&](auto rt) {
+        constexpr int RT = rt.value;
+        const int units = ((c.d_in + 16 * E - 1) / (16 * E) + (c.d_out + 16 * E - 1) / (16 * E)) * ((c.rank + 16 * RT - 1) / (16 * RT));
+        slot_grad_kernel<T, RT><<<dim3((unsigned)p.max_items, (unsigned)((units + 3) / 4)), 256, 0, c.st>>>(g);
+    };
+    if (c.rank <= 16) launch(std::integral_constant<int, 1>());
+    else if (c.rank <= 32) launch(std::integral_constant<int, 2>());
+    else launch(std::integral_constant<int, 4>());
     RAG_HIP(hipGetLastError());
-    b_grad_kernel<T><<<dim3((unsigned)c.slots_n, (unsigned)c.d_out), THREADS, 0, st>>>(c);
-    RAG_HIP(hipGetLastError());
+    if (c.n > p.len) {               // (else every slot is one item)
+        const long long size = (long long)c.rank * (c.d_in + c.d_out);
+        slot_join_kernel<<<dim3((unsigned)c.n_slots, (unsigned)std::min<long long>(64, (size + 255) / 256)), 256, 0, c.st>>>(g);
+        RAG_HIP(hipGetLastError());
+    }
     return RAG_OK;
 }
 
@@ -203,7 +520,7 @@ int rag_adapter_ws_bytes(int dtype, int64_t n, int d_in, int d_out, int n_slots,
     const int rc = check_shape("rag_adapter_ws_bytes", dtype, n, d_in, d_out, n_slots, rank);
     if (rc) return rc;
     if (!bytes) return fail(RAG_ERR_INVALID_ARG, "rag_adapter_ws_bytes: bytes is NULL");
-    *bytes = (int64_t)make_plan(n, rank, want_grad != 0).bytes;
+    *bytes = (int64_t)make_plan(dtype, n, d_in, d_out, n_slots, rank, want_grad != 0).bytes;
     return RAG_OK;
 }
 
@@ -220,18 +537,19 @@ int rag_adapter_apply_dev(int dtype, int64_t n, int d_in, int d_out, int n_slots
     if (ldx < d_in || ldy < d_out)
         return fail(RAG_ERR_INVALID_ARG, "%s: row strides %lld / %lld are below d_in=%d / d_out=%d", who, (long long)ldx,
                     (long long)ldy, d_in, d_out);
-    const Plan p = make_plan(n, rank, false);
+    const Plan p = make_plan(dtype, n, d_in, d_out, n_slots, rank, false);
     if (!ws_dev || ws_bytes < (int64_t)p.bytes || ((uintptr_t)ws_dev & 255))
         return fail(RAG_ERR_INVALID_ARG, "%s: needs a workspace of %lld bytes, aligned to 256 (rag_adapter_ws_bytes)", who,
                     (long long)p.bytes);
     Call c{};
-    c.n = n; c.d_in = d_in; c.d_out = d_out; c.slots_n = n_slots; c.rank = rank;
+    c.dtype = dtype; c.n = n; c.d_in = d_in; c.d_out = d_out; c.n_slots = n_slots; c.rank = rank;
     c.x = x_dev; c.ldx = ldx; c.w = w_dev; c.a = a_dev; c.b = b_dev; c.scale = scale_dev;
     c.slots = reinterpret_cast<const long long*>(slots_dev);
     c.y = y_dev; c.ldy = ldy;
-    c.u = reinterpret_cast<float*>(static_cast<char*>(ws_dev) + p.u_off);
+    c.ws = static_cast<char*>(ws_dev);
+    c.st = (hipStream_t)stream;
     DeviceScope dev;
-    return dtype == RAG_DTYPE_BF16 ? run_apply<unsigned short>(c, (hipStream_t)stream) : run_apply<float>(c, (hipStream_t)stream);
+    return dtype == RAG_DTYPE_BF16 ? run_apply<u16>(c, p) : run_apply<float>(c, p);
 }
 
 int rag_adapter_grad_dev(int dtype, int64_t n, int d_in, int d_out, int n_slots, int rank, const void* x_dev, int64_t ldx,
@@ -248,19 +566,19 @@ int rag_adapter_grad_dev(int dtype, int64_t n, int d_in, int d_out, int n_slots,
     if (n > 0 && (ldx < d_in || lddy < d_out || (dx_dev && lddx < d_in)))
         return fail(RAG_ERR_INVALID_ARG, "%s: row strides %lld / %lld / %lld are below d_in=%d / d_out=%d / d_in", who,
                     (long long)ldx, (long long)lddy, (long long)lddx, d_in, d_out);
-    const Plan p = make_plan(n, rank, true);
-    if (n > 0 && (!ws_dev || ws_bytes < (int64_t)p.bytes || ((uintptr_t)ws_dev & 255)))
+    const Plan p = make_plan(dtype, n, d_in, d_out, n_slots, rank, true);
+    if (!ws_dev || ws_bytes < (int64_t)p.bytes || ((uintptr_t)ws_dev & 255))
         return fail(RAG_ERR_INVALID_ARG, "%s: needs a workspace of %lld bytes, aligned to 256 (rag_adapter_ws_bytes)", who,
                     (long long)p.bytes);
     Call c{};
-    c.n = n; c.d_in = d_in; c.d_out = d_out; c.slots_n = n_slots; c.rank = rank;
+    c.dtype = dtype; c.n = n; c.d_in = d_in; c.d_out = d_out; c.n_slots = n_slots; c.rank = rank;
     c.x = x_dev; c.ldx = ldx; c.w = w_dev; c.a = a_dev; c.b = b_dev; c.scale = scale_dev;
     c.slots = reinterpret_cast<const long long*>(slots_dev);
     c.dy = dy_dev; c.lddy = lddy; c.dx = dx_dev; c.lddx = lddx; c.da = da_dev; c.db = db_dev;
-    c.u = reinterpret_cast<float*>(static_cast<char*>(ws_dev) + p.u_off);
-    c.v = reinterpret_cast<float*>(static_cast<char*>(ws_dev) + p.v_off);
+    c.ws = static_cast<char*>(ws_dev);
+    c.st = (hipStream_t)stream;
     DeviceScope dev;
-    return dtype == RAG_DTYPE_BF16 ? run_grad<unsigned short>(c, (hipStream_t)stream) : run_grad<float>(c, (hipStream_t)stream);
+    return dtype == RAG_DTYPE_BF16 ? run_grad<u16>(c, p) : run_grad<float>(c, p);
 }
 
 }  // extern "C"

@@ -1,0 +1,284 @@
+// adapter_gemm.h -- the matrix kernels of the query adapters (adapter.hip).
+//
+// Requests are met in the order of their slots (perm, slot_at: position -> request, slot), so that 16 neighbours mostly share an
+// adapter.  Every product is written transposed, (weights' rows) x (requests): a request is ONE lane of every result
+// (lane & 15), so slots are told apart per lane, and rows of x and of W, A, B are read along the summed index, 16 bytes a
+// lane, straight into MFMA operands (16x16x4 float32, 16x16x32 bfloat16).
+//     down:  U^T = c A_s X^T      (rank x requests)       float32, in sorted order, rank padded to Rp with zeros
+//     up:    Y^T = W X^T + B_s U^T
+// The backward is the same two with the transposed matrices: V = c B_s^T dY, dX = dY W + V A_s.
+// U keeps float32: for bfloat16 weights its product is made of two, with U's bfloat16 and the bfloat16 of what that leaves
+// (a single one would add an error of y's own rounding).
+#pragma once
+#include "common.h"
+
+#include <type_traits>
+
+namespace rag {
+namespace adapter {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16;
+
+__device__ __forceinline__ u16 f_to_bf(float f) { return __builtin_bit_cast(u16, (__bf16)f); }
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const u16* p) { return __uint_as_float((unsigned)*p << 16); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(u16* p, float v) { *p = f_to_bf(v); }
+
+// The bank as a product sees it (forward: W, A, B; backward: their transposes).
+struct Bank {
+    const void *w, *a, *b;      // d_out x d_in, slots x rank x d_in, slots x d_out x rank
+    const float* scale;         // slots
+    int d_in, d_out, slots, rank, rp;   // rp: row length of U
+    bool vec_in, vec_rank;      // 16-byte loads along d_in (x, W, A) and along rank (B)
+};
+struct Order {
+    const int* perm;            // NULL: position = request
+    const int* slot_at;         // NULL: from slots
+    const long long* slots;
+    long long n;
+    int n_slots;
+    // position -> slot: >= 0, -1 (none), -2 (outside the bank: NaN)
+    __device__ __forceinline__ int slot(long long pos) const {
+        if (slot_at) return slot_at[pos];
+        const long long s = slots[pos];
+        return s >= -1 && s < n_slots ? (int)s : -2;
+    }
+    __device__ __forceinline__ long long request(long long pos) const { return perm ? perm[pos] : pos; }
+};
+
+template <typename T> struct Mma;
+template <> struct Mma<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct Mma<u16> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+
+// The piece of `row` at `col`: zeros from `end` on.  VEC: rows and pieces are 16-byte aligned and end with a piece.
+template <bool VEC, typename T>
+__device__ __forceinline__ u32x4 piece(const T* row, int col, int end) {
+    constexpr int E = Mma<T>::E;
+    if (VEC) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(row + min(col, end - E));
+        const unsigned keep = col < end ? ~0u : 0u;
+        return u32x4{v[0] & keep, v[1] & keep, v[2] & keep, v[3] & keep};
+    }
+    T v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = row[min(col + e, end - 1)];
+    u32x4 r;
+    __builtin_memcpy(&r, v, 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (E == 8) r[e] &= (col + 2 * e < end ? 0xffffu : 0u) | (col + 2 * e + 1 < end ? 0xffff0000u : 0u);
+        else r[e] &= col + e < end ? ~0u : 0u;
+    }
+    return r;
+}
+
+// U (or V) of 32 positions: four waves take every fourth step along d_in, their sums meet in LDS.
+constexpr int DOWN_TOKENS = 32, DOWN_WAVES = 4;
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Bank k, Order ord, const void* xv, long long ldx, float* u) {
+    typedef Mma<T> M;
+    constexpr int E = M::E;
+    __shared__ float part[DOWN_WAVES][2 * RT][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, kl = lane >> 4;
+    const long long p0 = (long long)blockIdx.x * DOWN_TOKENS;
+    const T* x = static_cast<const T*>(xv);
+    const T* row[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) row[t] = x + ord.request(min(p0 + t * 16 + li, ord.n - 1)) * ldx;
+    const int mine = p0 + (lane & 31) < ord.n ? ord.slot(p0 + (lane & 31)) : -3;   // of position lane & 31
+    unsigned todo = (unsigned)__ballot(mine >= 0);
+    const int steps = (k.d_in + 4 * E - 1) / (4 * E);
+    // positions without an adapter: zeros, outside the bank: NaN
+    for (int j = threadIdx.x; j < DOWN_TOKENS * k.rp; j += 64 * DOWN_WAVES) {
+        const long long p = p0 + j / k.rp;
+        const int s = p < ord.n ? ord.slot(p) : 0;
+        if (s < 0) u[p * k.rp + j % k.rp] = s == -2 ? NAN : 0.f;
+    }
+    while (todo) {                    // (uniform over the workgroup: every wave has the same slots)
+        const int s = __shfl(mine, __ffs(todo) - 1);
+        const unsigned with = (unsigned)__ballot(mine == s) & todo;
+        todo &= ~with;
+        const T* a = static_cast<const T*>(k.a) + (long long)s * k.rank * k.d_in;
+        f32x4 acc[2][RT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        u32x4 xp[2][2], ap[2][RT];
+        auto load = [&](int st, u32x4* xt, u32x4* at) __attribute__((always_inline)) {      // (behind the end: zeros)
+            const int col = (st * 4 + kl) * E;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) xt[t] = piece<VEC>(row[t], col, k.d_in);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) at[r] = piece<VEC>(a + (long long)min(r * 16 + li, k.rank - 1) * k.d_in, col, k.d_in);
+        };
+        auto use = [&](const u32x4* xt, const u32x4* at) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[t][r] = M::mma(at[r], xt[t], acc[t][r]);
+        };
+        load(wave, xp[0], ap[0]);
+        for (int st = wave; st < steps; st += 2 * DOWN_WAVES) {
+            load(st + DOWN_WAVES, xp[1], ap[1]);
+            use(xp[0], ap[0]);
+            load(st + 2 * DOWN_WAVES, xp[0], ap[0]);
+            use(xp[1], ap[1]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) *reinterpret_cast<f32x4*>(&part[wave][t * RT + r][lane * 4]) = acc[t][r];
+        __syncthreads();
+        const float scale = k.scale[s];
+        for (int j = wave; j < 2 * RT; j += DOWN_WAVES) {
+            f32x4 sum = *reinterpret_cast<const f32x4*>(&part[0][j][lane * 4]);
+#pragma unroll
+            for (int w = 1; w < DOWN_WAVES; ++w) sum += *reinterpret_cast<const f32x4*>(&part[w][j][lane * 4]);
+            const int t = j / RT, r0 = j % RT * 16 + 4 * kl;
+            if ((with >> (t * 16 + li)) & 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = r0 + i < k.rank ? sum[i] * scale : 0.f;
+                if (r0 < k.rp) *reinterpret_cast<f32x4*>(u + (p0 + t * 16 + li) * k.rp + r0) = sum;
+            }
+        }
+    }
+}
+
+// += B_s U^T for a tile of 16 output columns (from o0) and the 16 positions from p: slot by slot.
+template <typename T, bool VEC>
+__device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, long long n, int my_slot, int o0, f32x4 acc) {
+    typedef Mma<T> M;
+    constexpr int E = M::E;
+    const int lane = threadIdx.x & 63, li = lane & 15, kl = lane >> 4;
+    unsigned todo = (unsigned)__ballot(my_slot >= 0) & 0xffffu;
+    const float* ur = u + min(p + li, n - 1) * k.rp;
+    while (todo) {
+        const int s = __shfl(my_slot, __ffs(todo) - 1);
+        const unsigned with = (unsigned)__ballot(my_slot == s) & todo;
+        todo &= ~with;
+        const T* b = static_cast<const T*>(k.b) + ((long long)s * k.d_out + min(o0 + li, k.d_out - 1)) * k.rank;
+        // (others' lanes keep what they have: a zero times this slot's infinity would not be one)
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < k.rank; r += 4 * E) {
+            const u32x4 bv = piece<VEC>(b, r + kl * E, k.rank);
+            if constexpr (E == 4) {
+                sum = M::mma(bv, *reinterpret_cast<const u32x4*>(ur + r + kl * 4), sum);
+            } else {
+                const f32x4 v[2] = {*reinterpret_cast<const f32x4*>(ur + r + kl * 8), *reinterpret_cast<const f32x4*>(ur + r + kl * 8 + 4)};
+                bf16x8 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    hi[e] = (__bf16)v[e >> 2][e & 3];
+                    lo[e] = (__bf16)(v[e >> 2][e & 3] - (float)hi[e]);
+                }
+                sum = M::mma(bv, __builtin_bit_cast(u32x4, lo), sum);
+                sum = M::mma(bv, __builtin_bit_cast(u32x4, hi), sum);
+            }
+        }
+        if ((with >> li) & 1) acc += sum;
+    }
+    return acc;
+}
+
+// A tile of Y^T to memory: lane = position, four columns.
+template <typename T>
+__device__ __forceinline__ void put(const Bank& k, void* y, long long ldy, long long request, int o, int slot, f32x4 v, bool vec) {
+    T* to = static_cast<T*>(y) + request * ldy + o;
+    if (slot == -2) v = f32x4{NAN, NAN, NAN, NAN};
+    if (vec && o + 4 <= k.d_out) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<f32x4*>(to) = v;
+        } else {
+            typedef u16 u16x4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<u16x4*>(to) = u16x4{f_to_bf(v[0]), f_to_bf(v[1]), f_to_bf(v[2]), f_to_bf(v[3])};
+        }
+        return;
+    }
+    for (int i = 0; i < 4; ++i)
+        if (o + i < k.d_out) store1(to + i, v[i]);
+}
+
+// Y for a few requests: a workgroup has OT x 16 output columns and TT x 16 positions, its waves every WAVES-th step along d_in,
+// straight from memory (each byte is used by one wave, LDS would only add a trip); their sums meet in LDS, a wave finishes a tile.
+template <typename T, int OT, int TT, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y,
+                                                               long long ldy, bool vec_out) {
+    typedef Mma<T> M;
+    constexpr int E = M::E;
+    __shared__ float part[WAVES][OT * TT][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, kl = lane >> 4;
+    const int outs = (k.d_out + 16 * OT - 1) / (16 * OT);        // (neighbours share their requests' rows)
+    const long long p0 = (long long)(blockIdx.x / outs) * TT * 16;
+    const int o0 = blockIdx.x % outs * OT * 16;
+    const T* x = static_cast<const T*>(xv);
+    const T* row[TT];
+    const T* w[OT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) row[t] = x + ord.request(min(p0 + t * 16 + li, ord.n - 1)) * ldx;
+#pragma unroll
+    for (int o = 0; o < OT; ++o) w[o] = static_cast<const T*>(k.w) + (long long)min(o0 + o * 16 + li, k.d_out - 1) * k.d_in;
+    f32x4 acc[OT][TT];
+#pragma unroll
+    for (int o = 0; o < OT; ++o)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[o][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int steps = (k.d_in + 4 * E - 1) / (4 * E);
+    u32x4 xp[2][TT], wp[2][OT];
+    auto load = [&](int st, u32x4* xt, u32x4* wt) __attribute__((always_inline)) {      // (behind the end: zeros)
+        const int col = (st * 4 + kl) * E;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) xt[t] = piece<VEC>(row[t], col, k.d_in);
+#pragma unroll
+        for (int o = 0; o < OT; ++o) wt[o] = piece<VEC>(w[o], col, k.d_in);
+    };
+    auto use = [&](const u32x4* xt, const u32x4* wt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int o = 0; o < OT; ++o)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[o][t] = M::mma(wt[o], xt[t], acc[o][t]);
+    };
+    load(wave, xp[0], wp[0]);
+    for (int st = wave; st < steps; st += 2 * WAVES) {
+        load(st + WAVES, xp[1], wp[1]);
+        use(xp[0], wp[0]);
+        load(st + 2 * WAVES, xp[0], wp[0]);
+        use(xp[1], wp[1]);
+    }
+#pragma unroll
+    for (int o = 0; o < OT; ++o)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4*>(&part[wave][o * TT + t][lane * 4]) = acc[o][t];
+    __syncthreads();
+    for (int j = wave; j < OT * TT; j += WAVES) {
+        f32x4 sum = *reinterpret_cast<const f32x4*>(&part[0][j][lane * 4]);
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) sum += *reinterpret_cast<const f32x4*>(&part[v][j][lane * 4]);
+        const int o = o0 + j / TT * 16;
+        const long long p = p0 + j % TT * 16, pos = p + li;
+        const int slot = pos < ord.n ? ord.slot(pos) : -3;
+        if (k.vec_rank) sum = up<T, true>(k, u, p, ord.n, slot, o, sum);
+        else sum = up<T, false>(k, u, p, ord.n, slot, o, sum);
+        if (pos < ord.n) put<T>(k, y, ldy, ord.request(pos), o + 4 * kl, slot, sum, vec_out);
+    }
+}
+
+}  // namespace adapter
+}  // namespace rag
