@@ -27,7 +27,7 @@ struct Item {
 };
 struct Sort {
     const long long* slots;
-    int n, n_slots, chunk, chunks, len;
+    int n, n_slots, bits, chunk, chunks, len;
     int *perm, *slot_at, *counts, *start;   // counts: chunks x (slots + 2); start: slots + 3
     int2* parts;                            // per slot: first partial, number of partials (0: none)
     int* n_items;
@@ -37,21 +37,15 @@ __device__ __forceinline__ int bin_of(const Sort& s, int t) {
     const long long v = s.slots[t];
     return v >= 0 && v < s.n_slots ? (int)v : v == -1 ? s.n_slots : s.n_slots + 1;
 }
-// lane's place among the lanes of its bin, and their number
-__device__ __forceinline__ int place_in_wave(int bin, bool live, int* of) {
-    const int lane = threadIdx.x & 63;
-    unsigned long long todo = __ballot(live);
-    int at = 0;
-    while (todo) {
-        const int b = __shfl(bin, __ffsll((long long)todo) - 1);
-        const unsigned long long with = __ballot(live && bin == b);
-        if (live && bin == b) {
-            at = __popcll(with & ((1ull << lane) - 1));
-            *of = __popcll(with);
-        }
-        todo &= ~with;
+// lane's place among the lanes of its bin, and their number: the lanes that agree in every bit of the bin
+__device__ __forceinline__ int place_in_wave(int bits, int bin, bool live, int* of) {
+    unsigned long long with = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long long set = __ballot((bin >> b) & 1);
+        with &= (bin >> b) & 1 ? set : ~set;
     }
-    return at;
+    *of = __popcll(with);
+    return __popcll(with & ((1ull << (threadIdx.x & 63)) - 1));
 }
 // counts[] += this wave's chunk; the last lane of a bin adds for all of them (one writer, no atomics)
 __device__ __forceinline__ void count_chunk(const Sort& s, int c, int* counts) {
@@ -60,7 +54,7 @@ __device__ __forceinline__ void count_chunk(const Sort& s, int c, int* counts) {
         const bool live = t0 + lane < end;
         const int bin = live ? bin_of(s, t0 + lane) : -1;
         int of = 0;
-        const int at = place_in_wave(bin, live, &of);
+        const int at = place_in_wave(s.bits, bin, live, &of);
         if (live && at == of - 1) counts[bin] += of;
     }
 }
@@ -70,7 +64,7 @@ __device__ __forceinline__ void place_chunk(const Sort& s, int c, int* next) {
         const bool live = t0 + lane < end;
         const int bin = live ? bin_of(s, t0 + lane) : -1;
         int of = 0;
-        const int at = place_in_wave(bin, live, &of);
+        const int at = place_in_wave(s.bits, bin, live, &of);
         const int to = live ? next[bin] + at : 0;
         if (live && at == of - 1) next[bin] = to + 1;
         if (live) {
@@ -162,16 +156,30 @@ __global__ __launch_bounds__(1024) void scan_kernel(Sort s) {
     const int bins = s.n_slots + 2;
     int* totals = lds;
     int* tmp = totals + bins;
-    for (int b = threadIdx.x; b < bins; b += 1024) {
+    // several threads a bin where there are few, each for a run of the chunks
+    const int teams = bins <= 512 ? 1024 / (bins <= 128 ? 128 : bins <= 256 ? 256 : 512) : 1, width = 1024 / teams;
+    const int team = threadIdx.x / width, run = (s.chunks + teams - 1) / teams, c0 = team * run, c1 = min(s.chunks, c0 + run);
+    for (int b0 = 0; b0 < bins; b0 += width) {
+        const int b = b0 + threadIdx.x % width;
         int sum = 0;
+        if (b < bins)
 #pragma unroll 16
-        for (int c = 0; c < s.chunks; ++c) {
-            int* at = s.counts + (long long)c * bins + b;
-            const int v = *at;
-            *at = sum;
-            sum += v;
+            for (int c = c0; c < c1; ++c) sum += s.counts[(long long)c * bins + b];
+        tmp[threadIdx.x] = sum;
+        __syncthreads();
+        if (b < bins) {
+            int before = 0;
+            for (int t = 0; t < team; ++t) before += tmp[t * width + threadIdx.x % width];
+            if (team == teams - 1) totals[b] = before + sum;
+#pragma unroll 16
+            for (int c = c0; c < c1; ++c) {
+                int* at = s.counts + (long long)c * bins + b;
+                const int v = *at;
+                *at = before;
+                before += v;
+            }
         }
-        totals[b] = sum;
+        __syncthreads();
     }
     __syncthreads();
     starts_and_items(s, totals, tmp);
@@ -248,7 +256,6 @@ __global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
     for (int t0 = it.begin; t0 < it.end; t0 += 64) {
         const int mine = g.s.perm[min(t0 + lane, it.end - 1)];
         const int steps = (min(64, it.end - t0) + 3) / 4;
-#pragma unroll 4
         for (int st = 0; st < steps; ++st) {
             const int t = t0 + st * 4 + kl;
             const T* row = src + (long long)__shfl(mine, st * 4 + kl) * ld;
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float b = E == 4 ? __uint_as_float(xv[e & 3]) : __uint_as_float(e & 1 ? xv[e >> 1] & 0xffff0000u : xv[e >> 1] << 16);
+                const float b = element<T>(xv, e);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b, acc[r][e], 0, 0, 0);
             }
@@ -327,7 +334,7 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
         p.start = take((size_t)(n_slots + 3) * 4);
     }
     if (grad) {
-        p.len = (int)std::max<long long>(128, ((n + 255) / 256 + 3) / 4 * 4);
+        p.len = (int)std::max<long long>(64, ((n + 255) / 256 + 3) / 4 * 4);
         p.max_items = n_slots + (int)(n / p.len) + 1;
         p.max_parts = 2 * (int)(n / p.len) + 2;
         p.v = take((size_t)n * p.rp * 4);
@@ -361,6 +368,7 @@ int run_order(const Call& c, const Plan& p, Sort* out, bool items) {
     s.slots = c.slots;
     s.n = (int)c.n;
     s.n_slots = c.n_slots;
+    while ((c.n_slots + 1) >> s.bits) ++s.bits;
     s.chunk = p.chunk;
     s.chunks = p.chunks;
     s.len = p.len;
@@ -394,6 +402,13 @@ int run_order(const Call& c, const Plan& p, Sort* out, bool items) {
 
 template <typename T, bool VEC>
 int launch_down(const Bank& k, const Order& o, const void* x, long long ldx, float* u, hipStream_t st) {
+    // Few requests a slot (on average: the host does not see them): a matrix tile of 32 neighbours would go over its slots
+    // one after the other (64 requests of 64 slots, 768 wide: 85 us against 4 us).
+    if (o.n < 16ll * k.slots && o.n * k.rank * k.d_in * (long long)sizeof(T) <= (256ll << 20)) {
+        down_each_kernel<T, VEC><<<(unsigned)o.n, 256, 0, st>>>(k, o, x, ldx, u);
+        RAG_HIP(hipGetLastError());
+        return RAG_OK;
+    }
     const unsigned groups = (unsigned)((o.n + DOWN_TOKENS - 1) / DOWN_TOKENS);
     if (k.rp <= 16) down_kernel<T, 1, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
     else if (k.rp <= 32) down_kernel<T, 2, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
@@ -406,12 +421,19 @@ int launch_down(const Bank& k, const Order& o, const void* x, long long ldx, flo
 template <typename T, bool VEC>
 int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const float* u, void* y, long long ldy, hipStream_t st) {
     const bool vec_out = ldy % 4 == 0 && ((uintptr_t)y & 15) == 0;
+    const unsigned tiles = (unsigned)((o.n + TILED_POS - 1) / TILED_POS * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
+    if (VEC && tiles >= 128 && (unsigned long long)o.n * ldx * sizeof(T) < (1ull << 32)) {
+        auto fn = k.rank <= 4 * Mma<T>::E ? up_tiled_kernel<T, 1> : up_tiled_kernel<T, 2>;
+        RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, TILED_LDS));
+        fn<<<tiles, 256, TILED_LDS, st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy, vec_out);
+        RAG_HIP(hipGetLastError());
+        return RAG_OK;
+    }
     auto grid = [&](int ot, int tt) { return (unsigned)((k.d_out + 16 * ot - 1) / (16 * ot) * ((o.n + 16 * tt - 1) / (16 * tt))); };
-    const unsigned wide = grid(2, 4);
-    if (o.n <= 16) up_direct_kernel<T, 1, 1, 8, VEC><<<grid(1, 1), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
-    else if (o.n <= 32) up_direct_kernel<T, 1, 2, 8, VEC><<<grid(1, 2), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
-    else if (wide < 512) up_direct_kernel<T, 1, 4, 8, VEC><<<grid(1, 4), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
-    else up_direct_kernel<T, 2, 4, 4, VEC><<<wide, 256, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    if (grid(2, 4) >= 1024) up_direct_kernel<T, 2, 4, 4, VEC><<<grid(2, 4), 256, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    else if (grid(1, 4) >= 512) up_direct_kernel<T, 1, 4, 8, VEC><<<grid(1, 4), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    else if (grid(1, 2) >= 512) up_direct_kernel<T, 1, 2, 8, VEC><<<grid(1, 2), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    else up_direct_kernel<T, 1, 1, 8, VEC><<<grid(1, 1), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
     RAG_HIP(hipGetLastError());
     return RAG_OK;
 }

@@ -10,7 +10,7 @@
 // U keeps float32: for bfloat16 weights its product is made of two, with U's bfloat16 and the bfloat16 of what that leaves
 // (a single one would add an error of y's own rounding).
 #pragma once
-#include "common.h"
+#include "distill_tile.h"
 
 #include <type_traits>
 
@@ -88,6 +88,13 @@ __device__ __forceinline__ u32x4 piece(const T* row, int col, int end) {
     return r;
 }
 
+// Element e of a piece, as a float.
+template <typename T>
+__device__ __forceinline__ float element(u32x4 p, int e) {
+    if (sizeof(T) == 4) return __uint_as_float(p[e & 3]);
+    return __uint_as_float(e & 1 ? p[e >> 1] & 0xffff0000u : p[e >> 1] << 16);
+}
+
 // U (or V) of 32 positions: four waves take every fourth step along d_in, their sums meet in LDS.
 constexpr int DOWN_TOKENS = 32, DOWN_WAVES = 4;
 template <typename T, int RT, bool VEC>
@@ -162,7 +169,45 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Bank k, Order ord
     }
 }
 
-// += B_s U^T for a tile of 16 output columns (from o0) and the 16 positions from p: slot by slot.
+// U where slots have few requests each: a workgroup per position, a wave per row of A_s.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void down_each_kernel(Bank k, Order ord, const void* xv, long long ldx, float* u) {
+    constexpr int E = Mma<T>::E;
+    const long long p = blockIdx.x;
+    const int s = ord.slot(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (s < 0) {
+        for (int r = threadIdx.x; r < k.rp; r += 256) u[p * k.rp + r] = s == -2 ? NAN : 0.f;
+        return;
+    }
+    const T* x = static_cast<const T*>(xv) + ord.request(p) * ldx;
+    const T* a = static_cast<const T*>(k.a) + (long long)s * k.rank * k.d_in;
+    const float scale = k.scale[s];
+    for (int r0 = wave * 4; r0 < k.rp; r0 += 16) {
+        float acc[4] = {};
+        for (int c = lane * E; c < k.d_in; c += 64 * E) {
+            const u32x4 xp = piece<VEC>(x, c, k.d_in);
+            u32x4 ap[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ap[r] = piece<VEC>(a + (long long)min(r0 + r, k.rank - 1) * k.d_in, c, k.d_in);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float xe = element<T>(xp, e);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[r] = fmaf(element<T>(ap[r], e), xe, acc[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            for (int o = 32; o > 0; o >>= 1) acc[r] += __shfl_xor(acc[r], o);
+        if (lane < 4) {
+            const float v = lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3];
+            u[p * k.rp + r0 + lane] = r0 + lane < k.rank ? v * scale : 0.f;
+        }
+    }
+}
+
+// += B_s U^T for a tile of 16 output columns (from o0) and the 16 positions from p: the first two slots by matrix products, slot
+// by slot; where there are more, each lane takes its own position's.
 template <typename T, bool VEC>
 __device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, long long n, int my_slot, int o0, f32x4 acc) {
     typedef Mma<T> M;
@@ -170,7 +215,27 @@ __device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, 
     const int lane = threadIdx.x & 63, li = lane & 15, kl = lane >> 4;
     unsigned todo = (unsigned)__ballot(my_slot >= 0) & 0xffffu;
     const float* ur = u + min(p + li, n - 1) * k.rp;
-    while (todo) {
+    for (int turn = 0; todo; ++turn) {
+        if (turn == 2) {
+            if ((todo >> li) & 1) {
+                const T* b = static_cast<const T*>(k.b) + (long long)my_slot * k.d_out * k.rank;
+                for (int r = 0; r < k.rank; r += E) {
+                    float v[E];
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        const f32x4 t = *reinterpret_cast<const f32x4*>(ur + r + e);
+                        v[e] = t[0], v[e + 1] = t[1], v[e + 2] = t[2], v[e + 3] = t[3];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const u32x4 bv = piece<VEC>(b + (long long)min(o0 + 4 * kl + i, k.d_out - 1) * k.rank, r, k.rank);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) acc[i] = fmaf(element<T>(bv, e), v[e], acc[i]);
+                    }
+                }
+            }
+            break;
+        }
         const int s = __shfl(my_slot, __ffs(todo) - 1);
         const unsigned with = (unsigned)__ballot(my_slot == s) & todo;
         todo &= ~with;
@@ -276,7 +341,150 @@ __global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord
         const int slot = pos < ord.n ? ord.slot(pos) : -3;
         if (k.vec_rank) sum = up<T, true>(k, u, p, ord.n, slot, o, sum);
         else sum = up<T, false>(k, u, p, ord.n, slot, o, sum);
-        if (pos < ord.n) put<T>(k, y, ldy, ord.request(pos), o + 4 * kl, slot, sum, vec_out);
+        if (pos < ord.n && o + 4 * kl < k.d_out) put<T>(k, y, ldy, ord.request(pos), o + 4 * kl, slot, sum, vec_out);
+    }
+}
+
+// Y for many requests: a workgroup has 128 output columns x 256 positions, a wave 64 x 128 (32 accumulators, two operand reads
+// for every five products), 128 bytes of every row a stage, three stages by LDS-DMA.  Rows of 16-byte pieces only.
+// RS: 64-byte steps of the rank that a wave keeps of its slot's B rows while neighbours share the slot.
+constexpr int TILED_OUTS = 128, TILED_POS = 256;
+constexpr int TILED_LDS = 3 * (TILED_OUTS + TILED_POS) * 128;
+template <typename T, int RS>
+__global__ __launch_bounds__(256, 1) void up_tiled_kernel(Bank k, Order ord, const void* xv, long long ldx, unsigned x_bytes, const float* u, void* y,
+                                                          long long ldy, bool vec_out) {
+    typedef Mma<T> M;
+    constexpr int E = M::E, ESZ = sizeof(T), ROWS = TILED_OUTS + TILED_POS, STAGE = ROWS * 128, LOADS = ROWS / 8 / 4;
+    extern __shared__ __align__(16) char tiled_lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, kl = lane >> 4;
+    const int outs = (k.d_out + TILED_OUTS - 1) / TILED_OUTS;
+    const long long p0 = (long long)(blockIdx.x / outs) * TILED_POS;
+    const int o0 = blockIdx.x % outs * TILED_OUTS;
+    const int stages = (k.d_in * ESZ + 127) / 128;
+    const int lr = lane >> 3, lp = (lane & 7) ^ lr;
+    // a wave's instructions: every fourth group of eight rows, W's first
+    unsigned from[LOADS];
+#pragma unroll
+    for (int a = 0; a < LOADS; ++a) {
+        const int row = (a * 4 + wave) * 8 + lr;
+        from[a] = a * 32 < TILED_OUTS ? (unsigned)min(o0 + row, k.d_out - 1) * (unsigned)(k.d_in * ESZ)
+                                      : (unsigned)(ord.request(min(p0 + row - TILED_OUTS, ord.n - 1)) * ldx * ESZ);
+    }
+    const unsigned w_bytes = (unsigned)k.d_out * k.d_in * ESZ;
+    auto fetch1 = [&](int t, int b, int a) __attribute__((always_inline)) {
+        const int col = min(t * 128 + lp * 16, k.d_in * ESZ - 16);       // (behind the end: masked in W)
+        distill::lds_dma16(a * 32 < TILED_OUTS ? k.w : xv, a * 32 < TILED_OUTS ? w_bytes : x_bytes, from[a] + col,
+                           tiled_lds + b * STAGE + (a * 4 + wave) * 1024);
+    };
+    f32x4 acc[4][8];
+#pragma unroll
+    for (int o = 0; o < 4; ++o)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[o][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int wo = (wave & 1) * 64, wp = (wave >> 1) * 128;
+    int off[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) off[h] = li * 128 + (((h * 4 + kl) ^ (li & 7)) << 4);
+    auto stage = [&](int t, int b, int b2, bool tail) __attribute__((always_inline)) {
+        const char* ws = tiled_lds + b * STAGE + wo * 128;
+        const char* xs = tiled_lds + b * STAGE + (TILED_OUTS + wp) * 128;
+        u32x4 a[2][4], v[2][8];
+        auto read = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+            for (int o = 0; o < 4; ++o) a[h][o] = *reinterpret_cast<const u32x4*>(ws + o * 2048 + off[h]);
+#pragma unroll
+            for (int p = 0; p < 8; ++p) v[h][p] = *reinterpret_cast<const u32x4*>(xs + p * 2048 + off[h]);
+            if (tail) {
+                const unsigned keep = t * 128 + (h * 4 + kl) * 16 < k.d_in * ESZ ? ~0u : 0u;
+#pragma unroll
+                for (int o = 0; o < 4; ++o) a[h][o] = u32x4{a[h][o][0] & keep, a[h][o][1] & keep, a[h][o][2] & keep, a[h][o][3] & keep};
+            }
+        };
+        read(0);
+        read(1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+#pragma unroll
+                for (int p = 0; p < 8; ++p) acc[o][p] = M::mma(a[h][o], v[h][p], acc[o][p]);
+#pragma unroll
+                for (int f = (h * 4 + o) * LOADS / 8; f < (h * 4 + o + 1) * LOADS / 8; ++f) fetch1(t + 2 < stages ? t + 2 : 0, b2, f);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int a = 0; a < LOADS; ++a) fetch1(b < stages ? b : 0, b, a);
+    int b = 0;
+    for (int t = 0; t + 1 < stages; ++t) {
+        distill::wait_meet<LOADS>();
+        stage(t, b, b > 0 ? b - 1 : 2, false);
+        b = b < 2 ? b + 1 : 0;
+    }
+    distill::wait_meet<LOADS>();
+    stage(stages - 1, b, b > 0 ? b - 1 : 2, true);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no LDS-DMA outlives the workgroup
+    // the adapters
+    const int ob = o0 + wo;
+    int kept = -1;
+    u32x4 bv[4][RS];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const long long q = p0 + wp + p * 16, pos = q + li;
+        const int slot = pos < ord.n ? ord.slot(pos) : -3;
+        const int first = __builtin_amdgcn_readfirstlane(slot);
+        if (first >= 0 && __all(slot == first) && k.rank <= RS * 4 * E && k.vec_rank) {      // (uniform) one slot
+            if (first != kept) {
+                const T* bs = static_cast<const T*>(k.b) + (long long)first * k.d_out * k.rank;
+#pragma unroll
+                for (int o = 0; o < 4; ++o)
+#pragma unroll
+                    for (int r = 0; r < RS; ++r)
+                        bv[o][r] = piece<true>(bs + (long long)min(ob + o * 16 + li, k.d_out - 1) * k.rank, (r * 4 + kl) * E, k.rank);
+                kept = first;
+            }
+            const float* ur = u + pos * k.rp;
+#pragma unroll
+            for (int r = 0; r < RS; ++r) {
+                if (r * 4 * E >= k.rank) break;
+                if constexpr (E == 4) {
+                    const u32x4 uv = *reinterpret_cast<const u32x4*>(ur + (r * 4 + kl) * 4);
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) acc[o][p] = M::mma(bv[o][r], uv, acc[o][p]);
+                } else {
+                    const f32x4 t[2] = {*reinterpret_cast<const f32x4*>(ur + (r * 4 + kl) * 8), *reinterpret_cast<const f32x4*>(ur + (r * 4 + kl) * 8 + 4)};
+                    bf16x8 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        hi[e] = (__bf16)t[e >> 2][e & 3];
+                        lo[e] = (__bf16)(t[e >> 2][e & 3] - (float)hi[e]);
+                    }
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) {
+                        acc[o][p] = M::mma(bv[o][r], __builtin_bit_cast(u32x4, lo), acc[o][p]);
+                        acc[o][p] = M::mma(bv[o][r], __builtin_bit_cast(u32x4, hi), acc[o][p]);
+                    }
+                }
+            }
+        } else if (__any(slot >= 0)) {
+            for (int o = 0; o < 4; ++o) {
+                f32x4 v = o == 0 ? acc[0][p] : o == 1 ? acc[1][p] : o == 2 ? acc[2][p] : acc[3][p];
+                v = k.vec_rank ? up<T, true>(k, u, q, ord.n, slot, ob + o * 16, v) : up<T, false>(k, u, q, ord.n, slot, ob + o * 16, v);
+                if (o == 0) acc[0][p] = v;
+                else if (o == 1) acc[1][p] = v;
+                else if (o == 2) acc[2][p] = v;
+                else acc[3][p] = v;
+            }
+        }
+        if (pos < ord.n) {
+            const long long request = ord.request(pos);
+#pragma unroll
+            for (int o = 0; o < 4; ++o)
+                if (ob + o * 16 + 4 * kl < k.d_out) put<T>(k, y, ldy, request, ob + o * 16 + 4 * kl, slot, acc[o][p], vec_out);
+        }
     }
 }
 
