@@ -425,7 +425,7 @@ int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const
     if (VEC && tiles >= 128 && (unsigned long long)o.n * ldx * sizeof(T) < (1ull << 32)) {
         auto fn = k.rank <= 4 * Mma<T>::E ? up_tiled_kernel<T, 1> : up_tiled_kernel<T, 2>;
         RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, TILED_LDS));
-        fn<<<tiles, 256, TILED_LDS, st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy, vec_out);
+        fn<<<tiles, 512, TILED_LDS, st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy, vec_out);
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }

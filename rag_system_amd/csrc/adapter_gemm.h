@@ -345,16 +345,18 @@ __global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord
     }
 }
 
-// Y for many requests: a workgroup has 128 output columns x 256 positions, a wave 64 x 128 (32 accumulators, two operand reads
-// for every five products), 128 bytes of every row a stage, three stages by LDS-DMA.  Rows of 16-byte pieces only.
+// Y for many requests: a workgroup has 128 output columns x 256 positions, each of its eight waves 64 x 64 (an operand read for
+// every two products; two waves on a SIMD, since an LDS-DMA instruction holds its wave for 60 to 180 cycles: four waves of
+// 64 x 128 read less and took 199 us where these take 169, 65536 x 768 x 768 bf16), 128 bytes of every row a stage, three
+// stages by LDS-DMA.  Rows of 16-byte pieces only.
 // RS: 64-byte steps of the rank that a wave keeps of its slot's B rows while neighbours share the slot.
 constexpr int TILED_OUTS = 128, TILED_POS = 256;
 constexpr int TILED_LDS = 3 * (TILED_OUTS + TILED_POS) * 128;
 template <typename T, int RS>
-__global__ __launch_bounds__(256, 1) void up_tiled_kernel(Bank k, Order ord, const void* xv, long long ldx, unsigned x_bytes, const float* u, void* y,
+__global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, const void* xv, long long ldx, unsigned x_bytes, const float* u, void* y,
                                                           long long ldy, bool vec_out) {
     typedef Mma<T> M;
-    constexpr int E = M::E, ESZ = sizeof(T), ROWS = TILED_OUTS + TILED_POS, STAGE = ROWS * 128, LOADS = ROWS / 8 / 4;
+    constexpr int E = M::E, ESZ = sizeof(T), ROWS = TILED_OUTS + TILED_POS, STAGE = ROWS * 128, LOADS = ROWS / 8 / 8;
     extern __shared__ __align__(16) char tiled_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, kl = lane >> 4;
     const int outs = (k.d_out + TILED_OUTS - 1) / TILED_OUTS;
@@ -362,38 +364,38 @@ __global__ __launch_bounds__(256, 1) void up_tiled_kernel(Bank k, Order ord, con
     const int o0 = blockIdx.x % outs * TILED_OUTS;
     const int stages = (k.d_in * ESZ + 127) / 128;
     const int lr = lane >> 3, lp = (lane & 7) ^ lr;
-    // a wave's instructions: every fourth group of eight rows, W's first
+    // a wave's instructions: every eighth group of eight rows, W's first
     unsigned from[LOADS];
 #pragma unroll
     for (int a = 0; a < LOADS; ++a) {
-        const int row = (a * 4 + wave) * 8 + lr;
-        from[a] = a * 32 < TILED_OUTS ? (unsigned)min(o0 + row, k.d_out - 1) * (unsigned)(k.d_in * ESZ)
+        const int row = (a * 8 + wave) * 8 + lr;
+        from[a] = a * 64 < TILED_OUTS ? (unsigned)min(o0 + row, k.d_out - 1) * (unsigned)(k.d_in * ESZ)
                                       : (unsigned)(ord.request(min(p0 + row - TILED_OUTS, ord.n - 1)) * ldx * ESZ);
     }
     const unsigned w_bytes = (unsigned)k.d_out * k.d_in * ESZ;
     auto fetch1 = [&](int t, int b, int a) __attribute__((always_inline)) {
         const int col = min(t * 128 + lp * 16, k.d_in * ESZ - 16);       // (behind the end: masked in W)
-        distill::lds_dma16(a * 32 < TILED_OUTS ? k.w : xv, a * 32 < TILED_OUTS ? w_bytes : x_bytes, from[a] + col,
-                           tiled_lds + b * STAGE + (a * 4 + wave) * 1024);
+        distill::lds_dma16(a * 64 < TILED_OUTS ? k.w : xv, a * 64 < TILED_OUTS ? w_bytes : x_bytes, from[a] + col,
+                           tiled_lds + b * STAGE + (a * 8 + wave) * 1024);
     };
-    f32x4 acc[4][8];
+    f32x4 acc[4][4];
 #pragma unroll
     for (int o = 0; o < 4; ++o)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) acc[o][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int wo = (wave & 1) * 64, wp = (wave >> 1) * 128;
+        for (int t = 0; t < 4; ++t) acc[o][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int wo = (wave & 1) * 64, wp = (wave >> 1) * 64, ob = o0 + wo;
     int off[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) off[h] = li * 128 + (((h * 4 + kl) ^ (li & 7)) << 4);
     auto stage = [&](int t, int b, int b2, bool tail) __attribute__((always_inline)) {
         const char* ws = tiled_lds + b * STAGE + wo * 128;
         const char* xs = tiled_lds + b * STAGE + (TILED_OUTS + wp) * 128;
-        u32x4 a[2][4], v[2][8];
+        u32x4 a[2][4], v[2][4];
         auto read = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
             for (int o = 0; o < 4; ++o) a[h][o] = *reinterpret_cast<const u32x4*>(ws + o * 2048 + off[h]);
 #pragma unroll
-            for (int p = 0; p < 8; ++p) v[h][p] = *reinterpret_cast<const u32x4*>(xs + p * 2048 + off[h]);
+            for (int p = 0; p < 4; ++p) v[h][p] = *reinterpret_cast<const u32x4*>(xs + p * 2048 + off[h]);
             if (tail) {
                 const unsigned keep = t * 128 + (h * 4 + kl) * 16 < k.d_in * ESZ ? ~0u : 0u;
 #pragma unroll
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(256, 1) void up_tiled_kernel(Bank k, Order ord, con
 #pragma unroll
             for (int o = 0; o < 4; ++o) {
 #pragma unroll
-                for (int p = 0; p < 8; ++p) acc[o][p] = M::mma(a[h][o], v[h][p], acc[o][p]);
+                for (int p = 0; p < 4; ++p) acc[o][p] = M::mma(a[h][o], v[h][p], acc[o][p]);
 #pragma unroll
                 for (int f = (h * 4 + o) * LOADS / 8; f < (h * 4 + o + 1) * LOADS / 8; ++f) fetch1(t + 2 < stages ? t + 2 : 0, b2, f);
                 __builtin_amdgcn_sched_barrier(0);
@@ -418,6 +420,55 @@ __global__ __launch_bounds__(256, 1) void up_tiled_kernel(Bank k, Order ord, con
     for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int a = 0; a < LOADS; ++a) fetch1(b < stages ? b : 0, b, a);
+    // what the adapters need of the wave's positions, on its way beside the products
+    int slot0, request0, kept = -1;
+    auto look = [&](int p, int* slot, int* request) __attribute__((always_inline)) {
+        const long long pos = p0 + wp + p * 16 + li;
+        *slot = pos < ord.n ? ord.slot(pos) : -3;
+        *request = (int)ord.request(min(pos, ord.n - 1));
+    };
+    look(0, &slot0, &request0);
+    u32x4 bv[4][RS];
+    f32x4 un[RS][E / 4];
+    auto load_u = [&](int p, f32x4 (*to)[E / 4]) __attribute__((always_inline)) {
+        const float* ur = u + min(p0 + wp + p * 16 + li, ord.n - 1) * k.rp;
+#pragma unroll
+        for (int r = 0; r < RS; ++r)
+#pragma unroll
+            for (int h = 0; h < E / 4; ++h) to[r][h] = *reinterpret_cast<const f32x4*>(ur + min((r * 4 + kl) * E + 4 * h, k.rp - 4));
+    };
+    auto load_b = [&](int s) __attribute__((always_inline)) {
+        if (s == kept) return;                  // (uniform)
+        const T* bs = static_cast<const T*>(k.b) + (long long)s * k.d_out * k.rank;
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+#pragma unroll
+            for (int r = 0; r < RS; ++r)
+                bv[o][r] = piece<true>(bs + (long long)min(ob + o * 16 + li, k.d_out - 1) * k.rank, (r * 4 + kl) * E, k.rank);
+        kept = s;
+    };
+    auto narrow = [&](const f32x4 (*from)[E / 4], u32x4* hi, u32x4* lo) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < RS; ++r) {
+            if constexpr (E == 4) {
+                hi[r] = __builtin_bit_cast(u32x4, from[r][0]);
+            } else {
+                bf16x8 h, l;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h[e] = (__bf16)from[r][e >> 2][e & 3];
+                    l[e] = (__bf16)(from[r][e >> 2][e & 3] - (float)h[e]);
+                }
+                hi[r] = __builtin_bit_cast(u32x4, h);
+                lo[r] = __builtin_bit_cast(u32x4, l);
+            }
+        }
+    };
+    auto times_u = [&](u32x4 bp, u32x4 hi, u32x4 lo, f32x4 c) __attribute__((always_inline)) {
+        if constexpr (E == 8) c = M::mma(bp, lo, c);
+        return M::mma(bp, hi, c);
+    };
+    load_u(0, un);
     int b = 0;
     for (int t = 0; t + 1 < stages; ++t) {
         distill::wait_meet<LOADS>();
@@ -427,63 +478,54 @@ __global__ __launch_bounds__(256, 1) void up_tiled_kernel(Bank k, Order ord, con
     distill::wait_meet<LOADS>();
     stage(stages - 1, b, b > 0 ? b - 1 : 2, true);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no LDS-DMA outlives the workgroup
-    // the adapters
-    const int ob = o0 + wo;
-    int kept = -1;
-    u32x4 bv[4][RS];
+    // The tiles go through LDS (the ring is done with) into a loop over the positions: the adapters' cases are too much code to
+    // stand here eight times.  A tile's U is loaded while the tile before it is finished, B's rows stay while the slot does.
+    __syncthreads();
+    char* tiles = tiled_lds + wave * 16 * 1024 + lane * 16;
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-        const long long q = p0 + wp + p * 16, pos = q + li;
-        const int slot = pos < ord.n ? ord.slot(pos) : -3;
-        const int first = __builtin_amdgcn_readfirstlane(slot);
-        if (first >= 0 && __all(slot == first) && k.rank <= RS * 4 * E && k.vec_rank) {      // (uniform) one slot
-            if (first != kept) {
-                const T* bs = static_cast<const T*>(k.b) + (long long)first * k.d_out * k.rank;
+    for (int p = 0; p < 4; ++p)
 #pragma unroll
-                for (int o = 0; o < 4; ++o)
+        for (int o = 0; o < 4; ++o) *reinterpret_cast<f32x4*>(tiles + (p * 4 + o) * 1024) = acc[o][p];
+    const bool kept_form = k.rank <= RS * 4 * E && k.vec_rank;      // (uniform)
+    int next_slot = slot0, next_request = request0;
+#pragma unroll 1
+    for (int p = 0; p < 4; ++p) {
+        const long long q = p0 + wp + p * 16;
+        const int slot = next_slot, request = next_request;
+        u32x4 uh[RS], ul[RS];
+        narrow(un, uh, ul);
+        if (p < 3) {
+            look(p + 1, &next_slot, &next_request);
+            load_u(p + 1, un);
+        }
+        f32x4 v[4];
 #pragma unroll
-                    for (int r = 0; r < RS; ++r)
-                        bv[o][r] = piece<true>(bs + (long long)min(ob + o * 16 + li, k.d_out - 1) * k.rank, (r * 4 + kl) * E, k.rank);
-                kept = first;
-            }
-            const float* ur = u + pos * k.rp;
+        for (int o = 0; o < 4; ++o) v[o] = *reinterpret_cast<const f32x4*>(tiles + (p * 4 + o) * 1024);
+        unsigned todo = (unsigned)__ballot(slot >= 0) & 0xffffu;
+        if (kept_form)
+            for (int turn = 0; todo && turn < 2; ++turn) {
+                const int s = __shfl(slot, __ffs(todo) - 1);
+                const unsigned with = (unsigned)__ballot(slot == s) & todo;
+                todo &= ~with;
+                load_b(s);
 #pragma unroll
-            for (int r = 0; r < RS; ++r) {
-                if (r * 4 * E >= k.rank) break;
-                if constexpr (E == 4) {
-                    const u32x4 uv = *reinterpret_cast<const u32x4*>(ur + (r * 4 + kl) * 4);
+                for (int o = 0; o < 4; ++o) {
+                    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int o = 0; o < 4; ++o) acc[o][p] = M::mma(bv[o][r], uv, acc[o][p]);
-                } else {
-                    const f32x4 t[2] = {*reinterpret_cast<const f32x4*>(ur + (r * 4 + kl) * 8), *reinterpret_cast<const f32x4*>(ur + (r * 4 + kl) * 8 + 4)};
-                    bf16x8 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        hi[e] = (__bf16)t[e >> 2][e & 3];
-                        lo[e] = (__bf16)(t[e >> 2][e & 3] - (float)hi[e]);
-                    }
-#pragma unroll
-                    for (int o = 0; o < 4; ++o) {
-                        acc[o][p] = M::mma(bv[o][r], __builtin_bit_cast(u32x4, lo), acc[o][p]);
-                        acc[o][p] = M::mma(bv[o][r], __builtin_bit_cast(u32x4, hi), acc[o][p]);
-                    }
+                    for (int r = 0; r < RS; ++r) sum = times_u(bv[o][r], uh[r], ul[r], sum);
+                    if ((with >> li) & 1) v[o] += sum;          // (others' lanes keep what they have)
                 }
             }
-        } else if (__any(slot >= 0)) {
-            for (int o = 0; o < 4; ++o) {
-                f32x4 v = o == 0 ? acc[0][p] : o == 1 ? acc[1][p] : o == 2 ? acc[2][p] : acc[3][p];
-                v = k.vec_rank ? up<T, true>(k, u, q, ord.n, slot, ob + o * 16, v) : up<T, false>(k, u, q, ord.n, slot, ob + o * 16, v);
-                if (o == 0) acc[0][p] = v;
-                else if (o == 1) acc[1][p] = v;
-                else if (o == 2) acc[2][p] = v;
-                else acc[3][p] = v;
-            }
-        }
-        if (pos < ord.n) {
-            const long long request = ord.request(pos);
+        if (todo) {                             // more slots in a tile, or rows of B in no whole pieces
+            const int rest = (todo >> li) & 1 ? slot : -3;
 #pragma unroll
             for (int o = 0; o < 4; ++o)
-                if (ob + o * 16 + 4 * kl < k.d_out) put<T>(k, y, ldy, request, ob + o * 16 + 4 * kl, slot, acc[o][p], vec_out);
+                v[o] = k.vec_rank ? up<T, true>(k, u, q, ord.n, rest, ob + o * 16, v[o]) : up<T, false>(k, u, q, ord.n, rest, ob + o * 16, v[o]);
+        }
+        if (slot > -3) {
+#pragma unroll
+            for (int o = 0; o < 4; ++o)
+                if (ob + o * 16 + 4 * kl < k.d_out) put<T>(k, y, ldy, request, ob + o * 16 + 4 * kl, slot, v[o], vec_out);
         }
     }
 }
