@@ -30,13 +30,14 @@ class QueryAdapters:
     its last rows of A and columns of B."""
 
     def __init__(self, weight, A, B, scale=None):
-        import torch
+        torch = dt.torch_module()
         self._lib = dt.engine_for(weight, "weight")
+        self._index = weight.get_device()
         if weight.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("weight must be of type float32 or bfloat16, got %s" % weight.dtype)
-        dt.check(weight, "weight", weight.dtype, (None, None))
+        dt.check(weight, "weight", weight.dtype, (None, None), self._index)
         self.d_out, self.d_in = (int(v) for v in weight.shape)
-        dt.check(A, "A", weight.dtype, (None, None, self.d_in), weight)
+        dt.check(A, "A", weight.dtype, (None, None, self.d_in), self._index)
         self.n_slots, self.rank = int(A.shape[0]), int(A.shape[1])
         if not 1 <= self.n_slots <= MAX_SLOTS or not 1 <= self.rank <= MAX_RANK:
             raise ValueError("%d slots of rank %d: 1 to %d slots of rank 1 to %d are served"
@@ -47,38 +48,39 @@ class QueryAdapters:
             scale = torch.ones(self.n_slots, dtype=torch.float32, device=weight.device)
         self.weight, self.A, self.B, self.scale = weight, A, B, scale
         self._code = _lib.DTYPE_BF16 if weight.dtype == torch.bfloat16 else _lib.DTYPE_F32
+        self._dtype, self._f32, self._i64 = weight.dtype, torch.float32, torch.int64
+        self._shapes = ((self.d_out, self.d_in), (self.n_slots, self.rank, self.d_in), (self.n_slots, self.d_out, self.rank),
+                        (self.n_slots,))
+        self._ws_bytes = {}
         self._weights()
 
     @property
     def dtype(self):
-        return self.weight.dtype
+        return self._dtype
 
     @property
     def device(self):
         return self.weight.device
 
     def _weights(self):
-        """Pointers of the bank as it is now (the attributes may have been replaced since)."""
-        import torch
-        t, w = self.weight.dtype, self.weight
-        dt.check(w, "weight", t, (self.d_out, self.d_in))
-        dt.check(self.A, "A", t, (self.n_slots, self.rank, self.d_in), w)
-        dt.check(self.B, "B", t, (self.n_slots, self.d_out, self.rank), w)
-        dt.check(self.scale, "scale", torch.float32, (self.n_slots,), w)
-        for name in ("weight", "A", "B", "scale"):
-            if not getattr(self, name).is_contiguous():
+        """Pointers of the bank as it is now (the tensors may have been replaced since)."""
+        out = []
+        for name, t, shape in zip(("weight", "A", "B", "scale"), (self.weight, self.A, self.B, self.scale), self._shapes):
+            dt.check(t, name, self._f32 if name == "scale" else self._dtype, shape, self._index)
+            if not t.is_contiguous():
                 raise ValueError("%s must be contiguous" % name)
-        return [C.c_void_p(p.data_ptr()) for p in (w, self.A, self.B, self.scale)]
+            out.append(t.data_ptr())
+        return out
 
     def slots_tensor(self, slots, n):
         """slots as the kernels read them: int64, n of them, in HBM.  A sequence of integers (None: no adapter) is checked
         here; a tensor on the GPU is taken as it is (a request outside [-1, n_slots) gets NaN)."""
-        import torch
+        torch = dt.torch_module()
         if dt.is_tensor(slots):
-            if slots.dtype not in (torch.int64, torch.int32):
-                raise ValueError("slots must be int64 or int32, got %s" % slots.dtype)
-            dt.check(slots, "slots", slots.dtype, (n,), self.weight)
-            return slots.to(torch.int64).contiguous()
+            if slots.dtype == torch.int32:
+                slots = slots.to(torch.int64)
+            dt.check(slots, "slots", self._i64, (n,), self._index)
+            return slots if slots.is_contiguous() else slots.contiguous()
         host = np.array([-1 if s is None else s for s in np.asarray(slots, dtype=object).reshape(-1)], dtype=object)
         if len(host) != n:
             raise ValueError("%d slots for %d requests" % (len(host), n))
@@ -87,58 +89,62 @@ class QueryAdapters:
         return torch.from_numpy(host.astype(np.int64)).to(self.device)
 
     def _input(self, t, name, width):
-        dt.check(t, name, self.weight.dtype, (None, width), self.weight)
+        dt.check(t, name, self._dtype, (None, width), self._index)
         if t.shape[0] > MAX_REQUESTS:
             raise ValueError("%s has %d rows: at most %d are served" % (name, t.shape[0], MAX_REQUESTS))
-        return dt.rows(t.detach())
+        return dt.rows(t.detach() if t.requires_grad else t)
 
     def _workspace(self, n, want_grad):
-        need = C.c_int64()
-        _lib.check(self._lib.rag_adapter_ws_bytes(self._code, n, self.d_in, self.d_out, self.n_slots, self.rank,
-                                                  1 if want_grad else 0, C.byref(need)), self._lib)
-        return dt.workspace(need.value, self.weight), need.value
+        need = self._ws_bytes.get((n, want_grad))
+        if need is None:
+            out = C.c_int64()
+            _lib.check(self._lib.rag_adapter_ws_bytes(self._code, n, self.d_in, self.d_out, self.n_slots, self.rank, want_grad,
+                                                      C.byref(out)), self._lib)
+            if len(self._ws_bytes) > 4096:
+                self._ws_bytes.clear()
+            need = self._ws_bytes[(n, want_grad)] = out.value
+        return dt.workspace(need, self.weight), need
 
     def apply(self, x, slots):
         """x: n x d_in, of the bank's type, in HBM.  Returns y, n x d_out, of the same type (rounded once from float32
         sums).  On torch's current stream; may be captured into a graph (with slots in HBM)."""
-        import torch
         x, ldx = self._input(x, "x", self.d_in)
-        n = int(x.shape[0])
+        n = x.shape[0]
         slots = self.slots_tensor(slots, n)
         w, a, b, scale = self._weights()
-        y = torch.empty((n, self.d_out), dtype=x.dtype, device=x.device)
-        ws, ws_bytes = self._workspace(n, False)
-        _lib.check(self._lib.rag_adapter_apply_dev(
-            self._code, n, self.d_in, self.d_out, self.n_slots, self.rank, C.c_void_p(x.data_ptr()), ldx, w, a, b, scale,
-            C.c_void_p(slots.data_ptr()), C.c_void_p(y.data_ptr()), self.d_out, C.c_void_p(ws.data_ptr()), ws_bytes,
-            C.c_void_p(dt.stream_of(x))), self._lib)
+        y = x.new_empty((n, self.d_out))
+        ws, ws_bytes = self._workspace(n, 0)
+        rc = self._lib.rag_adapter_apply_dev(self._code, n, self.d_in, self.d_out, self.n_slots, self.rank, x.data_ptr(), ldx, w, a, b,
+                                             scale, slots.data_ptr(), y.data_ptr(), self.d_out, ws.data_ptr(), ws_bytes,
+                                             dt.stream_of(x))
+        if rc:
+            _lib.check(rc, self._lib)
         return y
 
     def grad(self, x, slots, dy, input_grad=True):
         """Backward of apply(): (dx, dA, dB) for the gradient dy of y.  dx has the type of x (None with
         input_grad=False: embeddings of a frozen model need none); dA and dB are float32 and whole (zeros for slots
         that no request has).  Equal calls give equal bits."""
-        import torch
         x, ldx = self._input(x, "x", self.d_in)
         dy, lddy = self._input(dy, "dy", self.d_out)
-        n = int(x.shape[0])
+        n = x.shape[0]
         if dy.shape[0] != n:
             raise ValueError("dy has %d rows, x has %d" % (dy.shape[0], n))
         slots = self.slots_tensor(slots, n)
         w, a, b, scale = self._weights()
-        dx = torch.empty((n, self.d_in), dtype=x.dtype, device=x.device) if input_grad else None
-        dA = torch.empty(self.A.shape, dtype=torch.float32, device=x.device)
-        dB = torch.empty(self.B.shape, dtype=torch.float32, device=x.device)
-        ws, ws_bytes = self._workspace(n, True)
-        _lib.check(self._lib.rag_adapter_grad_dev(
-            self._code, n, self.d_in, self.d_out, self.n_slots, self.rank, C.c_void_p(x.data_ptr()), ldx, w, a, b, scale,
-            C.c_void_p(slots.data_ptr()), C.c_void_p(dy.data_ptr()), lddy,
-            C.c_void_p(dx.data_ptr() if input_grad else None), self.d_in, C.c_void_p(dA.data_ptr()),
-            C.c_void_p(dB.data_ptr()), C.c_void_p(ws.data_ptr()), ws_bytes, C.c_void_p(dt.stream_of(x))), self._lib)
+        dx = x.new_empty((n, self.d_in)) if input_grad else None
+        dA = x.new_empty(self._shapes[1], dtype=self._f32)
+        dB = x.new_empty(self._shapes[2], dtype=self._f32)
+        ws, ws_bytes = self._workspace(n, 1)
+        rc = self._lib.rag_adapter_grad_dev(self._code, n, self.d_in, self.d_out, self.n_slots, self.rank, x.data_ptr(), ldx, w, a, b,
+                                            scale, slots.data_ptr(), dy.data_ptr(), lddy, dx.data_ptr() if input_grad else None,
+                                            self.d_in, dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), ws_bytes, dt.stream_of(x))
+        if rc:
+            _lib.check(rc, self._lib)
         return dx, dA, dB
 
     def apply_host(self, x, slots):
         """apply() for a host array (n x d_in), as the embedding manager returns it: n x d_out float32 on the host."""
-        import torch
+        torch = dt.torch_module()
         x = np.ascontiguousarray(x, dtype=np.float32).reshape(-1, self.d_in)
         return self.apply(torch.from_numpy(x).to(self.device).to(self.dtype), slots).float().cpu().numpy()

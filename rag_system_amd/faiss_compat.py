@@ -36,6 +36,7 @@ class _HipFlatBackend:
         _lib.check(self._lib.rag_flat_create(int(d), int(metric), dtype, C.byref(h)), self._lib)
         self._h = h
         self.d = int(d)
+        self._ws_bytes = {}     # of distill(): they depend on its sizes alone
 
     def __del__(self):
         h, self._h = getattr(self, "_h", None), None
@@ -58,19 +59,24 @@ class _HipFlatBackend:
                    self._lib)
 
     def distill(self, q, ids, scores, temperature, teacher_temperature, over, weights, grad):
-        import torch
         q, ldq = dt.rows(q)
         nq, k = ids.shape
-        need = C.c_int64()
-        _lib.check(self._lib.rag_flat_distill_ws_bytes(self._h, nq, k, over, 1 if grad else 0, C.byref(need)), self._lib)
-        loss = torch.empty(nq, dtype=torch.float32, device=q.device)
-        dq = torch.empty((nq, self.d), dtype=q.dtype, device=q.device) if grad else None
-        ws = dt.workspace(need.value, q)
-        _lib.check(self._lib.rag_flat_distill_dev(
-            self._h, nq, C.c_void_p(q.data_ptr()), ldq, k, C.c_void_p(ids.data_ptr()), C.c_void_p(scores.data_ptr()),
-            float(temperature), float(teacher_temperature), over, C.c_void_p(None if weights is None else weights.data_ptr()),
-            C.c_void_p(loss.data_ptr()), C.c_void_p(dq.data_ptr() if grad else None), self.d, C.c_void_p(ws.data_ptr()),
-            need.value, C.c_void_p(dt.stream_of(q))), self._lib)
+        need = self._ws_bytes.get((nq, k, over, grad)) if over == _lib.OVER_INDEX else 0
+        if need is None:
+            out = C.c_int64()
+            _lib.check(self._lib.rag_flat_distill_ws_bytes(self._h, nq, k, over, grad, C.byref(out)), self._lib)
+            if len(self._ws_bytes) > 4096:
+                self._ws_bytes.clear()
+            need = self._ws_bytes[(nq, k, over, grad)] = out.value
+        loss = scores.new_empty(nq)
+        dq = q.new_empty((nq, self.d)) if grad else None
+        ws = dt.workspace(need, q) if need else None
+        rc = self._lib.rag_flat_distill_dev(
+            self._h, nq, q.data_ptr(), ldq, k, ids.data_ptr(), scores.data_ptr(), temperature, teacher_temperature, over,
+            None if weights is None else weights.data_ptr(), loss.data_ptr(), dq.data_ptr() if grad else None, self.d,
+            ws.data_ptr() if need else None, need, dt.stream_of(q))
+        if rc:
+            _lib.check(rc, self._lib)
         return loss, dq
 
     def add_synthetic(self, n, seed, first_global_row):
@@ -208,21 +214,21 @@ class IndexFlat:
         carry no autograd history: y.backward(dq), or adapters.QueryAdapters.grad(x, slots, dq).  A query without an
         entry has loss 0 and dq 0, one with a row number outside the index NaN.  On torch's current stream; may be
         captured into a graph behind any one call."""
-        import torch
         if over not in ("index", "list"):
             raise ValueError("over must be 'index' or 'list', got %r" % (over,))
         if not hasattr(self._b, "distill"):
             raise NotImplementedError("this index' backend has no distill()")
         dt.engine_for(q, "q")
-        dt.check(q, "q", torch.bfloat16 if self.storage == "bf16" else torch.float32, (None, self.d))
+        torch, gpu = dt.torch_module(), q.get_device()
+        dt.check(q, "q", torch.bfloat16 if self.storage == "bf16" else torch.float32, (None, self.d), gpu)
         nq = q.shape[0]
-        dt.check(ids, "ids", torch.int64, (nq, None), q)
-        dt.check(scores, "scores", torch.float32, tuple(ids.shape), q)
+        dt.check(ids, "ids", torch.int64, (nq, None), gpu)
+        dt.check(scores, "scores", torch.float32, ids.shape, gpu)
         if weights is not None:
-            dt.check(weights, "weights", torch.float32, (nq,), q)
-            weights = weights.detach().contiguous()
-        return self._b.distill(q.detach(), ids.contiguous(), scores.detach().contiguous(), temperature, teacher_temperature,
-                               _lib.OVER_INDEX if over == "index" else _lib.OVER_LIST, weights, bool(grad))
+            dt.check(weights, "weights", torch.float32, (nq,), gpu)
+            weights = weights.contiguous()
+        return self._b.distill(q, ids.contiguous(), scores.contiguous(), float(temperature), float(teacher_temperature),
+                               _lib.OVER_INDEX if over == "index" else _lib.OVER_LIST, weights, 1 if grad else 0)
 
     def search(self, x, k):
         x = np.ascontiguousarray(x, dtype=np.float32)
