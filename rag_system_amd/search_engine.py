@@ -45,7 +45,10 @@ class _Begun:
 
 class SearchEngine:
     def __init__(self, vector_storage, embedding_manager, cross_encoder=None, weight_dense=0.4, weight_bm25=0.3,
-                 weight_tfidf=0.3, verbose=False):
+                 weight_tfidf=0.3, verbose=False, query_adapters=None):
+        """query_adapters (not in the reference): an adapters.QueryAdapters bank that every dense query goes through, with
+        the slot that the call names (adapter=..., None: the shared projection alone)."""
+        self.query_adapters = query_adapters
         self.vector_storage = vector_storage
         self.embedding_manager = embedding_manager
         self.cross_encoder = cross_encoder
@@ -62,19 +65,20 @@ class SearchEngine:
 
     def search_with_strategy(self, query: str, strategy="faiss", top_k=10, retrieval_mode="chunk", threshold=0.0,
                              use_knee_detection: bool = False, use_mmr: bool = False, mmr_lambda: float = 0.5,
-                             max_context_bytes: int = None, mmr_reuse_index_vectors: bool = False) -> List[Dict[str, Any]]:
+                             max_context_bytes: int = None, mmr_reuse_index_vectors: bool = False,
+                             adapter: int = None) -> List[Dict[str, Any]]:
         strategy = strategy.lower().strip()
         retrieval_mode = retrieval_mode.lower().strip()
         self._debug("search_with_strategy strategy=%s top_k=%s mode=%s threshold=%s"
                     % (strategy, top_k, retrieval_mode, threshold))
         if strategy == "faiss":
-            results = self.search_faiss(query, top_k, retrieval_mode)
+            results = self.search_faiss(query, top_k, retrieval_mode, adapter=adapter)
         elif strategy == "bm25":
             results = self.search_bm25(query, top_k, retrieval_mode)
         elif strategy in ("ibrido", "hybrid"):
-            results = self.search_hybrid(query, top_k, retrieval_mode)
+            results = self.search_hybrid(query, top_k, retrieval_mode, adapter=adapter)
         elif strategy == "multi":
-            results = self.search_multi_representation(query, top_k, "document")
+            results = self.search_multi_representation(query, top_k, "document", adapter=adapter)
         elif strategy == "rrf":
             # everything behind the three rankings -- fusion, sort, cut, knee, threshold and (with
             # mmr_reuse_index_vectors) MMR -- in one engine call when it is served (rag_hybrid_rrf_mmr)
@@ -83,7 +87,7 @@ class SearchEngine:
                 post = {"threshold": threshold, "knee": bool(use_knee_detection),
                         "mmr": bool(use_mmr and mmr_reuse_index_vectors), "lambda": mmr_lambda,
                         "max_bytes": max_context_bytes}
-            results, final = self._search_rrf(query, top_k, post)
+            results, final = self._search_rrf(query, top_k, post, adapter)
             if final is not None:
                 kept, order = final
                 if not use_mmr or not kept:
@@ -91,7 +95,8 @@ class SearchEngine:
                 if order is not None:
                     return [kept[i] for i in order]
                 return self.mmr_selection(query, kept, self.embedding_manager, lambda_param=mmr_lambda, top_k=top_k,
-                                          max_context_bytes=max_context_bytes, reuse_index_vectors=mmr_reuse_index_vectors)
+                                          max_context_bytes=max_context_bytes, reuse_index_vectors=mmr_reuse_index_vectors,
+                                          adapter=adapter)
         else:
             raise ValueError(f"Unknown retrieval strategy: {strategy}")
         results.sort(key=_rank_key, reverse=True)
@@ -101,7 +106,8 @@ class SearchEngine:
         kept = [r for r in results if _rank_key(r) >= threshold]
         if use_mmr and kept:
             kept = self.mmr_selection(query, kept, self.embedding_manager, lambda_param=mmr_lambda, top_k=top_k,
-                                      max_context_bytes=max_context_bytes, reuse_index_vectors=mmr_reuse_index_vectors)
+                                      max_context_bytes=max_context_bytes, reuse_index_vectors=mmr_reuse_index_vectors,
+                                      adapter=adapter)
         return kept
 
     # ------------------------------------------------------------------ helpers
@@ -123,12 +129,27 @@ class SearchEngine:
                 g["chunks"].append(r["chunk"])
         return groups
 
-    def _dense_chunks_begin(self, query, k):
+    def _adapted(self, vecs, slots):
+        """Query embeddings through the bank, to unit length as embed_query's are (embedding_manager.py:92-97)."""
+        out = self.query_adapters.apply_host(vecs, slots)
+        norm = np.linalg.norm(out, axis=1, keepdims=True)
+        return out / np.where(norm < 1e-9, 1.0, norm).astype(np.float32)
+
+    def _query_vector(self, query, adapter=None, embedding_manager=None):
+        """The vector the dense index is searched with."""
+        v = (embedding_manager or self.embedding_manager).embed_query(query)
+        if self.query_adapters is None:
+            if adapter is not None:
+                raise ValueError("adapter=%r, but this SearchEngine has no query_adapters" % (adapter,))
+            return v
+        return self._adapted(np.asarray(v, dtype="float32").reshape(1, -1), [adapter]).reshape(np.asarray(v).shape[:-1] + (-1,))
+
+    def _dense_chunks_begin(self, query, k, adapter=None):
         """The dense pass in two halves: the reference computes the dense ranking and then the BM25
         ranking of the same query (search_engine.py:266-267, :230-231, :170-173); they do not depend
         on each other, so the flat search is enqueued here (rag_flat_search_begin) and the sparse
         scoring runs beside it.  Stores without the split (test backends) search at once."""
-        q_vec = self.embedding_manager.embed_query(query)
+        q_vec = self._query_vector(query, adapter)
         vs = self.vector_storage
         if hasattr(vs, "search_begin"):
             return _Begun(vs.search_begin(q_vec, top_k=k), q_vec)
@@ -163,14 +184,14 @@ class SearchEngine:
 
     # ------------------------------------------------------------------ single-signal strategies
 
-    def search_faiss(self, query: str, top_k=10, retrieval_mode="chunk") -> List[Dict[str, Any]]:
-        return self._search_faiss_end(self._search_faiss_begin(query, top_k, retrieval_mode))
+    def search_faiss(self, query: str, top_k=10, retrieval_mode="chunk", adapter: int = None) -> List[Dict[str, Any]]:
+        return self._search_faiss_end(self._search_faiss_begin(query, top_k, retrieval_mode, adapter))
 
-    def _search_faiss_begin(self, query, top_k, retrieval_mode):
+    def _search_faiss_begin(self, query, top_k, retrieval_mode, adapter=None):
         if "faiss" not in self.vector_storage.indices_present:
             return None
         k = top_k * 3 if retrieval_mode == "document" else top_k
-        return (self._dense_chunks_begin(query, k), query, top_k, retrieval_mode)
+        return (self._dense_chunks_begin(query, k, adapter), query, top_k, retrieval_mode)
 
     def _search_faiss_end(self, pending, want_text=True):
         """want_text=False (fusion strategies without a cross-encoder): the joined chunk texts of the document
@@ -203,16 +224,21 @@ class SearchEngine:
         results.sort(key=lambda x: x["score"], reverse=True)
         return results[:top_k]
 
-    def search_faiss_batch(self, queries, top_k=10, retrieval_mode="chunk") -> List[List[Dict[str, Any]]]:
+    def search_faiss_batch(self, queries, top_k=10, retrieval_mode="chunk", adapters=None) -> List[List[Dict[str, Any]]]:
         """search_faiss for a list of queries with ONE index.search(nq x d) call -- the batched
         front end the reference lacks (search_engine.py:141 is strictly one query).
         Element i equals search_faiss(queries[i], top_k, retrieval_mode) up to near-ties between
-        the batch and single-query kernels (both within the 1e-5 dense tolerance)."""
+        the batch and single-query kernels (both within the 1e-5 dense tolerance).  adapters: a slot per query (None: none),
+        with query_adapters -- the requests of many users in one call."""
         queries = list(queries)
+        if adapters is not None and (self.query_adapters is None or len(adapters) != len(queries)):
+            raise ValueError("adapters needs query_adapters and one slot per query")
         if "faiss" not in self.vector_storage.indices_present or not queries:
             return [[] for _ in queries]
         k = top_k * 3 if retrieval_mode == "document" else top_k
         q_vecs = self._embed_queries(queries)
+        if self.query_adapters is not None:
+            q_vecs = self._adapted(q_vecs, [None] * len(queries) if adapters is None else adapters)
         out = []
         for query, hits in zip(queries, self.vector_storage.search_batch(q_vecs, top_k=k)):
             for r in hits:
@@ -271,10 +297,10 @@ class SearchEngine:
 
     # ------------------------------------------------------------------ hybrid (dense + bm25, raw scores)
 
-    def search_hybrid(self, query: str, top_k=10, retrieval_mode="chunk") -> List[Dict[str, Any]]:
+    def search_hybrid(self, query: str, top_k=10, retrieval_mode="chunk", adapter: int = None) -> List[Dict[str, Any]]:
         pending = None
         if "faiss" in self.vector_storage.indices_present:
-            pending = self._dense_chunks_begin(query, top_k * 3 if retrieval_mode == "document" else top_k)
+            pending = self._dense_chunks_begin(query, top_k * 3 if retrieval_mode == "document" else top_k, adapter)
         sparse = []
         if "bm25" in self.vector_storage.indices_present:
             try:
@@ -362,8 +388,9 @@ class SearchEngine:
 
     # ------------------------------------------------------------------ multi (dense + bm25 + tfidf, max-normalised)
 
-    def search_multi_representation(self, query: str, top_k=10, retrieval_mode="document") -> List[Dict[str, Any]]:
-        pending = self._search_faiss_begin(query, top_k * 3, "document")
+    def search_multi_representation(self, query: str, top_k=10, retrieval_mode="document",
+                                    adapter: int = None) -> List[Dict[str, Any]]:
+        pending = self._search_faiss_begin(query, top_k * 3, "document", adapter)
         tf_begun = self._tfidf_begin(query, top_k * 7)     # beside the dense pass, like the BM25 scoring below
         try:
             bm25_hits = self.search_bm25(query, top_k=top_k * 3, retrieval_mode="document", _want_text=False)
@@ -412,8 +439,8 @@ class SearchEngine:
 
     # ------------------------------------------------------------------ rrf
 
-    def search_rrf(self, query: str, top_k=10, retrieval_mode="document") -> List[Dict[str, Any]]:
-        return self._search_rrf(query, top_k, None)[0]
+    def search_rrf(self, query: str, top_k=10, retrieval_mode="document", adapter: int = None) -> List[Dict[str, Any]]:
+        return self._search_rrf(query, top_k, None, adapter)[0]
 
     def _tfidf_rows(self, doc_ids):
         """TF-IDF row of every doc id (built once per store), or None without a TF-IDF index."""
@@ -427,7 +454,7 @@ class SearchEngine:
             vs._tfidf_pos = pos
         return pos[1]
 
-    def _search_rrf(self, query, top_k, post):
+    def _search_rrf(self, query, top_k, post, adapter=None):
         """search_rrf (:320-350).  post = None: plain.  post = {threshold, knee, mmr, lambda, max_bytes} (from
         search_with_strategy, no cross-encoder): what follows the fusion there (:121-133) may run in the same
         engine call; then the second return value is (kept results, MMR order or None), else it is None and
@@ -440,7 +467,7 @@ class SearchEngine:
                 tables_ok = bool(tables is not None and tables(self.vector_storage.get_tfidf_scorer()))
             except Exception as e:
                 self._debug("hybrid_doc_tables failed: %s" % e)
-        pending = self._search_faiss_begin(query, top_k * 3, "document")
+        pending = self._search_faiss_begin(query, top_k * 3, "document", adapter)
         tf_begun = self._tfidf_begin(query, top_k * 7)     # beside the dense pass, like the BM25 scoring below
         try:
             bm25_ranking = self.search_bm25(query, top_k=top_k * 3, retrieval_mode="document", _want_text=False)
@@ -458,7 +485,7 @@ class SearchEngine:
         # ---- one engine call for everything behind the rankings (rag_hybrid_rrf_mmr), when it is served
         if tf_begun is not None:
             try:
-                done = self._rrf_tail(query, top_k, post, pending, tf_begun, ordered, tables_ok)
+                done = self._rrf_tail(query, top_k, post, pending, tf_begun, ordered, tables_ok, adapter)
             except Exception:
                 self._tfidf_abort(tf_begun)
                 raise
@@ -485,7 +512,7 @@ class SearchEngine:
             combined = self.rerank_with_cross_encoder(query, combined, normalize_ce=True)
         return combined, None
 
-    def _rrf_tail(self, query, top_k, post, pending, tf_begun, ordered, tables_ok=False):
+    def _rrf_tail(self, query, top_k, post, pending, tf_begun, ordered, tables_ok=False, adapter=None):
         """The fused tail.  None = not served (the TF-IDF query is still begun); else _search_rrf's result."""
         scorer, tok = tf_begun
         if not hasattr(scorer, "hybrid_tail") or top_k > 64 or len(ordered[0]) > 128 or len(ordered[1]) > 128:
@@ -505,7 +532,7 @@ class SearchEngine:
             flat = self.vector_storage.index
             q_vec = np.asarray(pending[0].q_vec, dtype="float32").reshape(-1) if pending else None
             if q_vec is None:
-                q_vec = np.asarray(self.embedding_manager.embed_query(query), dtype="float32").reshape(-1)
+                q_vec = np.asarray(self._query_vector(query, adapter), dtype="float32").reshape(-1)
         out = scorer.hybrid_tail(tok, flat, rows[0], rows[1], top_k, 60,
                                  post["threshold"] if in_kernel else None, post["knee"] if in_kernel else False,
                                  q_vec, post["lambda"] if in_kernel else 0.5, post["max_bytes"] if in_kernel else None)
@@ -559,11 +586,50 @@ class SearchEngine:
         results.sort(key=lambda x: x["ce_score"], reverse=True)
         return results
 
+    # ------------------------------------------------------------------ training the query adapters
+
+    def distill_step(self, queries, adapters=None, top_k=30, temperature=0.05, teacher_temperature=1.0, over="index"):
+        """One training step's gradients of the query adapters (not in the reference): the cross-encoder, which the
+        strategies ask to re-rank a list (:362-394), teaches the dense score to rank like it.
+
+        The queries are embedded and sent through the bank, the index' top_k chunks for them scored by
+        cross_encoder.predict, and the KL divergence of its softmax(scores / teacher_temperature) from the dense
+        softmax(scores / temperature) -- over every row of the index, or over the list alone (over="list") -- taken back
+        to the adapters.  Returns (loss per query, dA, dB), torch tensors in HBM, gradients of the mean loss; the caller's
+        optimiser applies them to query_adapters.A / .B in place."""
+        bank, index = self.query_adapters, self.vector_storage.index
+        if bank is None or self.cross_encoder is None:
+            raise ValueError("distill_step needs query_adapters and a cross_encoder")
+        if getattr(index, "sharded", False):
+            raise NotImplementedError("distill_step needs the whole index on this GPU; this one is row-sharded")
+        queries = list(queries)
+        n = len(queries)
+        if n == 0 or index.ntotal == 0:
+            raise ValueError("distill_step needs queries and a filled index")
+        if adapters is not None and len(adapters) != n:
+            raise ValueError("%d adapters for %d queries" % (len(adapters), n))
+        from . import device_tensors as dt
+        torch = dt.torch_module()
+        slots = bank.slots_tensor([None] * n if adapters is None else adapters, n)
+        x = torch.from_numpy(np.ascontiguousarray(self._embed_queries(queries), dtype="float32")).to(bank.device).to(bank.dtype)
+        y = bank.apply(x, slots)
+        _, ids = index.search(y.float().cpu().numpy(), min(int(top_k), index.ntotal))
+        scores = np.full(ids.shape, -np.inf, dtype=np.float32)
+        chunks = self.vector_storage.chunks_data
+        at = [(i, j) for i in range(n) for j in range(ids.shape[1]) if ids[i, j] >= 0]
+        scores[tuple(zip(*at))] = np.asarray(
+            self.cross_encoder.predict([(queries[i], chunks[ids[i, j]]["chunk"]) for i, j in at]), dtype=np.float32).reshape(-1)
+        loss, dy = index.distill(y.to(torch.bfloat16 if index.storage == "bf16" else torch.float32),
+                                 torch.from_numpy(ids).to(bank.device), torch.from_numpy(scores).to(bank.device), temperature,
+                                 teacher_temperature, over, weights=torch.full((n,), 1.0 / n, device=bank.device))
+        _, dA, dB = bank.grad(x, slots, dy.to(bank.dtype), input_grad=False)
+        return loss, dA, dB
+
     # ------------------------------------------------------------------ MMR
 
     def mmr_selection(self, query: str, results: List[Dict[str, Any]], embedding_manager, lambda_param: float = 0.5,
                       top_k: int = None, max_context_bytes: int = None,
-                      reuse_index_vectors: bool = False) -> List[Dict[str, Any]]:
+                      reuse_index_vectors: bool = False, adapter: int = None) -> List[Dict[str, Any]]:
         """Greedy Maximal Marginal Relevance over the candidates' re-encoded texts; the cosine
         matrix and the greedy loop run in rag_mmr (csrc/cand.hip).
 
@@ -578,7 +644,7 @@ class SearchEngine:
             return results
         top_k = top_k if top_k is not None else len(results)
         texts = [r.get("chunk", r.get("text", "")) for r in results]
-        q = np.asarray(embedding_manager.embed_query(query), dtype="float32").reshape(-1)
+        q = np.asarray(self._query_vector(query, adapter, embedding_manager), dtype="float32").reshape(-1)
         byte_lens = [len(t.encode("utf-8")) for t in texts]
         if reuse_index_vectors:
             rows = self._chunk_rows(results)
