@@ -47,31 +47,40 @@ __device__ __forceinline__ int place_in_wave(int bits, int bin, bool live, int* 
     *of = __popcll(with);
     return __popcll(with & ((1ull << (threadIdx.x & 63)) - 1));
 }
+// f(request, bin, live) for 64 requests of the chunk at a time, eight lots of slots on their way at once.
+template <typename F>
+__device__ __forceinline__ void each_of_chunk(const Sort& s, int c, F f) {
+    const int lane = threadIdx.x & 63, end = min(s.n, (c + 1) * s.chunk);
+    for (int t0 = c * s.chunk; t0 < end; t0 += 512) {
+        int bin[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bin[j] = bin_of(s, min(t0 + j * 64 + lane, s.n - 1));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (t0 + j * 64 >= end) break;      // (uniform)
+            f(t0 + j * 64 + lane, bin[j], t0 + j * 64 + lane < end);
+        }
+    }
+}
 // counts[] += this wave's chunk; the last lane of a bin adds for all of them (one writer, no atomics)
 __device__ __forceinline__ void count_chunk(const Sort& s, int c, int* counts) {
-    const int lane = threadIdx.x & 63, end = min(s.n, (c + 1) * s.chunk);
-    for (int t0 = c * s.chunk; t0 < end; t0 += 64) {
-        const bool live = t0 + lane < end;
-        const int bin = live ? bin_of(s, t0 + lane) : -1;
+    each_of_chunk(s, c, [&](int, int bin, bool live) {
         int of = 0;
         const int at = place_in_wave(s.bits, bin, live, &of);
         if (live && at == of - 1) counts[bin] += of;
-    }
+    });
 }
 __device__ __forceinline__ void place_chunk(const Sort& s, int c, int* next) {
-    const int lane = threadIdx.x & 63, end = min(s.n, (c + 1) * s.chunk);
-    for (int t0 = c * s.chunk; t0 < end; t0 += 64) {
-        const bool live = t0 + lane < end;
-        const int bin = live ? bin_of(s, t0 + lane) : -1;
+    each_of_chunk(s, c, [&](int t, int bin, bool live) {
         int of = 0;
         const int at = place_in_wave(s.bits, bin, live, &of);
         const int to = live ? next[bin] + at : 0;
         if (live && at == of - 1) next[bin] = to + 1;
         if (live) {
-            s.perm[to] = t0 + lane;
+            s.perm[to] = t;
             s.slot_at[to] = bin < s.n_slots ? bin : bin == s.n_slots ? -1 : -2;
         }
-    }
+    });
 }
 // From the bins' totals (in LDS, destroyed): start[], and with items the list of items.  One workgroup of 1024.
 __device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int* tmp) {
@@ -85,19 +94,26 @@ __device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int
         sum[1] += it;
         sum[2] += it > 1 ? it : 0;
     }
-    for (int a = 0; a < 3; ++a) tmp[a * 1024 + threadIdx.x] = sum[a];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int upto[3] = {sum[0], sum[1], sum[2]};         // within the wave, then over the waves
+    for (int d = 1; d < 64; d *= 2)
+        for (int a = 0; a < 3; ++a) {
+            const int v = __shfl_up(upto[a], d);
+            upto[a] += lane >= d ? v : 0;
+        }
+    if (lane == 63)
+        for (int a = 0; a < 3; ++a) tmp[a * 16 + wave] = upto[a];
     __syncthreads();
-    for (int d = 1; d < 1024; d *= 2) {
-        int v[3];
-        for (int a = 0; a < 3; ++a) v[a] = threadIdx.x >= d ? tmp[a * 1024 + threadIdx.x - d] : 0;
-        __syncthreads();
-        for (int a = 0; a < 3; ++a) tmp[a * 1024 + threadIdx.x] += v[a];
-        __syncthreads();
+    int all_items = 0;
+    for (int w = 0; w < 16; ++w) {
+        all_items += tmp[16 + w];
+        if (w < wave)
+            for (int a = 0; a < 3; ++a) upto[a] += tmp[a * 16 + w];
     }
-    int at = tmp[threadIdx.x] - sum[0], item = tmp[1024 + threadIdx.x] - sum[1], part = tmp[2048 + threadIdx.x] - sum[2];
+    int at = upto[0] - sum[0], item = upto[1] - sum[1], part = upto[2] - sum[2];
     if (threadIdx.x == 0) {
         s.start[bins] = s.n;
-        if (s.items) *s.n_items = tmp[2047];
+        if (s.items) *s.n_items = all_items;
     }
     for (int b = b0; b < min(bins, b0 + per); ++b) {
         const int total = totals[b], it = items_of(b);
@@ -115,33 +131,6 @@ __device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int
     __syncthreads();
 }
 
-// All of it in one workgroup: sixteen waves, sixteen chunks, counts in LDS.
-constexpr int SMALL_BINS = 1026, SMALL_N = 16384;
-__global__ __launch_bounds__(1024) void order_small_kernel(Sort s) {
-    extern __shared__ int lds[];
-    const int bins = s.n_slots + 2, wave = threadIdx.x >> 6;
-    int* counts = lds;                 // 16 x bins
-    int* totals = counts + 16 * bins;  // bins
-    int* tmp = totals + bins;          // 3 x 1024
-    for (int j = threadIdx.x; j < 16 * bins; j += 1024) counts[j] = 0;
-    __syncthreads();
-    count_chunk(s, wave, counts + wave * bins);
-    __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 1024) {
-        int sum = 0;
-        for (int w = 0; w < 16; ++w) {
-            const int v = counts[w * bins + b];
-            counts[w * bins + b] = sum;
-            sum += v;
-        }
-        totals[b] = sum;
-    }
-    __syncthreads();
-    starts_and_items(s, totals, tmp);
-    for (int j = threadIdx.x; j < 16 * bins; j += 1024) counts[j] += totals[j % bins];
-    __syncthreads();
-    place_chunk(s, wave, counts + wave * bins);
-}
 __global__ __launch_bounds__(64) void count_kernel(Sort s) {
     extern __shared__ int lds[];
     const int bins = s.n_slots + 2;
@@ -199,21 +188,60 @@ struct Turn {
     int rows[3], cols[3], count[3];   // count matrices of rows x cols, dense
     int first[4];                     // first workgroup of each kind
 };
-template <typename T>
-__global__ __launch_bounds__(256) void turn_kernel(Turn j) {
-    __shared__ T tile[64][66];
+// One 64 x 64 tile by WAVES waves.
+template <typename T, int WAVES>
+__device__ __forceinline__ void turn_tile(const Turn& j, int block, T (*tile)[66]) {
     int kind = 0;
-    while (kind < 2 && (int)blockIdx.x >= j.first[kind + 1]) ++kind;
+    while (kind < 2 && block >= j.first[kind + 1]) ++kind;
     const int rows = j.rows[kind], cols = j.cols[kind], tr = (rows + 63) / 64, tc = (cols + 63) / 64;
-    const int b = blockIdx.x - j.first[kind], m = b / (tr * tc), r0 = b / tc % tr * 64, c0 = b % tc * 64;
+    const int b = block - j.first[kind], m = b / (tr * tc), r0 = b / tc % tr * 64, c0 = b % tc * 64;
     const T* from = static_cast<const T*>(j.from[kind]) + (long long)m * rows * cols;
     T* to = static_cast<T*>(j.to[kind]) + (long long)m * rows * cols;
     const int lane = threadIdx.x & 63;
-    for (int r = threadIdx.x >> 6; r < 64; r += 4)
+    for (int r = threadIdx.x >> 6; r < 64; r += WAVES)
         if (r0 + r < rows && c0 + lane < cols) tile[r][lane] = from[(long long)(r0 + r) * cols + c0 + lane];
     __syncthreads();
-    for (int c = threadIdx.x >> 6; c < 64; c += 4)
+    for (int c = threadIdx.x >> 6; c < 64; c += WAVES)
         if (c0 + c < cols && r0 + lane < rows) to[(long long)(c0 + c) * rows + r0 + lane] = tile[lane][c];
+}
+template <typename T>
+__global__ __launch_bounds__(256) void turn_kernel(Turn j) {
+    __shared__ T tile[64][66];
+    turn_tile<T, 4>(j, blockIdx.x, tile);
+}
+
+// All of it in one workgroup: sixteen waves, sixteen chunks, counts in LDS.
+constexpr int SMALL_BINS = 1026, SMALL_N = 16384;
+__device__ __forceinline__ void order_small(const Sort& s, int* lds) {
+    const int bins = s.n_slots + 2, wave = threadIdx.x >> 6;
+    int* counts = lds;                 // 16 x bins
+    int* totals = counts + 16 * bins;  // bins
+    int* tmp = totals + bins;          // 48
+    for (int j = threadIdx.x; j < 16 * bins; j += 1024) counts[j] = 0;
+    __syncthreads();
+    count_chunk(s, wave, counts + wave * bins);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += 1024) {
+        int sum = 0;
+        for (int w = 0; w < 16; ++w) {
+            const int v = counts[w * bins + b];
+            counts[w * bins + b] = sum;
+            sum += v;
+        }
+        totals[b] = sum;
+    }
+    __syncthreads();
+    starts_and_items(s, totals, tmp);
+    for (int j = threadIdx.x; j < 16 * bins; j += 1024) counts[j] += totals[j % bins];
+    __syncthreads();
+    place_chunk(s, wave, counts + wave * bins);
+}
+// The first workgroup sorts, the others turn the bank's matrices (none for a forward): a launch fewer.
+template <typename T>
+__global__ __launch_bounds__(1024) void prepare_kernel(Sort s, Turn j) {
+    extern __shared__ __align__(16) int prepare_lds[];
+    if (blockIdx.x == 0) order_small(s, prepare_lds);
+    else turn_tile<T, 16>(j, blockIdx.x - 1, reinterpret_cast<T(*)[66]>(prepare_lds));
 }
 
 // ---- gradients of the bank -----------------------------------------------------------------------------------------------
@@ -232,14 +260,13 @@ struct SlotGrad {
     bool vec_x, vec_dy;
 };
 template <typename T, int RT>
-__global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
-    constexpr int E = Mma<T>::E;
-    if ((int)blockIdx.x >= *g.s.n_items) return;
-    const Item it = g.s.items[blockIdx.x];
+__device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit) {
+    constexpr int E = Mma<T>::E, LOT = RT >= 4 ? 4 : 8;       // steps whose operands are on their way at once
+    if (item >= *g.s.n_items) return;
+    const Item it = g.s.items[item];
     const int lane = threadIdx.x & 63, li = lane & 15, kl = lane >> 4;
     const int rcs = (g.rank + RT * 16 - 1) / (RT * 16);
     const int cols_a = (g.d_in + 16 * E - 1) / (16 * E), cols_b = (g.d_out + 16 * E - 1) / (16 * E);
-    int unit = blockIdx.y * 4 + (threadIdx.x >> 6);
     if (unit >= (cols_a + cols_b) * rcs) return;      // (no barrier below)
     const bool is_b = unit >= cols_a * rcs;
     if (is_b) unit -= cols_a * rcs;
@@ -256,24 +283,30 @@ __global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
     for (int t0 = it.begin; t0 < it.end; t0 += 64) {
         const int mine = g.s.perm[min(t0 + lane, it.end - 1)];
         const int steps = (min(64, it.end - t0) + 3) / 4;
-        for (int st = 0; st < steps; ++st) {
-            const int t = t0 + st * 4 + kl;
-            const T* row = src + (long long)__shfl(mine, st * 4 + kl) * ld;
-            const unsigned keep = t < it.end ? ~0u : 0u;
-            u32x4 xv = vec ? piece<true>(row, c0, d) : piece<false>(row, c0, d);
+        for (int s0 = 0; s0 < steps; s0 += LOT) {
+            u32x4 xv[LOT];
+            float a[LOT][RT];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) xv[e] &= keep;
-            float a[RT];
+            for (int j = 0; j < LOT; ++j) {
+                const int t = t0 + (s0 + j) * 4 + kl;
+                const T* row = src + (long long)__shfl(mine, min((s0 + j) * 4 + kl, 63)) * ld;
+                xv[j] = vec ? piece<true>(row, c0, d) : piece<false>(row, c0, d);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const float f = cf[(long long)min(t, it.end - 1) * g.rp + min(r * 16 + li, g.rp - 1 - r0)];
-                a[r] = __uint_as_float(__float_as_uint(f) & keep);
+                for (int r = 0; r < RT; ++r) a[j][r] = cf[(long long)min(t, it.end - 1) * g.rp + min(r * 16 + li, g.rp - 1 - r0)];
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float b = element<T>(xv, e);
+            for (int j = 0; j < LOT; ++j) {
+                const unsigned keep = t0 + (s0 + j) * 4 + kl < it.end ? ~0u : 0u;
 #pragma unroll
-                for (int r = 0; r < RT; ++r) acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b, acc[r][e], 0, 0, 0);
+                for (int e = 0; e < 4; ++e) xv[j][e] &= keep;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) a[j][r] = __uint_as_float(__float_as_uint(a[j][r]) & keep);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float b = element<T>(xv[j], e);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j][r], b, acc[r][e], 0, 0, 0);
+                }
             }
         }
     }
@@ -289,6 +322,22 @@ __global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
                 const int rr = r0 + r * 16 + 4 * kl + i, cc = c0 + e;
                 if (rr < g.rank && cc < d) to[is_b ? (long long)cc * g.rank + rr : (long long)rr * g.d_in + cc] = acc[r][e][i];
             }
+}
+template <typename T, int RT>
+__global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
+    slot_grad<T, RT>(g, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 6));
+}
+// dx of a few requests and the bank's gradients, which do not depend on each other: a launch fewer, and neither waits for the
+// other's last workgroups.
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(512) void up_and_slot_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y, long long ldy,
+                                                          bool vec_out, unsigned up_groups, SlotGrad g, unsigned unit_groups) {
+    if (blockIdx.x < up_groups) {
+        up_direct<T, 1, 2, 8, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, blockIdx.x);
+        return;
+    }
+    const unsigned b = blockIdx.x - up_groups;
+    slot_grad<T, RT>(g, b / unit_groups, b % unit_groups * 8 + (threadIdx.x >> 6));
 }
 // The slots of several items: their partials, in order.
 __global__ __launch_bounds__(256) void slot_join_kernel(SlotGrad g) {
@@ -321,8 +370,9 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
         return at;
     };
     p.rp = (rank + unit - 1) / unit * unit;
-    // (few requests: sorting them costs a launch and saves little)
-    p.sorted = grad || n > 64;
+    // Unsorted where sorting would bring few neighbours together (less than 16 requests a slot on average) or saves little
+    // (one or two slots): it costs a launch, 7 us for 1000 requests.
+    p.sorted = grad || (n > 64 && n_slots > 2 && n > 16ll * n_slots);
     p.u = take((size_t)n * p.rp * 4);
     if (p.sorted) {
         const bool small = n <= SMALL_N && n_slots + 2 <= SMALL_BINS;
@@ -363,7 +413,8 @@ struct Call {
 
 bool aligned16(const void* p, long long ld, size_t esz) { return ((uintptr_t)p & 15) == 0 && ld * (long long)esz % 16 == 0; }
 
-int run_order(const Call& c, const Plan& p, Sort* out, bool items) {
+template <typename T>
+int run_order(const Call& c, const Plan& p, Sort* out, const Turn* turn) {      // turn: with the list of items, for the backward
     Sort s{};
     s.slots = c.slots;
     s.n = (int)c.n;
@@ -376,53 +427,65 @@ int run_order(const Call& c, const Plan& p, Sort* out, bool items) {
     s.slot_at = reinterpret_cast<int*>(c.ws + p.slot_at);
     s.counts = reinterpret_cast<int*>(c.ws + p.counts);
     s.start = reinterpret_cast<int*>(c.ws + p.start);
-    if (items) {
+    if (turn) {
         s.parts = reinterpret_cast<int2*>(c.ws + p.parts);
         s.n_items = reinterpret_cast<int*>(c.ws + p.n_items);
         s.items = reinterpret_cast<Item*>(c.ws + p.items);
     }
     *out = s;
     const size_t bins = c.n_slots + 2;
+    const unsigned tiles = turn ? (unsigned)turn->first[3] : 0;
     if (p.chunks == 0) {
-        const size_t lds = (17 * bins + 3 * 1024) * 4;
+        const size_t lds = std::max<size_t>((17 * bins + 48) * 4, 64 * 66 * sizeof(T));
         if (lds > 48 * 1024)
-            RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(order_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        order_small_kernel<<<1, 1024, lds, c.st>>>(s);
+            RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(prepare_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        prepare_kernel<T><<<1 + tiles, 1024, lds, c.st>>>(s, turn ? *turn : Turn{});
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
     count_kernel<<<(unsigned)p.chunks, 64, bins * 4, c.st>>>(s);
     RAG_HIP(hipGetLastError());
-    scan_kernel<<<1, 1024, (bins + 3 * 1024) * 4, c.st>>>(s);
+    scan_kernel<<<1, 1024, (bins + 1024) * 4, c.st>>>(s);
     RAG_HIP(hipGetLastError());
     place_kernel<<<(unsigned)p.chunks, 64, bins * 4, c.st>>>(s);
+    RAG_HIP(hipGetLastError());
+    if (tiles > 0) {
+        turn_kernel<T><<<tiles, 256, 0, c.st>>>(*turn);
+        RAG_HIP(hipGetLastError());
+    }
+    return RAG_OK;
+}
+
+// U of one bank, or U and V of two at once
+template <typename T, bool VEC>
+int launch_down(const Down& d, const Order& o, unsigned kinds, hipStream_t st) {
+    const Bank& k = d.bank[0];
+    // Few requests a slot (on average: the host does not see them): a matrix tile of 32 neighbours would go over its slots
+    // one after the other (64 requests of 64 slots, 768 wide: 85 us against 4 us).
+    if (o.n < 16ll * k.slots && o.n * k.rank * std::max(k.d_in, k.d_out) * (long long)sizeof(T) <= (256ll << 20)) {
+        down_each_kernel<T, VEC><<<dim3((unsigned)o.n, kinds), 256, 0, st>>>(d, o);
+        RAG_HIP(hipGetLastError());
+        return RAG_OK;
+    }
+    const dim3 groups((unsigned)((o.n + DOWN_TOKENS - 1) / DOWN_TOKENS), kinds);
+    if (k.rp <= 16) down_kernel<T, 1, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(d, o);
+    else if (k.rp <= 32) down_kernel<T, 2, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(d, o);
+    else if (k.rp <= 64) down_kernel<T, 4, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(d, o);
+    else down_kernel<T, 8, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(d, o);
     RAG_HIP(hipGetLastError());
     return RAG_OK;
 }
 
-template <typename T, bool VEC>
-int launch_down(const Bank& k, const Order& o, const void* x, long long ldx, float* u, hipStream_t st) {
-    // Few requests a slot (on average: the host does not see them): a matrix tile of 32 neighbours would go over its slots
-    // one after the other (64 requests of 64 slots, 768 wide: 85 us against 4 us).
-    if (o.n < 16ll * k.slots && o.n * k.rank * k.d_in * (long long)sizeof(T) <= (256ll << 20)) {
-        down_each_kernel<T, VEC><<<(unsigned)o.n, 256, 0, st>>>(k, o, x, ldx, u);
-        RAG_HIP(hipGetLastError());
-        return RAG_OK;
-    }
-    const unsigned groups = (unsigned)((o.n + DOWN_TOKENS - 1) / DOWN_TOKENS);
-    if (k.rp <= 16) down_kernel<T, 1, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
-    else if (k.rp <= 32) down_kernel<T, 2, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
-    else if (k.rp <= 64) down_kernel<T, 4, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
-    else down_kernel<T, 8, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(k, o, x, ldx, u);
-    RAG_HIP(hipGetLastError());
-    return RAG_OK;
+bool wants_tiles(const Bank& k, const Order& o, long long ldx, size_t esz) {
+    const long long tiles = (o.n + TILED_POS - 1) / TILED_POS * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS);
+    return tiles >= 128 && (unsigned long long)o.n * ldx * esz < (1ull << 32);
 }
 
 template <typename T, bool VEC>
 int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const float* u, void* y, long long ldy, hipStream_t st) {
     const bool vec_out = ldy % 4 == 0 && ((uintptr_t)y & 15) == 0;
-    const unsigned tiles = (unsigned)((o.n + TILED_POS - 1) / TILED_POS * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
-    if (VEC && tiles >= 128 && (unsigned long long)o.n * ldx * sizeof(T) < (1ull << 32)) {
+    if (VEC && wants_tiles(k, o, ldx, sizeof(T))) {
+        const unsigned tiles = (unsigned)((o.n + TILED_POS - 1) / TILED_POS * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
         auto fn = k.rank <= 4 * Mma<T>::E ? up_tiled_kernel<T, 1> : up_tiled_kernel<T, 2>;
         RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, TILED_LDS));
         fn<<<tiles, 512, TILED_LDS, st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy, vec_out);
@@ -438,15 +501,6 @@ int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const
     return RAG_OK;
 }
 
-// U and, with y, Y of a bank
-template <typename T>
-int run_product(const Bank& k, const Order& o, const void* x, long long ldx, float* u, void* y, long long ldy, hipStream_t st) {
-    const bool vec = k.vec_in && aligned16(x, ldx, sizeof(T));
-    int rc = vec ? launch_down<T, true>(k, o, x, ldx, u, st) : launch_down<T, false>(k, o, x, ldx, u, st);
-    if (rc || !y) return rc;
-    return vec ? launch_up<T, true>(k, o, x, ldx, u, y, ldy, st) : launch_up<T, false>(k, o, x, ldx, u, y, ldy, st);
-}
-
 Bank make_bank(const Call& c, const Plan& p, const void* w, const void* a, const void* b, int d_in, int d_out) {
     const int e = c.dtype == RAG_DTYPE_BF16 ? 8 : 4;
     Bank k{w, a, b, c.scale, d_in, d_out, c.n_slots, c.rank, p.rp, false, false};
@@ -460,53 +514,68 @@ int run_apply(const Call& c, const Plan& p) {
     Order o{nullptr, nullptr, c.slots, c.n, c.n_slots};
     if (p.sorted) {
         Sort s;
-        const int rc = run_order(c, p, &s, false);
+        const int rc = run_order<T>(c, p, &s, nullptr);
         if (rc) return rc;
         o.perm = s.perm;
         o.slot_at = s.slot_at;
     }
-    return run_product<T>(make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out), o, c.x, c.ldx, reinterpret_cast<float*>(c.ws + p.u), c.y, c.ldy, c.st);
+    const Bank k = make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out);
+    float* u = reinterpret_cast<float*>(c.ws + p.u);
+    const Down d{{k, k}, {c.x, nullptr}, {c.ldx, 0}, {u, nullptr}};
+    if (k.vec_in && aligned16(c.x, c.ldx, sizeof(T))) {
+        const int rc = launch_down<T, true>(d, o, 1, c.st);
+        return rc ? rc : launch_up<T, true>(k, o, c.x, c.ldx, u, c.y, c.ldy, c.st);
+    }
+    const int rc = launch_down<T, false>(d, o, 1, c.st);
+    return rc ? rc : launch_up<T, false>(k, o, c.x, c.ldx, u, c.y, c.ldy, c.st);
 }
 
 template <typename T>
 int run_grad(const Call& c, const Plan& p) {
+    // the transposed bank: B always (v), W and A for dx
+    Turn t{};
+    const void* from[3] = {c.b, c.w, c.a};
+    void* to[3] = {c.ws + p.bt, c.ws + p.wt, c.ws + p.at};
+    const int rows[3] = {c.d_out, c.d_out, c.rank}, cols[3] = {c.rank, c.d_in, c.d_in}, count[3] = {c.n_slots, 1, c.n_slots};
+    for (int i = 0; i < 3; ++i) {
+        t.from[i] = from[i];
+        t.to[i] = to[i];
+        t.rows[i] = rows[i];
+        t.cols[i] = cols[i];
+        t.first[i + 1] = t.first[i] + (c.n > 0 && (i == 0 || c.dx) ? count[i] * ((rows[i] + 63) / 64) * ((cols[i] + 63) / 64) : 0);
+    }
     Sort s;
-    int rc = run_order(c, p, &s, true);
+    int rc = run_order<T>(c, p, &s, &t);
     if (rc) return rc;
+    constexpr int E = Mma<T>::E;
     const Order o{s.perm, s.slot_at, c.slots, c.n, c.n_slots};
     float* u = reinterpret_cast<float*>(c.ws + p.u);
     float* v = reinterpret_cast<float*>(c.ws + p.v);
+    const SlotGrad g{s, u, v, c.x, c.dy, c.ldx, c.lddy, c.da, c.db, reinterpret_cast<float*>(c.ws + p.part), c.d_in, c.d_out, c.rank, p.rp,
+                     c.d_in % E == 0 && aligned16(c.x, c.ldx, sizeof(T)), c.d_out % E == 0 && aligned16(c.dy, c.lddy, sizeof(T))};
+    const Bank fore = make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out), back = make_bank(c, p, to[1], to[0], to[2], c.d_out, c.d_in);
+    const bool vec = fore.vec_in && g.vec_x && back.vec_in && g.vec_dy;
     if (c.n > 0) {
-        // the transposed bank: B always (v), W and A for dx
-        Turn t{};
-        const void* from[3] = {c.b, c.w, c.a};
-        void* to[3] = {c.ws + p.bt, c.ws + p.wt, c.ws + p.at};
-        const int rows[3] = {c.d_out, c.d_out, c.rank}, cols[3] = {c.rank, c.d_in, c.d_in}, count[3] = {c.n_slots, 1, c.n_slots};
-        int at = 0;
-        for (int i = 0; i < 3; ++i) {
-            t.from[i] = from[i];
-            t.to[i] = to[i];
-            t.rows[i] = rows[i];
-            t.cols[i] = cols[i];
-            t.count[i] = i == 0 || c.dx ? count[i] : 0;
-            t.first[i] = at;
-            at += t.count[i] * ((rows[i] + 63) / 64) * ((cols[i] + 63) / 64);
-        }
-        t.first[3] = at;
-        turn_kernel<T><<<(unsigned)at, 256, 0, c.st>>>(t);
-        RAG_HIP(hipGetLastError());
-        rc = run_product<T>(make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out), o, c.x, c.ldx, u, nullptr, 0, c.st);
-        if (rc) return rc;
-        rc = run_product<T>(make_bank(c, p, to[1], to[0], to[2], c.d_out, c.d_in), o, c.dy, c.lddy, v, c.dx, c.lddx, c.st);
+        const Down d{{fore, back}, {c.x, c.dy}, {c.ldx, c.lddy}, {u, v}};
+        rc = vec ? launch_down<T, true>(d, o, 2, c.st) : launch_down<T, false>(d, o, 2, c.st);
         if (rc) return rc;
     }
-    constexpr int E = Mma<T>::E;
-    SlotGrad g{s, u, v, c.x, c.dy, c.ldx, c.lddy, c.da, c.db, reinterpret_cast<float*>(c.ws + p.part), c.d_in, c.d_out, c.rank, p.rp,
-               c.d_in % E == 0 && aligned16(c.x, c.ldx, sizeof(T)), c.d_out % E == 0 && aligned16(c.dy, c.lddy, sizeof(T))};
+    const bool together = c.n > 0 && c.dx && !(vec && wants_tiles(back, o, c.lddy, sizeof(T)));
+    if (c.n > 0 && c.dx && !together) {
+        rc = launch_up<T, true>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, c.st);
+        if (rc) return rc;
+    }
     auto launch = [&](auto rt) {
         constexpr int RT = rt.value;
         const int units = ((c.d_in + 16 * E - 1) / (16 * E) + (c.d_out + 16 * E - 1) / (16 * E)) * ((c.rank + 16 * RT - 1) / (16 * RT));
-        slot_grad_kernel<T, RT><<<dim3((unsigned)p.max_items, (unsigned)((units + 3) / 4)), 256, 0, c.st>>>(g);
+        if (!together) {
+            slot_grad_kernel<T, RT><<<dim3((unsigned)p.max_items, (unsigned)((units + 3) / 4)), 256, 0, c.st>>>(g);
+            return;
+        }
+        const unsigned ups = (unsigned)((c.d_in + 15) / 16 * ((c.n + 31) / 32)), groups = (unsigned)((units + 7) / 8);
+        const bool vec_out = c.lddx % 4 == 0 && ((uintptr_t)c.dx & 15) == 0;
+        auto fn = vec ? up_and_slot_kernel<T, RT, true> : up_and_slot_kernel<T, RT, false>;
+        fn<<<ups + (unsigned)p.max_items * groups, 512, 0, c.st>>>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, vec_out, ups, g, groups);
     };
     if (c.rank <= 16) launch(std::integral_constant<int, 1>());
     else if (c.rank <= 32) launch(std::integral_constant<int, 2>());

@@ -95,16 +95,27 @@ __device__ __forceinline__ float element(u32x4 p, int e) {
     return __uint_as_float(e & 1 ? p[e >> 1] & 0xffff0000u : p[e >> 1] << 16);
 }
 
+// Up to two products of this kind in a launch (blockIdx.y): U, and V in a backward.
+struct Down {
+    Bank bank[2];
+    const void* x[2];
+    long long ldx[2];
+    float* u[2];
+};
+
 // U (or V) of 32 positions: four waves take every fourth step along d_in, their sums meet in LDS.
 constexpr int DOWN_TOKENS = 32, DOWN_WAVES = 4;
 template <typename T, int RT, bool VEC>
-__global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Bank k, Order ord, const void* xv, long long ldx, float* u) {
+__global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Down d, Order ord) {
+    const Bank& k = d.bank[blockIdx.y];
+    const long long ldx = d.ldx[blockIdx.y];
+    float* u = d.u[blockIdx.y];
     typedef Mma<T> M;
     constexpr int E = M::E;
     __shared__ float part[DOWN_WAVES][2 * RT][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, kl = lane >> 4;
     const long long p0 = (long long)blockIdx.x * DOWN_TOKENS;
-    const T* x = static_cast<const T*>(xv);
+    const T* x = static_cast<const T*>(d.x[blockIdx.y]);
     const T* row[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) row[t] = x + ord.request(min(p0 + t * 16 + li, ord.n - 1)) * ldx;
@@ -171,7 +182,9 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Bank k, Order ord
 
 // U where slots have few requests each: a workgroup per position, a wave per row of A_s.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void down_each_kernel(Bank k, Order ord, const void* xv, long long ldx, float* u) {
+__global__ __launch_bounds__(256) void down_each_kernel(Down d, Order ord) {
+    const Bank& k = d.bank[blockIdx.y];
+    float* u = d.u[blockIdx.y];
     constexpr int E = Mma<T>::E;
     const long long p = blockIdx.x;
     const int s = ord.slot(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -179,7 +192,7 @@ __global__ __launch_bounds__(256) void down_each_kernel(Bank k, Order ord, const
         for (int r = threadIdx.x; r < k.rp; r += 256) u[p * k.rp + r] = s == -2 ? NAN : 0.f;
         return;
     }
-    const T* x = static_cast<const T*>(xv) + ord.request(p) * ldx;
+    const T* x = static_cast<const T*>(d.x[blockIdx.y]) + ord.request(p) * d.ldx[blockIdx.y];
     const T* a = static_cast<const T*>(k.a) + (long long)s * k.rank * k.d_in;
     const float scale = k.scale[s];
     for (int r0 = wave * 4; r0 < k.rp; r0 += 16) {
@@ -284,15 +297,15 @@ __device__ __forceinline__ void put(const Bank& k, void* y, long long ldy, long 
 // Y for a few requests: a workgroup has OT x 16 output columns and TT x 16 positions, its waves every WAVES-th step along d_in,
 // straight from memory (each byte is used by one wave, LDS would only add a trip); their sums meet in LDS, a wave finishes a tile.
 template <typename T, int OT, int TT, int WAVES, bool VEC>
-__global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y,
-                                                               long long ldy, bool vec_out) {
+__device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const void* xv, long long ldx, const float* u, void* y,
+                                          long long ldy, bool vec_out, int block) {
     typedef Mma<T> M;
     constexpr int E = M::E;
     __shared__ float part[WAVES][OT * TT][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, kl = lane >> 4;
     const int outs = (k.d_out + 16 * OT - 1) / (16 * OT);        // (neighbours share their requests' rows)
-    const long long p0 = (long long)(blockIdx.x / outs) * TT * 16;
-    const int o0 = blockIdx.x % outs * OT * 16;
+    const long long p0 = (long long)(block / outs) * TT * 16;
+    const int o0 = block % outs * OT * 16;
     const T* x = static_cast<const T*>(xv);
     const T* row[TT];
     const T* w[OT];
@@ -343,6 +356,12 @@ __global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord
         else sum = up<T, false>(k, u, p, ord.n, slot, o, sum);
         if (pos < ord.n && o + 4 * kl < k.d_out) put<T>(k, y, ldy, ord.request(pos), o + 4 * kl, slot, sum, vec_out);
     }
+}
+
+template <typename T, int OT, int TT, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y,
+                                                               long long ldy, bool vec_out) {
+    up_direct<T, OT, TT, WAVES, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, blockIdx.x);
 }
 
 // Y for many requests: a workgroup has 128 output columns x 256 positions, each of its eight waves 64 x 64 (an operand read for
