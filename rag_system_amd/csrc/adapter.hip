@@ -259,15 +259,16 @@ struct SlotGrad {
     int d_in, d_out, rank, rp;
     bool vec_x, vec_dy;
 };
+// Four waves share an item and a unit, 64 requests at a time each; their sums meet in LDS.  (They take the same branches:
+// every wave of the workgroup comes to the barriers.)
 template <typename T, int RT>
-__device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit) {
+__device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit, float (*part)[4][256]) {
     constexpr int E = Mma<T>::E, LOT = RT >= 4 ? 4 : 8;       // steps whose operands are on their way at once
-    if (item >= *g.s.n_items) return;
-    const Item it = g.s.items[item];
-    const int lane = threadIdx.x & 63, li = lane & 15, kl = lane >> 4;
+    const int lane = threadIdx.x & 63, li = lane & 15, kl = lane >> 4, team = threadIdx.x >> 6 & 3;
     const int rcs = (g.rank + RT * 16 - 1) / (RT * 16);
     const int cols_a = (g.d_in + 16 * E - 1) / (16 * E), cols_b = (g.d_out + 16 * E - 1) / (16 * E);
-    if (unit >= (cols_a + cols_b) * rcs) return;      // (no barrier below)
+    const bool live = item < *g.s.n_items && unit < (cols_a + cols_b) * rcs;
+    const Item it = live ? g.s.items[item] : Item{0, 0, 0, -1};
     const bool is_b = unit >= cols_a * rcs;
     if (is_b) unit -= cols_a * rcs;
     const int r0 = unit % rcs * RT * 16, c0 = unit / rcs * 16 * E + li * E, d = is_b ? g.d_out : g.d_in;
@@ -280,7 +281,7 @@ __device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit)
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int t0 = it.begin; t0 < it.end; t0 += 64) {
+    for (int t0 = it.begin + team * 64; t0 < it.end; t0 += 256) {
         const int mine = g.s.perm[min(t0 + lane, it.end - 1)];
         const int steps = (min(64, it.end - t0) + 3) / 4;
         for (int s0 = 0; s0 < steps; s0 += LOT) {
@@ -313,31 +314,42 @@ __device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit)
     const long long size_a = (long long)g.rank * g.d_in, size_b = (long long)g.rank * g.d_out;
     float* to = it.part >= 0 ? g.part + it.part * (size_a + size_b) + (is_b ? size_a : 0)
                              : is_b ? g.db + it.slot * size_b : g.da + it.slot * size_a;
+    // four tiles at a time: each wave adds up one of them
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int e0 = 0; e0 < E; e0 += 4) {
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int rr = r0 + r * 16 + 4 * kl + i, cc = c0 + e;
-                if (rr < g.rank && cc < d) to[is_b ? (long long)cc * g.rank + rr : (long long)rr * g.d_in + cc] = acc[r][e][i];
-            }
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<f32x4*>(&part[team][e][lane * 4]) = acc[r][e0 + e];
+            __syncthreads();
+            f32x4 sum = *reinterpret_cast<const f32x4*>(&part[0][team][lane * 4]);
+#pragma unroll
+            for (int w = 1; w < 4; ++w) sum += *reinterpret_cast<const f32x4*>(&part[w][team][lane * 4]);
+            const int rr = r0 + r * 16 + 4 * kl, cc = c0 + e0 + team;
+            if (live && cc < d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (rr + i < g.rank) to[is_b ? (long long)cc * g.rank + rr + i : (long long)(rr + i) * g.d_in + cc] = sum[i];
+        }
 }
 template <typename T, int RT>
 __global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
-    slot_grad<T, RT>(g, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 6));
+    __shared__ float part[4][4][256];
+    slot_grad<T, RT>(g, blockIdx.x, blockIdx.y, part);
 }
 // dx of a few requests and the bank's gradients, which do not depend on each other: a launch fewer, and neither waits for the
 // other's last workgroups.
 template <typename T, int RT, bool VEC>
 __global__ __launch_bounds__(512) void up_and_slot_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y, long long ldy,
                                                           bool vec_out, unsigned up_groups, SlotGrad g, unsigned unit_groups) {
+    __shared__ float part[2][4][4][256];
     if (blockIdx.x < up_groups) {
         up_direct<T, 1, 2, 8, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, blockIdx.x);
         return;
     }
-    const unsigned b = blockIdx.x - up_groups;
-    slot_grad<T, RT>(g, b / unit_groups, b % unit_groups * 8 + (threadIdx.x >> 6));
+    const unsigned b = blockIdx.x - up_groups, half = threadIdx.x >> 8;
+    slot_grad<T, RT>(g, b / unit_groups, b % unit_groups * 2 + half, part[half]);
 }
 // The slots of several items: their partials, in order.
 __global__ __launch_bounds__(256) void slot_join_kernel(SlotGrad g) {
@@ -355,7 +367,7 @@ __global__ __launch_bounds__(256) void slot_join_kernel(SlotGrad g) {
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    bool sorted;
+    bool sorted, each;
     int rp, chunk, chunks, len, max_items, max_parts;
     size_t u, v, perm, slot_at, counts, start, parts, n_items, items, wt, at, bt, part, bytes;
 };
@@ -370,9 +382,12 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
         return at;
     };
     p.rp = (rank + unit - 1) / unit * unit;
-    // Unsorted where sorting would bring few neighbours together (less than 16 requests a slot on average) or saves little
-    // (one or two slots): it costs a launch, 7 us for 1000 requests.
-    p.sorted = grad || (n > 64 && n_slots > 2 && n > 16ll * n_slots);
+    // Few requests a slot (on average: the host does not see them): U request by request.  A matrix tile of 32 neighbours would go
+    // over its slots one after the other (64 requests of 64 slots, 768 wide: 85 us against 4 us); each A_s is read once per
+    // request, so only while that stays in the caches.
+    p.each = n_slots > 2 && n <= (grad ? 16ll : 32ll) * n_slots && n * rank * std::max(d_in, d_out) * (long long)esz <= (256ll << 20);
+    // Then nothing needs an order, and it costs a launch, 7 us for 1000 requests; nor do one or two slots.
+    p.sorted = grad || (n > 64 && n_slots > 2 && !p.each);
     p.u = take((size_t)n * p.rp * 4);
     if (p.sorted) {
         const bool small = n <= SMALL_N && n_slots + 2 <= SMALL_BINS;
@@ -384,7 +399,7 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
         p.start = take((size_t)(n_slots + 3) * 4);
     }
     if (grad) {
-        p.len = (int)std::max<long long>(64, ((n + 255) / 256 + 3) / 4 * 4);
+        p.len = (int)std::max<long long>(512, (n + 255) / 256);
         p.max_items = n_slots + (int)(n / p.len) + 1;
         p.max_parts = 2 * (int)(n / p.len) + 2;
         p.v = take((size_t)n * p.rp * 4);
@@ -458,11 +473,9 @@ int run_order(const Call& c, const Plan& p, Sort* out, const Turn* turn) {      
 
 // U of one bank, or U and V of two at once
 template <typename T, bool VEC>
-int launch_down(const Down& d, const Order& o, unsigned kinds, hipStream_t st) {
+int launch_down(const Plan& p, const Down& d, const Order& o, unsigned kinds, hipStream_t st) {
     const Bank& k = d.bank[0];
-    // Few requests a slot (on average: the host does not see them): a matrix tile of 32 neighbours would go over its slots
-    // one after the other (64 requests of 64 slots, 768 wide: 85 us against 4 us).
-    if (o.n < 16ll * k.slots && o.n * k.rank * std::max(k.d_in, k.d_out) * (long long)sizeof(T) <= (256ll << 20)) {
+    if (p.each) {
         down_each_kernel<T, VEC><<<dim3((unsigned)o.n, kinds), 256, 0, st>>>(d, o);
         RAG_HIP(hipGetLastError());
         return RAG_OK;
@@ -523,10 +536,10 @@ int run_apply(const Call& c, const Plan& p) {
     float* u = reinterpret_cast<float*>(c.ws + p.u);
     const Down d{{k, k}, {c.x, nullptr}, {c.ldx, 0}, {u, nullptr}};
     if (k.vec_in && aligned16(c.x, c.ldx, sizeof(T))) {
-        const int rc = launch_down<T, true>(d, o, 1, c.st);
+        const int rc = launch_down<T, true>(p, d, o, 1, c.st);
         return rc ? rc : launch_up<T, true>(k, o, c.x, c.ldx, u, c.y, c.ldy, c.st);
     }
-    const int rc = launch_down<T, false>(d, o, 1, c.st);
+    const int rc = launch_down<T, false>(p, d, o, 1, c.st);
     return rc ? rc : launch_up<T, false>(k, o, c.x, c.ldx, u, c.y, c.ldy, c.st);
 }
 
@@ -557,7 +570,7 @@ int run_grad(const Call& c, const Plan& p) {
     const bool vec = fore.vec_in && g.vec_x && back.vec_in && g.vec_dy;
     if (c.n > 0) {
         const Down d{{fore, back}, {c.x, c.dy}, {c.ldx, c.lddy}, {u, v}};
-        rc = vec ? launch_down<T, true>(d, o, 2, c.st) : launch_down<T, false>(d, o, 2, c.st);
+        rc = vec ? launch_down<T, true>(p, d, o, 2, c.st) : launch_down<T, false>(p, d, o, 2, c.st);
         if (rc) return rc;
     }
     const bool together = c.n > 0 && c.dx && !(vec && wants_tiles(back, o, c.lddy, sizeof(T)));
@@ -569,10 +582,10 @@ int run_grad(const Call& c, const Plan& p) {
         constexpr int RT = rt.value;
         const int units = ((c.d_in + 16 * E - 1) / (16 * E) + (c.d_out + 16 * E - 1) / (16 * E)) * ((c.rank + 16 * RT - 1) / (16 * RT));
         if (!together) {
-            slot_grad_kernel<T, RT><<<dim3((unsigned)p.max_items, (unsigned)((units + 3) / 4)), 256, 0, c.st>>>(g);
+            slot_grad_kernel<T, RT><<<dim3((unsigned)p.max_items, (unsigned)units), 256, 0, c.st>>>(g);
             return;
         }
-        const unsigned ups = (unsigned)((c.d_in + 15) / 16 * ((c.n + 31) / 32)), groups = (unsigned)((units + 7) / 8);
+        const unsigned ups = (unsigned)((c.d_in + 15) / 16 * ((c.n + 31) / 32)), groups = (unsigned)((units + 1) / 2);
         const bool vec_out = c.lddx % 4 == 0 && ((uintptr_t)c.dx & 15) == 0;
         auto fn = vec ? up_and_slot_kernel<T, RT, true> : up_and_slot_kernel<T, RT, false>;
         fn<<<ups + (unsigned)p.max_items * groups, 512, 0, c.st>>>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, vec_out, ups, g, groups);
