@@ -489,19 +489,24 @@ int launch_down(const Plan& p, const Down& d, const Order& o, unsigned kinds, hi
     return RAG_OK;
 }
 
-bool wants_tiles(const Bank& k, const Order& o, long long ldx, size_t esz) {
-    const long long tiles = (o.n + TILED_POS - 1) / TILED_POS * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS);
-    return tiles >= 128 && (unsigned long long)o.n * ldx * esz < (1ull << 32);
+// Positions of a workgroup of the tiled product, or 0: too few of them to fill the card, the direct one takes it.
+int tiled_positions(const Bank& k, const Order& o, long long ldx, size_t esz) {
+    if ((unsigned long long)o.n * ldx * esz >= (1ull << 32)) return 0;      // (rows are found by 32-bit offsets)
+    const long long outs = (k.d_out + TILED_OUTS - 1) / TILED_OUTS;
+    return (o.n + 255) / 256 * outs >= 128 ? 256 : (o.n + 63) / 64 * outs >= 128 ? 64 : 0;
 }
 
 template <typename T, bool VEC>
 int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const float* u, void* y, long long ldy, hipStream_t st) {
     const bool vec_out = ldy % 4 == 0 && ((uintptr_t)y & 15) == 0;
-    if (VEC && wants_tiles(k, o, ldx, sizeof(T))) {
-        const unsigned tiles = (unsigned)((o.n + TILED_POS - 1) / TILED_POS * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
-        auto fn = k.rank <= 4 * Mma<T>::E ? up_tiled_kernel<T, 1> : up_tiled_kernel<T, 2>;
-        RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, TILED_LDS));
-        fn<<<tiles, 512, TILED_LDS, st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy, vec_out);
+    const int pos = VEC ? tiled_positions(k, o, ldx, sizeof(T)) : 0;
+    if (pos > 0) {
+        const unsigned tiles = (unsigned)((o.n + pos - 1) / pos * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
+        const bool short_rank = k.rank <= 4 * Mma<T>::E;
+        auto fn = pos == 256 ? (short_rank ? up_tiled_kernel<T, 1, 256> : up_tiled_kernel<T, 2, 256>)
+                             : (short_rank ? up_tiled_kernel<T, 1, 64> : up_tiled_kernel<T, 2, 64>);
+        RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, tiled_lds_bytes(pos)));
+        fn<<<tiles, 512, tiled_lds_bytes(pos), st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy, vec_out);
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
@@ -573,7 +578,7 @@ int run_grad(const Call& c, const Plan& p) {
         rc = vec ? launch_down<T, true>(p, d, o, 2, c.st) : launch_down<T, false>(p, d, o, 2, c.st);
         if (rc) return rc;
     }
-    const bool together = c.n > 0 && c.dx && !(vec && wants_tiles(back, o, c.lddy, sizeof(T)));
+    const bool together = c.n > 0 && c.dx && !(vec && tiled_positions(back, o, c.lddy, sizeof(T)) > 0);
     if (c.n > 0 && c.dx && !together) {
         rc = launch_up<T, true>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, c.st);
         if (rc) return rc;

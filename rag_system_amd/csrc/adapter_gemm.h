@@ -364,22 +364,23 @@ __global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord
     up_direct<T, OT, TT, WAVES, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, blockIdx.x);
 }
 
-// Y for many requests: a workgroup has 128 output columns x 256 positions, each of its eight waves 64 x 64 (an operand read for
-// every two products; two waves on a SIMD, since an LDS-DMA instruction holds its wave for 60 to 180 cycles: four waves of
+// Y for many requests: a workgroup has 128 output columns x POS positions (256, or 64 where that would leave CUs idle), each of
+// its eight waves 64 x 64 (an operand read for every two products; 32 x 32:  for every one; two waves on a SIMD, since an LDS-DMA instruction holds its wave for 60 to 180 cycles: four waves of
 // 64 x 128 read less and took 199 us where these take 169, 65536 x 768 x 768 bf16), 128 bytes of every row a stage, three
 // stages by LDS-DMA.  Rows of 16-byte pieces only.
 // RS: 64-byte steps of the rank that a wave keeps of its slot's B rows while neighbours share the slot.
-constexpr int TILED_OUTS = 128, TILED_POS = 256;
-constexpr int TILED_LDS = 3 * (TILED_OUTS + TILED_POS) * 128;
-template <typename T, int RS>
+constexpr int TILED_OUTS = 128;
+constexpr int tiled_lds_bytes(int pos) { return 3 * (TILED_OUTS + pos) * 128; }
+template <typename T, int RS, int POS>
 __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, const void* xv, long long ldx, unsigned x_bytes, const float* u, void* y,
                                                           long long ldy, bool vec_out) {
     typedef Mma<T> M;
-    constexpr int E = M::E, ESZ = sizeof(T), ROWS = TILED_OUTS + TILED_POS, STAGE = ROWS * 128, LOADS = ROWS / 8 / 8;
+    constexpr int E = M::E, ESZ = sizeof(T), ROWS = TILED_OUTS + POS, STAGE = ROWS * 128, LOADS = ROWS / 8 / 8;
+    constexpr int WP = POS / 64 >= 4 ? 4 : 2, WO = 8 / WP, TO = 8 / WO, TP = POS / 16 / WP;   // waves, and tiles of a wave
     extern __shared__ __align__(16) char tiled_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, kl = lane >> 4;
     const int outs = (k.d_out + TILED_OUTS - 1) / TILED_OUTS;
-    const long long p0 = (long long)(blockIdx.x / outs) * TILED_POS;
+    const long long p0 = (long long)(blockIdx.x / outs) * POS;
     const int o0 = blockIdx.x % outs * TILED_OUTS;
     const int stages = (k.d_in * ESZ + 127) / 128;
     const int lr = lane >> 3, lp = (lane & 7) ^ lr;
@@ -397,28 +398,28 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
         distill::lds_dma16(a * 64 < TILED_OUTS ? k.w : xv, a * 64 < TILED_OUTS ? w_bytes : x_bytes, from[a] + col,
                            tiled_lds + b * STAGE + (a * 8 + wave) * 1024);
     };
-    f32x4 acc[4][4];
+    f32x4 acc[TO][TP];
 #pragma unroll
-    for (int o = 0; o < 4; ++o)
+    for (int o = 0; o < TO; ++o)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[o][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int wo = (wave & 1) * 64, wp = (wave >> 1) * 64, ob = o0 + wo;
+        for (int t = 0; t < TP; ++t) acc[o][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int wo = wave % WO * TO * 16, wp = wave / WO * TP * 16, ob = o0 + wo;
     int off[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) off[h] = li * 128 + (((h * 4 + kl) ^ (li & 7)) << 4);
     auto stage = [&](int t, int b, int b2, bool tail) __attribute__((always_inline)) {
         const char* ws = tiled_lds + b * STAGE + wo * 128;
         const char* xs = tiled_lds + b * STAGE + (TILED_OUTS + wp) * 128;
-        u32x4 a[2][4], v[2][4];
+        u32x4 a[2][TO], v[2][TP];
         auto read = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-            for (int o = 0; o < 4; ++o) a[h][o] = *reinterpret_cast<const u32x4*>(ws + o * 2048 + off[h]);
+            for (int o = 0; o < TO; ++o) a[h][o] = *reinterpret_cast<const u32x4*>(ws + o * 2048 + off[h]);
 #pragma unroll
-            for (int p = 0; p < 4; ++p) v[h][p] = *reinterpret_cast<const u32x4*>(xs + p * 2048 + off[h]);
+            for (int p = 0; p < TP; ++p) v[h][p] = *reinterpret_cast<const u32x4*>(xs + p * 2048 + off[h]);
             if (tail) {
                 const unsigned keep = t * 128 + (h * 4 + kl) * 16 < k.d_in * ESZ ? ~0u : 0u;
 #pragma unroll
-                for (int o = 0; o < 4; ++o) a[h][o] = u32x4{a[h][o][0] & keep, a[h][o][1] & keep, a[h][o][2] & keep, a[h][o][3] & keep};
+                for (int o = 0; o < TO; ++o) a[h][o] = u32x4{a[h][o][0] & keep, a[h][o][1] & keep, a[h][o][2] & keep, a[h][o][3] & keep};
             }
         };
         read(0);
@@ -427,11 +428,11 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int o = 0; o < 4; ++o) {
+            for (int o = 0; o < TO; ++o) {
 #pragma unroll
-                for (int p = 0; p < 4; ++p) acc[o][p] = M::mma(a[h][o], v[h][p], acc[o][p]);
+                for (int p = 0; p < TP; ++p) acc[o][p] = M::mma(a[h][o], v[h][p], acc[o][p]);
 #pragma unroll
-                for (int f = (h * 4 + o) * LOADS / 8; f < (h * 4 + o + 1) * LOADS / 8; ++f) fetch1(t + 2 < stages ? t + 2 : 0, b2, f);
+                for (int f = (h * TO + o) * LOADS / (2 * TO); f < (h * TO + o + 1) * LOADS / (2 * TO); ++f) fetch1(t + 2 < stages ? t + 2 : 0, b2, f);
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
         *request = (int)ord.request(min(pos, ord.n - 1));
     };
     look(0, &slot0, &request0);
-    u32x4 bv[4][RS];
+    u32x4 bv[TO][RS];
     f32x4 un[RS][E / 4];
     auto load_u = [&](int p, f32x4 (*to)[E / 4]) __attribute__((always_inline)) {
         const float* ur = u + min(p0 + wp + p * 16 + li, ord.n - 1) * k.rp;
@@ -460,7 +461,7 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
         if (s == kept) return;                  // (uniform)
         const T* bs = static_cast<const T*>(k.b) + (long long)s * k.d_out * k.rank;
 #pragma unroll
-        for (int o = 0; o < 4; ++o)
+        for (int o = 0; o < TO; ++o)
 #pragma unroll
             for (int r = 0; r < RS; ++r)
                 bv[o][r] = piece<true>(bs + (long long)min(ob + o * 16 + li, k.d_out - 1) * k.rank, (r * 4 + kl) * E, k.rank);
@@ -500,26 +501,26 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
     // The tiles go through LDS (the ring is done with) into a loop over the positions: the adapters' cases are too much code to
     // stand here eight times.  A tile's U is loaded while the tile before it is finished, B's rows stay while the slot does.
     __syncthreads();
-    char* tiles = tiled_lds + wave * 16 * 1024 + lane * 16;
+    char* tiles = tiled_lds + wave * TO * TP * 1024 + lane * 16;
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
+    for (int p = 0; p < TP; ++p)
 #pragma unroll
-        for (int o = 0; o < 4; ++o) *reinterpret_cast<f32x4*>(tiles + (p * 4 + o) * 1024) = acc[o][p];
+        for (int o = 0; o < TO; ++o) *reinterpret_cast<f32x4*>(tiles + (p * TO + o) * 1024) = acc[o][p];
     const bool kept_form = k.rank <= RS * 4 * E && k.vec_rank;      // (uniform)
     int next_slot = slot0, next_request = request0;
 #pragma unroll 1
-    for (int p = 0; p < 4; ++p) {
+    for (int p = 0; p < TP; ++p) {
         const long long q = p0 + wp + p * 16;
         const int slot = next_slot, request = next_request;
         u32x4 uh[RS], ul[RS];
         narrow(un, uh, ul);
-        if (p < 3) {
+        if (p < TP - 1) {
             look(p + 1, &next_slot, &next_request);
             load_u(p + 1, un);
         }
-        f32x4 v[4];
+        f32x4 v[TO];
 #pragma unroll
-        for (int o = 0; o < 4; ++o) v[o] = *reinterpret_cast<const f32x4*>(tiles + (p * 4 + o) * 1024);
+        for (int o = 0; o < TO; ++o) v[o] = *reinterpret_cast<const f32x4*>(tiles + (p * TO + o) * 1024);
         unsigned todo = (unsigned)__ballot(slot >= 0) & 0xffffu;
         if (kept_form)
             for (int turn = 0; todo && turn < 2; ++turn) {
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
                 todo &= ~with;
                 load_b(s);
 #pragma unroll
-                for (int o = 0; o < 4; ++o) {
+                for (int o = 0; o < TO; ++o) {
                     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int r = 0; r < RS; ++r) sum = times_u(bv[o][r], uh[r], ul[r], sum);
@@ -538,12 +539,12 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
         if (todo) {                             // more slots in a tile, or rows of B in no whole pieces
             const int rest = (todo >> li) & 1 ? slot : -3;
 #pragma unroll
-            for (int o = 0; o < 4; ++o)
+            for (int o = 0; o < TO; ++o)
                 v[o] = k.vec_rank ? up<T, true>(k, u, q, ord.n, rest, ob + o * 16, v[o]) : up<T, false>(k, u, q, ord.n, rest, ob + o * 16, v[o]);
         }
         if (slot > -3) {
 #pragma unroll
-            for (int o = 0; o < 4; ++o)
+            for (int o = 0; o < TO; ++o)
                 if (ob + o * 16 + 4 * kl < k.d_out) put<T>(k, y, ldy, request, ob + o * 16 + 4 * kl, slot, v[o], vec_out);
         }
     }

@@ -56,6 +56,15 @@ def test_wide(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,d_in,d_out,S,R", [(520, 72, 1904, 3, 16), (520, 200, 1912, 40, 12), (515, 1904, 136, 2, 96), (2100, 72, 2000, 7, 16),
+                                              (2065, 1000, 72, 5, 33), (4111, 40, 1040, 300, 64)])
+def test_many_requests(n, d_in, d_out, S, R, dtype):
+    """Enough requests (or columns) for the tiled product, forward or backward: summed widths that are no whole stages, columns
+    and requests that are no whole tiles, neighbours of one, two and many slots, ranks of no whole pieces."""
+    check(*make(n, d_in, d_out, S, R, dtype, seed=11))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("how", ["one slot", "none", "sorted", "last slot only", "each its own"])
 def test_slot_patterns(how, dtype):
     n, S = 200, 200
