@@ -320,3 +320,48 @@ def test_c_refusals():
     torch.cuda.synchronize()
     assert bool((loss == 7).all()) and bool((dq == 7).all())
     assert call() == 0
+
+
+def rising(M, N, d, storage, metric, seed=0):
+    """(index, X, q, ids, scores): every third query sees its logits (tau 0.1) rise by 40 from 32 rows to the next 32, eight
+    times over, then again from the start; the others lie across that direction, and one is zero."""
+    g = torch.Generator(device="cuda").manual_seed(seed + M + d)
+    u = torch.nn.functional.normalize(torch.randn(d, generator=g, device="cuda"), dim=0)
+
+    def across(n):
+        r = torch.randn(n, d, generator=g, device="cuda")
+        r -= (r @ u)[:, None] * u
+        return r / r.norm(dim=1, keepdim=True)
+
+    k = (torch.arange(N, device="cuda") // 32 % 8).float()
+    far = (4.0 * 7) ** 0.5
+    a = far - (4.0 * (7 - k)) ** 0.5 if metric == 1 else 4.0 * k
+    X = (across(N) + a[:, None] * u).to(TYPE[storage])
+    q = across(M)
+    q[::3] = (far if metric == 1 else 1.0) * u + 0.05 * across(len(q[::3]))
+    if M > 1:
+        q[1] = 0
+    q = q.to(TYPE[storage])
+    ids = torch.randint(0, N, (M, 3), generator=g, device="cuda")
+    scores = torch.randn(M, 3, generator=g, device="cuda")
+    index = faiss.IndexFlat(d, metric, storage=storage)
+    index.add(X)
+    return index, X, q, ids, scores
+
+
+@pytest.mark.parametrize("M,N,d", [(1, 70001, 64), (3, 70001, 64), (12, 70001, 64), (12, 20001, 700), (30, 40001, 100), (64, 40001, 40),
+                                   (300, 70001, 32), (33000, 20001, 32), (20000, 33001, 72)])
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("metric", [0, 1])
+def test_rising_logits_and_long_shares(M, N, d, storage, metric):
+    """The reference of a query's weights moves within a share (its logits rise by far more than its slack) while other
+    queries' stay; the largest batches leave one or two shares of more than a hundred tiles."""
+    index, X, q, ids, scores = rising(M, N, d, storage, metric)
+    loss, dq = index.distill(q, ids, scores, 0.1, 1.0, "index")
+    some = torch.unique(torch.tensor([0, 1, 2, 3, 15, 16, 17, 47, M // 2, M - 2, M - 1]).clamp(0, M - 1)).cuda()
+    ref_loss, ref_dq, e_loss, e_dq = distill_ref(q[some], X, ids[some], scores[some], 0.1, 1.0, metric, "index")
+    assert_within(loss[some], ref_loss, e_loss, "loss")
+    assert_within(dq[some], ref_dq, e_dq, "dq")
+    assert torch.isfinite(loss).all() and torch.isfinite(dq).all()
+    alone, _ = index.distill(q, ids, scores, 0.1, 1.0, "index", grad=False)
+    assert_within(alone[some], ref_loss, e_loss, "loss alone")
