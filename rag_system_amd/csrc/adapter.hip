@@ -489,6 +489,8 @@ int launch_down(const Plan& p, const Down& d, const Order& o, unsigned kinds, hi
     return RAG_OK;
 }
 
+constexpr long long MAX_THREADS = 1ll << 31;      // of a launch (the runtime refuses 2^32)
+
 // Positions of a workgroup of the tiled product, or 0: too few of them to fill the card, the direct one takes it.
 int tiled_positions(const Bank& k, const Order& o, long long ldx, size_t esz) {
     if ((unsigned long long)o.n * ldx * esz >= (1ull << 32)) return 0;      // (rows are found by 32-bit offsets)
@@ -510,11 +512,16 @@ int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
-    auto grid = [&](int ot, int tt) { return (unsigned)((k.d_out + 16 * ot - 1) / (16 * ot) * ((o.n + 16 * tt - 1) / (16 * tt))); };
-    if (grid(2, 4) >= 1024) up_direct_kernel<T, 2, 4, 4, VEC><<<grid(2, 4), 256, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
-    else if (grid(1, 4) >= 512) up_direct_kernel<T, 1, 4, 8, VEC><<<grid(1, 4), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
-    else if (grid(1, 2) >= 512) up_direct_kernel<T, 1, 2, 8, VEC><<<grid(1, 2), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
-    else up_direct_kernel<T, 1, 1, 8, VEC><<<grid(1, 1), 512, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out);
+    auto grid = [&](int ot, int tt) { return (k.d_out + 16 * ot - 1) / (16 * ot) * ((o.n + 16 * tt - 1) / (16 * tt)); };
+    auto launch = [&](auto fn, int ot, int tt, int threads) {
+        const long long groups = grid(ot, tt), most = MAX_THREADS / threads;
+        for (long long first = 0; first < groups; first += most)
+            fn<<<(unsigned)std::min(most, groups - first), threads, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out, (int)first);
+    };
+    if (grid(2, 4) >= 1024) launch(up_direct_kernel<T, 2, 4, 4, VEC>, 2, 4, 256);
+    else if (grid(1, 4) >= 512) launch(up_direct_kernel<T, 1, 4, 8, VEC>, 1, 4, 512);
+    else if (grid(1, 2) >= 512) launch(up_direct_kernel<T, 1, 2, 8, VEC>, 1, 2, 512);
+    else launch(up_direct_kernel<T, 1, 1, 8, VEC>, 1, 1, 512);
     RAG_HIP(hipGetLastError());
     return RAG_OK;
 }
@@ -578,9 +585,11 @@ int run_grad(const Call& c, const Plan& p) {
         rc = vec ? launch_down<T, true>(p, d, o, 2, c.st) : launch_down<T, false>(p, d, o, 2, c.st);
         if (rc) return rc;
     }
-    const bool together = c.n > 0 && c.dx && !(vec && tiled_positions(back, o, c.lddy, sizeof(T)) > 0);
+    const long long ups = (long long)((c.d_in + 15) / 16) * ((c.n + 31) / 32);
+    const bool together = c.n > 0 && c.dx && !(vec && tiled_positions(back, o, c.lddy, sizeof(T)) > 0) && ups * 512 <= MAX_THREADS;
     if (c.n > 0 && c.dx && !together) {
-        rc = launch_up<T, true>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, c.st);
+        rc = vec ? launch_up<T, true>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, c.st)
+                 : launch_up<T, false>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, c.st);
         if (rc) return rc;
     }
     auto launch = [&](auto rt) {
@@ -590,10 +599,10 @@ int run_grad(const Call& c, const Plan& p) {
             slot_grad_kernel<T, RT><<<dim3((unsigned)p.max_items, (unsigned)units), 256, 0, c.st>>>(g);
             return;
         }
-        const unsigned ups = (unsigned)((c.d_in + 15) / 16 * ((c.n + 31) / 32)), groups = (unsigned)((units + 1) / 2);
+        const unsigned groups = (unsigned)((units + 1) / 2);
         const bool vec_out = c.lddx % 4 == 0 && ((uintptr_t)c.dx & 15) == 0;
         auto fn = vec ? up_and_slot_kernel<T, RT, true> : up_and_slot_kernel<T, RT, false>;
-        fn<<<ups + (unsigned)p.max_items * groups, 512, 0, c.st>>>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, vec_out, ups, g, groups);
+        fn<<<(unsigned)ups + (unsigned)p.max_items * groups, 512, 0, c.st>>>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, vec_out, (unsigned)ups, g, groups);
     };
     if (c.rank <= 16) launch(std::integral_constant<int, 1>());
     else if (c.rank <= 32) launch(std::integral_constant<int, 2>());

@@ -360,8 +360,8 @@ __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const
 
 template <typename T, int OT, int TT, int WAVES, bool VEC>
 __global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y,
-                                                               long long ldy, bool vec_out) {
-    up_direct<T, OT, TT, WAVES, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, blockIdx.x);
+                                                               long long ldy, bool vec_out, int first) {
+    up_direct<T, OT, TT, WAVES, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, first + (int)blockIdx.x);
 }
 
 // Y for many requests: a workgroup has 128 output columns x POS positions (256, or 64 where that would leave CUs idle), each of

@@ -264,3 +264,30 @@ def test_c_refusals():
     torch.cuda.synchronize()
     assert all(bool((t == 7).all()) for t in (y, dA, dB))
     assert call() == 0 and grad() == 0
+
+
+def test_more_workgroups_than_a_launch_takes():
+    """Results of 35 GB: rows of the first and the last launch, forward and dx."""
+    n = 1 << 24
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free memory")
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").bfloat16()
+
+    some = torch.tensor([0, 1, 63, 64, n // 2, 16000000, n - 65, n - 2, n - 1], device="cuda")
+    slots = (torch.arange(n, device="cuda") // 1000) % 2
+    x, dy = normal(n, 3), None
+    W, A, B = normal(1056, 3), normal(2, 2, 3), normal(2, 1056, 2)
+    bank = QueryAdapters(W, A, B)
+    y = bank.apply(x, slots)[some]
+    want, allow = adapters_ref(x[some], W, A, B, bank.scale, slots[some].tolist())
+    assert_within(y, want, allow, "y")
+    x, dy = torch.zeros(n, 144, dtype=torch.bfloat16, device="cuda"), normal(n, 5)
+    W, A, B = normal(5, 144), normal(2, 2, 144), normal(2, 5, 2)
+    bank = QueryAdapters(W, A, B)
+    dx, dA, dB = bank.grad(x, slots, dy)
+    ref = adapters_grad_ref(x[some], W, A, B, bank.scale, slots[some].tolist(), dy[some])["dx"]
+    assert_within(dx[some], *ref, "dx")
+    assert not dB.any()                 # (x is zero)
