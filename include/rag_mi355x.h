@@ -362,8 +362,8 @@ int rag_adapter_grad_dev(int dtype, int64_t n, int d_in, int d_out, int n_slots,
  * `ws_dev`: rag_flat_distill_ws_bytes bytes (it does not depend on the number of rows; 0 for the list), 256-byte
  * aligned, the caller's until the call's work on `stream` is done.  Asynchronous on `stream`; equal calls give equal
  * bits.  May be captured into a graph once no added row is staged on the host (L2: once the norms exist), that is
- * after any one call; the graph keeps the rows it was captured with (rows added later are not seen, rows replaced
- * behind rag_flat_reset are) and must not outlive the handle. */
+ * after any one call; the graph keeps the rows it was captured with (rows added later are not seen), is captured anew after
+ * rag_flat_reset (it would read the new rows, L2 with the old norms) and must not outlive the handle. */
 #define RAG_OVER_INDEX 0
 #define RAG_OVER_LIST 1
 #define RAG_DISTILL_MAX_NQ 65535

@@ -684,7 +684,7 @@ int rag_flat_distill_dev(rag_flat_t* h, int64_t nq, const void* q_dev, int64_t l
     int rc = check_shape(who, h, nq, k, over);
     if (rc) return rc;
     if (!(temperature > 0) || !(teacher_temperature > 0) || !std::isfinite(temperature) || !std::isfinite(teacher_temperature) ||
-        !std::isfinite((float)(1.0 / temperature)) || !std::isfinite((float)(1.0 / teacher_temperature)))
+        !std::isfinite((float)(2.0 / temperature)) || !std::isfinite((float)(1.0 / teacher_temperature)))   // (2: the factors below)
         return fail(RAG_ERR_INVALID_ARG, "%s: temperatures must be positive and finite (%g, %g)", who, temperature,
                     teacher_temperature);
     if (nq == 0) return RAG_OK;

@@ -859,6 +859,7 @@ struct rag_flat {
     float* xnorm = nullptr;  int64_t xnorm_cap = 0;    // ||x||^2 per row (L2, MFMA path), lazily filled
     int64_t norm_valid = 0;
     int64_t norm_done = 0;                             // ... of which the device is known to have finished (flat_rows_on_stream)
+    bool on_streams = false;                           // work of flat_rows_on_stream may be under way on callers' streams
     bool captured = false;                             // a captured graph names x / xnorm: replaced arrays go to `retired`
     std::vector<void*> retired;
     float* ws_hq = nullptr;  int64_t ws_hq_cap = 0;    // host-variant device copies
@@ -1734,6 +1735,7 @@ int flat_rows_on_stream(rag_flat_t* h, bool want_norms, hipStream_t st, const ch
     }
     const FlatRows v{h->x, want_norms ? h->xnorm : nullptr, h->ld, h->d, h->dtype == RAG_DTYPE_BF16 ? 1 : 0, h->metric,
                      h->ndev};
+    h->on_streams = true;
     return use(v, ctx);
 }
 
@@ -1942,6 +1944,10 @@ int rag_flat_reset(rag_flat_t* h) {
     RAG_REQUIRE_INIT();
     if (!h) return fail(RAG_ERR_INVALID_ARG, "bad handle");
     std::lock_guard<std::mutex> lk(h->mu);
+    if (h->on_streams) {  // rows added next take the place of those that such work still reads
+        RAG_HIP(hipDeviceSynchronize());
+        h->on_streams = h->captured;  // (a graph may be replayed at any time)
+    }
     h->staged.clear();
     h->ntotal = 0;
     h->ndev = 0;

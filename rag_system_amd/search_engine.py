@@ -606,6 +606,8 @@ class SearchEngine:
         n = len(queries)
         if n == 0 or index.ntotal == 0:
             raise ValueError("distill_step needs queries and a filled index")
+        if int(top_k) < 1:
+            raise ValueError("distill_step needs top_k of 1 or more, got %r" % (top_k,))
         if adapters is not None and len(adapters) != n:
             raise ValueError("%d adapters for %d queries" % (len(adapters), n))
         from . import device_tensors as dt

@@ -194,3 +194,11 @@ def test_distill_step(over):
     want_loss, dy = vs.index.distill(y, torch.from_numpy(ids).cuda(), z, 0.2, 1.0, over, weights=torch.full((4,), 0.25, device="cuda"))
     _, wA, wB = bank.grad(x, slots, dy, input_grad=False)
     assert torch.equal(loss, want_loss) and torch.equal(dA, wA) and torch.equal(dB, wB)
+
+
+def test_distill_step_refuses_an_empty_list():
+    em, vs = _store(8)
+    se = SearchEngine(vs, em, cross_encoder=_CrossEncoder(), query_adapters=_bank(2, 2, DIM, DIM))
+    for k in (0, -1):
+        with pytest.raises(ValueError, match="top_k"):
+            se.distill_step(QUERIES, top_k=k)

@@ -365,3 +365,30 @@ def test_rising_logits_and_long_shares(M, N, d, storage, metric):
     assert torch.isfinite(loss).all() and torch.isfinite(dq).all()
     alone, _ = index.distill(q, ids, scores, 0.1, 1.0, "index", grad=False)
     assert_within(alone[some], ref_loss, e_loss, "loss alone")
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_rows_replaced_while_a_call_is_under_way(storage):
+    """reset() and add() behind a call that is still running: it has read the rows that were there."""
+    index, X, q, ids, scores = make(512, 400000, 64, 5, storage, 1, seed=21)
+    other = X[:300000].flip(0).float().cpu().numpy()
+    want = index.distill(q, ids, scores)
+    torch.cuda.synchronize()
+    ids2 = ids.clamp(max=299999)
+    got = index.distill(q, ids, scores)
+    index.reset()
+    index.add(other)
+    new = index.distill(q, ids2, scores)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    fresh = faiss.IndexFlat(64, 1, storage=storage)
+    fresh.add(other)
+    again = fresh.distill(q, ids2, scores)
+    assert torch.equal(new[0], again[0]) and torch.equal(new[1], again[1])
+
+
+@pytest.mark.parametrize("storage,d", [("f32", 40), ("f32", 1024), ("bf16", 770), ("f32", 8192)])
+@pytest.mark.parametrize("M", [1, 6, 70])
+def test_longest_lists(M, d, storage):
+    index, X, q, ids, scores = make(M, 900, d, 1024, storage, 0, seed=22)
+    for over in ("list", "index"):
+        check(index, X, q, ids, scores, over, 0)
