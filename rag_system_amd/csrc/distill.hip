@@ -478,15 +478,18 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_kernel(Call c) {
                 if (col + e < c.d) store1(dq + col + e, live);
         return;
     }
-    // the shares' references and sums, by each wave for itself
+    // the shares' references and sums
     float m = -INFINITY, l = 0.f;
-    for (int s = lane; s < c.splits; s += 64) m = fmaxf(m, c.part_ml[2 * (s * c.m + i)]);
-    m = wave_max(m);
-    for (int s = lane; s < c.splits; s += 64) {
-        const float ms = c.part_ml[2 * (s * c.m + i)], ls = c.part_ml[2 * (s * c.m + i) + 1];
-        l += (ms == -INFINITY ? 0.f : expf((ms - m) * c.beta)) * ls;
+#pragma unroll 2
+    for (int s = tid; s < c.splits; s += JOIN_THREADS) {
+        const float ms = c.part_ml[2 * (s * c.m + i)], ls = c.part_ml[2 * (s * c.m + i) + 1], top = fmaxf(m, ms);
+        if (top != -INFINITY) l = l * expf((m - top) * c.beta) + ls * expf((ms - top) * c.beta);
+        else l += ls;                     // (nothing, or NaN)
+        m = top;
     }
-    l = wave_sum(l);
+    const float mine = m;
+    m = block_max<JOIN_WAVES>(m, red);
+    l = block_sum<JOIN_WAVES>(mine == -INFINITY ? l : l * expf((mine - m) * c.beta), red);
     if (loss) {
         float* s_of = sh;                 // k
         float* qs = s_of + c.k;           // ld
@@ -557,7 +560,7 @@ Plan make_plan(long long m, int d, int bf16, int over, bool grad) {
     Plan p{};
     if (over == RAG_OVER_LIST || m == 0) return p;
     const size_t ld = elem_ld(d, bf16);
-    if (distill::tile_plan(m, (int)ld, bf16 != 0, &p.tile)) p.splits = p.tile.splits;
+    if (distill::tile_plan(m, (int)ld, bf16 != 0, grad, &p.tile)) p.splits = p.tile.splits;
     else p.splits = (int)std::max<long long>(1, std::min<long long>(1024, 2048 / m));
     auto take = [&](size_t floats) {
         const size_t at = p.bytes;

@@ -53,7 +53,7 @@ struct TilePlan {
     int rows;        // rows per tile
     int splits, q_tiles;
 };
-bool tile_plan(long long m, int ld, bool bf16, TilePlan* p);
+bool tile_plan(long long m, int ld, bool bf16, bool grad, TilePlan* p);
 int tile_launch(const TilePlan& p, const TileCall& c, bool grad, hipStream_t st);
 
 // 16 bytes a lane from `off` bytes behind `base` (uniform) into LDS, lane after lane from `l` (uniform) on.  The buffer form: behind

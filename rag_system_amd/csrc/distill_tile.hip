@@ -39,29 +39,31 @@ const Few FEW[] = {
 };
 constexpr int N_FEW = sizeof FEW / sizeof FEW[0];
 
-}  // namespace
-
-namespace {
+const Variants& variants(bool bf16, bool grad) { return (bf16 ? VARIANTS_BF16 : VARIANTS_F32)[grad]; }
 
 // Workgroups of a variant that a CU holds (its LDS and registers; asked of the runtime once per variant).
-int resident(bool bf16, int v, const Variant& a) {
-    static std::atomic<int> known[2][64];
-    int n = known[bf16][v];
+int resident(bool bf16, bool grad, int v) {
+    static std::atomic<int> known[2][2][64];
+    int n = known[bf16][grad][v];
     if (n == 0) {
-        const void* fn = reinterpret_cast<const void*>(a.fn[1][1]);
+        const Variant& a = variants(bf16, grad).all[v];
+        const void* fn = reinterpret_cast<const void*>(a.fn[1]);
         if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, a.lds) != hipSuccess ||
             hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, 64 * a.wq * a.wd, a.lds) != hipSuccess || n < 1) {
             (void)hipGetLastError();
             n = 1;
         }
-        known[bf16][v] = n;
+        known[bf16][grad][v] = n;
     }
     return n;
 }
 
+// TFLOP/s that a group of 16, 32, 64, 128 queries reaches (1M rows of 384, float32 and bfloat16, the loss alone and with its gradient).
+constexpr double RATE[2][2][4] = {{{48, 71, 118, 131}, {80, 113, 129, 143}}, {{91, 170, 430, 640}, {171, 306, 600, 840}}};
+
 }  // namespace
 
-bool tile_plan(long long m, int ld, bool bf16, TilePlan* p) {
+bool tile_plan(long long m, int ld, bool bf16, bool grad, TilePlan* p) {
     *p = TilePlan{-1, false, bf16, 0, 0, 0};
     if (m <= 4)
         for (int v = 0; v < N_FEW; ++v)
@@ -69,16 +71,14 @@ bool tile_plan(long long m, int ld, bool bf16, TilePlan* p) {
                 *p = TilePlan{v, true, bf16, 64 / FEW[v].lpr * ROWS_WAVES, num_cus() * 2, 1};
                 return true;
             }
-    // The variant with the least work for these queries: whole groups of them, whole columns, over the rate its groups reach
-    // (float32 rows of 384, 1M: 16 queries a group 80, 32: 113, 64: 129, 128: 143 TFLOP/s).
-    const Variant* const all = bf16 ? VARIANTS_BF16 : VARIANTS_F32;
-    const int n_all = bf16 ? N_VARIANTS_BF16 : N_VARIANTS_F32;
+    // The variant with the least work for these queries: whole groups of them, whole columns, over the rate its groups reach.
+    const Variants& of = variants(bf16, grad);
     double least = 0;
     int best = -1;
-    for (int v = 0; v < n_all; ++v) {
-        const Variant& a = all[v];
+    for (int v = 0; v < of.n; ++v) {
+        const Variant& a = of.all[v];
         if (a.cw * a.wd < ld) continue;
-        const double rate = a.wq == 1 ? 80 : a.wq == 2 ? 113 : a.wq == 4 ? 129 : 143;
+        const double rate = RATE[bf16][grad][a.wq == 1 ? 0 : a.wq == 2 ? 1 : a.wq == 4 ? 2 : 3];
         const double cost = (double)((m + 16 * a.wq - 1) / (16 * a.wq)) * a.wq * a.cw * a.wd / rate;
         if (best < 0 || cost < least) {
             best = v;
@@ -86,13 +86,13 @@ bool tile_plan(long long m, int ld, bool bf16, TilePlan* p) {
         }
     }
     if (best < 0) return false;
-    const Variant& a = all[best];
+    const Variant& a = of.all[best];
     p->kind = best;
     p->rows = a.rt;
     p->q_tiles = (int)((m + 16 * a.wq - 1) / (16 * a.wq));
     // as many shares as leave the fewest places for a workgroup idle in the last round; more shares cost their row
     // sums (written once, read once by the join), so the fewest of equals
-    const int places = num_cus() * resident(bf16, best, a);
+    const int places = num_cus() * resident(bf16, grad, best);
     double best_time = 0;
     for (int s = 1; s <= places; ++s) {
         const long long groups = (long long)s * p->q_tiles, rounds = (groups + places - 1) / places;
@@ -113,8 +113,8 @@ int tile_launch(const TilePlan& p, const TileCall& c, bool grad, hipStream_t st)
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
-    const Variant& a = p.bf16 ? VARIANTS_BF16[p.kind] : VARIANTS_F32[p.kind];
-    kernel_t fn = a.fn[grad ? 1 : 0][c.norms ? 1 : 0];
+    const Variant& a = variants(p.bf16, grad).all[p.kind];
+    const kernel_t fn = a.fn[c.norms ? 1 : 0];
     if (a.lds > 48 * 1024)
         RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, a.lds));
     const unsigned groups = (unsigned)((c.splits + 7) / 8 * 8) * (unsigned)c.q_tiles;

@@ -10,12 +10,13 @@ namespace distill {
 typedef void (*kernel_t)(TileCall);
 struct Variant {
     int wq, wd, cw, rt, lds;
-    kernel_t fn[2][2];   // [grad][l2]
+    kernel_t fn[2];   // [l2]
 };
-extern const Variant* const VARIANTS_F32;
-extern const int N_VARIANTS_F32;
-extern const Variant* const VARIANTS_BF16;
-extern const int N_VARIANTS_BF16;
+struct Variants {
+    const Variant* all;
+    int n;
+};
+extern const Variants VARIANTS_F32[2], VARIANTS_BF16[2];   // [grad]
 
 constexpr int LDS_MAX = 160 * 1024;
 constexpr int exch_bytes(int wq, int wd, int rt) { return wd > 1 ? wq * wd * (rt / 16) * 1024 : 0; }
@@ -24,14 +25,17 @@ constexpr int ring(int wq, int wd, int cw, int rt, int esz) {
     return std::min(3, (LDS_MAX - exch_bytes(wq, wd, rt)) / (rt * cw * wd * esz));
 }
 
-template <typename T, int WQ, int WD, int CW, int RT>
+template <typename T, bool GRAD, int WQ, int WD, int CW, int RT>
 Variant variant() {
     constexpr int E = sizeof(T), NB = ring(WQ, WD, CW, RT, E);
     static_assert(NB >= 1, "tile does not fit");
     return Variant{WQ, WD, CW, RT, NB * RT * CW * WD * E + exch_bytes(WQ, WD, RT),
-                   {{tile_kernel<T, WQ, WD, CW, RT, NB, false, false>, tile_kernel<T, WQ, WD, CW, RT, NB, false, true>},
-                    {tile_kernel<T, WQ, WD, CW, RT, NB, true, false>, tile_kernel<T, WQ, WD, CW, RT, NB, true, true>}}};
+                   {tile_kernel<T, WQ, WD, CW, RT, NB, GRAD, false>, tile_kernel<T, WQ, WD, CW, RT, NB, GRAD, true>}};
 }
+template <typename T, int WQ, int WD, int CW, int RT>
+Variant grad() { return variant<T, true, WQ, WD, CW, RT>(); }
+template <typename T, int WQ, int WD, int CW, int RT>
+Variant loss() { return variant<T, false, WQ, WD, CW, RT>(); }
 
 }  // namespace distill
 }  // namespace rag
