@@ -249,7 +249,7 @@ __global__ __launch_bounds__(1024) void prepare_kernel(Sort s, Turn j) {
 // dA_s = sum_t v_t x_t^T and dB_s = sum_t dy_t u_t^T over the requests of an item.  MFMA 16x16x4 in float32 (u and v are float32,
 // and the sums are small beside W's products): the A operand is u or v (16 of the rank x 4 requests), the B operand x or dy.
 // A lane loads 16 bytes of a request's row, E columns, and gives one of them to each of E products: product e has the columns
-// li * E + e.  Nothing is staged; a wave has 16 E columns and up to 64 of the rank.
+// li * E + e (the last lane's: the row's last E columns).  Nothing is staged; a wave has 16 E columns and up to 64 of the rank.
 struct SlotGrad {
     Sort s;
     const float *u, *v;
@@ -271,7 +271,7 @@ __device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit,
     const Item it = live ? g.s.items[item] : Item{0, 0, 0, -1};
     const bool is_b = unit >= cols_a * rcs;
     if (is_b) unit -= cols_a * rcs;
-    const int r0 = unit % rcs * RT * 16, c0 = unit / rcs * 16 * E + li * E, d = is_b ? g.d_out : g.d_in;
+    const int r0 = unit % rcs * RT * 16, c0 = unit / rcs * 16 * E + li * E, d = is_b ? g.d_out : g.d_in, begin = begin_of<E>(c0, d);
     const T* src = static_cast<const T*>(is_b ? g.dy : g.x);
     const long long ld = is_b ? g.lddy : g.ldx;
     const float* cf = (is_b ? g.u : g.v) + r0;
@@ -291,7 +291,7 @@ __device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit,
             for (int j = 0; j < LOT; ++j) {
                 const int t = t0 + (s0 + j) * 4 + kl;
                 const T* row = src + (long long)__shfl(mine, min((s0 + j) * 4 + kl, 63)) * ld;
-                xv[j] = vec ? piece<true>(row, c0, d) : piece<false>(row, c0, d);
+                xv[j] = vec ? whole_piece<true>(row, begin, d) : whole_piece<false>(row, begin, d);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) a[j][r] = cf[(long long)min(t, it.end - 1) * g.rp + min(r * 16 + li, g.rp - 1 - r0)];
             }
@@ -326,8 +326,8 @@ __device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit,
             f32x4 sum = *reinterpret_cast<const f32x4*>(&part[0][team][lane * 4]);
 #pragma unroll
             for (int w = 1; w < 4; ++w) sum += *reinterpret_cast<const f32x4*>(&part[w][team][lane * 4]);
-            const int rr = r0 + r * 16 + 4 * kl, cc = c0 + e0 + team;
-            if (live && cc < d)
+            const int rr = r0 + r * 16 + 4 * kl, cc = begin + e0 + team;
+            if (live && cc >= c0 && cc < d)       // (columns before c0 are another lane's)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (rr + i < g.rank) to[is_b ? (long long)cc * g.rank + rr + i : (long long)(rr + i) * g.d_in + cc] = sum[i];

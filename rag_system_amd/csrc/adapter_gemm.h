@@ -66,26 +66,53 @@ template <> struct Mma<u16> {
     }
 };
 
-// The piece of `row` at `col`: zeros from `end` on.  VEC: rows and pieces are 16-byte aligned and end with a piece.
+// Where the piece of a row of `end` values at `col` begins.  Rows of any length and alignment are read 16 bytes at a time too (the
+// hardware takes any address): the piece that would pass the end is the row's LAST one, without the values before `col`.
+template <int E>
+__device__ __forceinline__ int begin_of(int col, int end) { return end < E ? col : min(col, end - E); }
+// E values of `row` from there on (behind the end: the last one again).
+template <bool VEC, typename T>
+__device__ __forceinline__ u32x4 whole_piece(const T* row, int begin, int end) {
+    constexpr int E = Mma<T>::E;
+    if (VEC) return *reinterpret_cast<const u32x4*>(row + begin);
+    u32x4 r;
+    if (end >= E) {                     // (uniform)
+        __builtin_memcpy(&r, row + begin, 16);
+    } else {
+        T v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = row[min(begin + e, end - 1)];
+        __builtin_memcpy(&r, v, 16);
+    }
+    return r;
+}
+// That piece of `row`; zeros in the place of values before `col` and behind the end.  Two rows' pieces at the same place hold
+// matching values, which is all that a sum over them needs.  VEC: rows are 16-byte aligned and end with a piece.
 template <bool VEC, typename T>
 __device__ __forceinline__ u32x4 piece(const T* row, int col, int end) {
     constexpr int E = Mma<T>::E;
     if (VEC) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(row + min(col, end - E));
+        const u32x4 v = whole_piece<true>(row, min(col, end - E), end);
         const unsigned keep = col < end ? ~0u : 0u;
         return u32x4{v[0] & keep, v[1] & keep, v[2] & keep, v[3] & keep};
     }
-    T v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = row[min(col + e, end - 1)];
-    u32x4 r;
-    __builtin_memcpy(&r, v, 16);
+    const int begin = begin_of<E>(col, end), skip = col - begin, stop = end - begin;
+    u32x4 r = whole_piece<false>(row, begin, end);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        if (E == 8) r[e] &= (col + 2 * e < end ? 0xffffu : 0u) | (col + 2 * e + 1 < end ? 0xffff0000u : 0u);
-        else r[e] &= col + e < end ? ~0u : 0u;
+        if (E == 8) r[e] &= (2 * e >= skip && 2 * e < stop ? 0xffffu : 0u) | (2 * e + 1 >= skip && 2 * e + 1 < stop ? 0xffff0000u : 0u);
+        else r[e] &= e >= skip && e < stop ? ~0u : 0u;
     }
     return r;
+}
+// U's values that go with piece<VEC, T>(b, col, rank), E of them.  (Behind the rank U holds zeros.)
+template <bool VEC, int E>
+__device__ __forceinline__ void piece_of_u(const float* u, int col, int rank, float* v) {
+    const int begin = VEC ? col : begin_of<E>(col, rank), skip = col - begin;
+    __builtin_memcpy(v, VEC ? static_cast<const float*>(__builtin_assume_aligned(u + begin, 16)) : u + begin, E * 4);
+    if (!VEC)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = e >= skip ? v[e] : 0.f;
 }
 
 // Element e of a piece, as a float.
@@ -220,9 +247,10 @@ __global__ __launch_bounds__(256) void down_each_kernel(Down d, Order ord) {
 }
 
 // += B_s U^T for a tile of 16 output columns (from o0) and the 16 positions from p: the first two slots by matrix products, slot
-// by slot; where there are more, each lane takes its own position's.
+// by slot; where there are more, each lane takes its own position's.  share of shares: every shares-th step of the rank.
 template <typename T, bool VEC>
-__device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, long long n, int my_slot, int o0, f32x4 acc) {
+__device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, long long n, int my_slot, int o0, f32x4 acc, int share = 0,
+                                    int shares = 1) {
     typedef Mma<T> M;
     constexpr int E = M::E;
     const int lane = threadIdx.x & 63, li = lane & 15, kl = lane >> 4;
@@ -232,13 +260,9 @@ __device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, 
         if (turn == 2) {
             if ((todo >> li) & 1) {
                 const T* b = static_cast<const T*>(k.b) + (long long)my_slot * k.d_out * k.rank;
-                for (int r = 0; r < k.rank; r += E) {
+                for (int r = share * E; r < k.rank; r += shares * E) {
                     float v[E];
-#pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        const f32x4 t = *reinterpret_cast<const f32x4*>(ur + r + e);
-                        v[e] = t[0], v[e + 1] = t[1], v[e + 2] = t[2], v[e + 3] = t[3];
-                    }
+                    piece_of_u<VEC, E>(ur, r, k.rank, v);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const u32x4 bv = piece<VEC>(b + (long long)min(o0 + 4 * kl + i, k.d_out - 1) * k.rank, r, k.rank);
@@ -255,17 +279,20 @@ __device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, 
         const T* b = static_cast<const T*>(k.b) + ((long long)s * k.d_out + min(o0 + li, k.d_out - 1)) * k.rank;
         // (others' lanes keep what they have: a zero times this slot's infinity would not be one)
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < k.rank; r += 4 * E) {
+        for (int r = share * 4 * E; r < k.rank; r += shares * 4 * E) {
             const u32x4 bv = piece<VEC>(b, r + kl * E, k.rank);
+            float v[E];
+            piece_of_u<VEC, E>(ur, r + kl * E, k.rank, v);
             if constexpr (E == 4) {
-                sum = M::mma(bv, *reinterpret_cast<const u32x4*>(ur + r + kl * 4), sum);
+                u32x4 uv;
+                __builtin_memcpy(&uv, v, 16);
+                sum = M::mma(bv, uv, sum);
             } else {
-                const f32x4 v[2] = {*reinterpret_cast<const f32x4*>(ur + r + kl * 8), *reinterpret_cast<const f32x4*>(ur + r + kl * 8 + 4)};
                 bf16x8 hi, lo;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    hi[e] = (__bf16)v[e >> 2][e & 3];
-                    lo[e] = (__bf16)(v[e >> 2][e & 3] - (float)hi[e]);
+                    hi[e] = (__bf16)v[e];
+                    lo[e] = (__bf16)(v[e] - (float)hi[e]);
                 }
                 sum = M::mma(bv, __builtin_bit_cast(u32x4, lo), sum);
                 sum = M::mma(bv, __builtin_bit_cast(u32x4, hi), sum);
@@ -344,16 +371,24 @@ __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const
     for (int o = 0; o < OT; ++o)
 #pragma unroll
         for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4*>(&part[wave][o * TT + t][lane * 4]) = acc[o][t];
+    // the adapters' side: the waves of a tile share the steps of the rank
+    constexpr int TILES = OT * TT, SHARES = WAVES > TILES ? WAVES / TILES : 1;
+    static_assert(WAVES % TILES == 0 || TILES % WAVES == 0, "waves of a tile");
+    for (int j = wave % TILES; j < TILES; j += WAVES) {
+        const long long p = p0 + j % TT * 16, pos = p + li;
+        const int slot = pos < ord.n ? ord.slot(pos) : -3, o = o0 + j / TT * 16;
+        f32x4* mine = reinterpret_cast<f32x4*>(&part[wave][j][lane * 4]);
+        if (k.vec_rank) *mine = up<T, true>(k, u, p, ord.n, slot, o, *mine, wave / TILES, SHARES);
+        else *mine = up<T, false>(k, u, p, ord.n, slot, o, *mine, wave / TILES, SHARES);
+    }
     __syncthreads();
-    for (int j = wave; j < OT * TT; j += WAVES) {
+    for (int j = wave; j < TILES; j += WAVES) {
         f32x4 sum = *reinterpret_cast<const f32x4*>(&part[0][j][lane * 4]);
 #pragma unroll
         for (int v = 1; v < WAVES; ++v) sum += *reinterpret_cast<const f32x4*>(&part[v][j][lane * 4]);
         const int o = o0 + j / TT * 16;
-        const long long p = p0 + j % TT * 16, pos = p + li;
+        const long long pos = p0 + j % TT * 16 + li;
         const int slot = pos < ord.n ? ord.slot(pos) : -3;
-        if (k.vec_rank) sum = up<T, true>(k, u, p, ord.n, slot, o, sum);
-        else sum = up<T, false>(k, u, p, ord.n, slot, o, sum);
         if (pos < ord.n && o + 4 * kl < k.d_out) put<T>(k, y, ldy, ord.request(pos), o + 4 * kl, slot, sum, vec_out);
     }
 }
