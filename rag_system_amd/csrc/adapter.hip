@@ -28,7 +28,7 @@ struct Item {
 struct Sort {
     const long long* slots;
     int n, n_slots, bits, chunk, chunks, len;
-    int *perm, *slot_at, *counts, *start;   // counts: chunks x (slots + 2); start: slots + 3
+    int *perm, *slot_at, *counts;           // counts: chunks x (slots + 2)
     int2* parts;                            // per slot: first partial, number of partials (0: none)
     int* n_items;
     Item* items;
@@ -82,8 +82,8 @@ __device__ __forceinline__ void place_chunk(const Sort& s, int c, int* next) {
         }
     });
 }
-// From the bins' totals (in LDS, destroyed): start[], and with items the list of items.  One workgroup of 1024.
-__device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int* tmp) {
+// From the bins' totals (in LDS) where each bin starts (there), and, if it shall write, the list of items.  A workgroup of 1024.
+__device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int* tmp, bool write) {
     const int bins = s.n_slots + 2, per = (bins + 1023) / 1024, b0 = threadIdx.x * per;
     // three sums over the bins at a time: requests, items, partials
     int sum[3] = {0, 0, 0};
@@ -111,15 +111,11 @@ __device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int
             for (int a = 0; a < 3; ++a) upto[a] += tmp[a * 16 + w];
     }
     int at = upto[0] - sum[0], item = upto[1] - sum[1], part = upto[2] - sum[2];
-    if (threadIdx.x == 0) {
-        s.start[bins] = s.n;
-        if (s.items) *s.n_items = all_items;
-    }
+    if (threadIdx.x == 0 && write && s.items) *s.n_items = all_items;
     for (int b = b0; b < min(bins, b0 + per); ++b) {
         const int total = totals[b], it = items_of(b);
-        s.start[b] = at;
         totals[b] = at;
-        if (it > 0) {
+        if (it > 0 && write) {
             s.parts[b] = int2{part, it > 1 ? it : 0};
             for (int j = 0; j < it; ++j)
                 s.items[item + j] = Item{b, at + j * s.len, min(at + total, at + (j + 1) * s.len), it > 1 ? part + j : -1};
@@ -131,54 +127,59 @@ __device__ __forceinline__ void starts_and_items(const Sort& s, int* totals, int
     __syncthreads();
 }
 
-__global__ __launch_bounds__(64) void count_kernel(Sort s) {
-    extern __shared__ int lds[];
+// The place of every wave's first request of every bin, from the counts of all chunks: this workgroup's `waves` chunks from c0 on
+// (next: waves x bins).  Every workgroup adds up the counts for itself, which is less than a launch to do it once.  tmp: 2048.
+__device__ __forceinline__ void places(const Sort& s, int c0, int waves, int* next, int* totals, int* tmp) {
     const int bins = s.n_slots + 2;
-    for (int b = threadIdx.x; b < bins; b += 64) lds[b] = 0;
-    __syncthreads();
-    count_chunk(s, blockIdx.x, lds);
-    __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 64) s.counts[(long long)blockIdx.x * bins + b] = lds[b];
-}
-__global__ __launch_bounds__(1024) void scan_kernel(Sort s) {
-    extern __shared__ int lds[];
-    const int bins = s.n_slots + 2;
-    int* totals = lds;
-    int* tmp = totals + bins;
     // several threads a bin where there are few, each for a run of the chunks
-    const int teams = bins <= 512 ? 1024 / (bins <= 128 ? 128 : bins <= 256 ? 256 : 512) : 1, width = 1024 / teams;
-    const int team = threadIdx.x / width, run = (s.chunks + teams - 1) / teams, c0 = team * run, c1 = min(s.chunks, c0 + run);
+    const int width = min(1024, (bins + 63) / 64 * 64), teams = 1024 / width;
+    const int team = threadIdx.x / width, run = (s.chunks + teams - 1) / teams, from = team * run, to = team < teams ? min(s.chunks, from + run) : 0;
     for (int b0 = 0; b0 < bins; b0 += width) {
         const int b = b0 + threadIdx.x % width;
-        int sum = 0;
+        int all = 0, before = 0;
         if (b < bins)
-#pragma unroll 16
-            for (int c = c0; c < c1; ++c) sum += s.counts[(long long)c * bins + b];
-        tmp[threadIdx.x] = sum;
+            for (int c = from; c < to; c += 16) {           // (sixteen on their way at once)
+                int v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = s.counts[min(c + j, to - 1) * bins + b];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    all += c + j < to ? v[j] : 0;
+                    before += c + j < min(to, c0) ? v[j] : 0;
+                }
+            }
+        tmp[threadIdx.x] = all;
+        tmp[1024 + threadIdx.x] = before;
         __syncthreads();
-        if (b < bins) {
-            int before = 0;
-            for (int t = 0; t < team; ++t) before += tmp[t * width + threadIdx.x % width];
-            if (team == teams - 1) totals[b] = before + sum;
-#pragma unroll 16
-            for (int c = c0; c < c1; ++c) {
-                int* at = s.counts + (long long)c * bins + b;
-                const int v = *at;
-                *at = before;
-                before += v;
+        if (b < bins && team == 0) {
+            for (int t = 1; t < teams; ++t) {
+                all += tmp[t * width + threadIdx.x];
+                before += tmp[1024 + t * width + threadIdx.x];
+            }
+            totals[b] = all;
+            for (int w0 = 0; w0 < waves; w0 += 4) {
+                int v[4];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) v[w] = s.counts[min(c0 + w0 + w, s.chunks - 1) * bins + b];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    next[(w0 + w) * bins + b] = before;
+                    before += v[w];               // (behind the last chunk: not used)
+                }
             }
         }
         __syncthreads();
     }
+    starts_and_items(s, totals, tmp, blockIdx.x == 0);
+    for (int j = threadIdx.x; j < waves * bins; j += 1024) next[j] += totals[j % bins];
     __syncthreads();
-    starts_and_items(s, totals, tmp);
 }
-__global__ __launch_bounds__(64) void place_kernel(Sort s) {
+__global__ __launch_bounds__(1024) void place_kernel(Sort s, int waves) {
     extern __shared__ int lds[];
-    const int bins = s.n_slots + 2;
-    for (int b = threadIdx.x; b < bins; b += 64) lds[b] = s.counts[(long long)blockIdx.x * bins + b] + s.start[b];
-    __syncthreads();
-    place_chunk(s, blockIdx.x, lds);
+    const int bins = s.n_slots + 2, wave = threadIdx.x >> 6, c0 = blockIdx.x * waves;
+    int* totals = lds + waves * bins;
+    places(s, c0, waves, lds, totals, totals + bins);
+    if (wave < waves && c0 + wave < s.chunks) place_chunk(s, c0 + wave, lds + wave * bins);
 }
 
 // ---- transposes of the bank for the backward ---------------------------------------------------------------------------
@@ -186,6 +187,7 @@ struct Turn {
     const void* from[3];
     void* to[3];
     int rows[3], cols[3], count[3];   // count matrices of rows x cols, dense
+    int to_rows[3], to_cols[3];       // of the transposes: cols and rows, or more, filled up with zeros
     int first[4];                     // first workgroup of each kind
 };
 // One 64 x 64 tile by WAVES waves.
@@ -193,25 +195,56 @@ template <typename T, int WAVES>
 __device__ __forceinline__ void turn_tile(const Turn& j, int block, T (*tile)[66]) {
     int kind = 0;
     while (kind < 2 && block >= j.first[kind + 1]) ++kind;
-    const int rows = j.rows[kind], cols = j.cols[kind], tr = (rows + 63) / 64, tc = (cols + 63) / 64;
+    const int rows = j.rows[kind], cols = j.cols[kind], to_rows = j.to_rows[kind], to_cols = j.to_cols[kind];
+    const int tr = (to_cols + 63) / 64, tc = (to_rows + 63) / 64;
     const int b = block - j.first[kind], m = b / (tr * tc), r0 = b / tc % tr * 64, c0 = b % tc * 64;
     const T* from = static_cast<const T*>(j.from[kind]) + (long long)m * rows * cols;
-    T* to = static_cast<T*>(j.to[kind]) + (long long)m * rows * cols;
+    T* to = static_cast<T*>(j.to[kind]) + (long long)m * to_rows * to_cols;
     const int lane = threadIdx.x & 63;
     for (int r = threadIdx.x >> 6; r < 64; r += WAVES)
-        if (r0 + r < rows && c0 + lane < cols) tile[r][lane] = from[(long long)(r0 + r) * cols + c0 + lane];
+        tile[r][lane] = r0 + r < rows && c0 + lane < cols ? from[(long long)(r0 + r) * cols + c0 + lane] : (T)0;
     __syncthreads();
     for (int c = threadIdx.x >> 6; c < 64; c += WAVES)
-        if (c0 + c < cols && r0 + lane < rows) to[(long long)(c0 + c) * rows + r0 + lane] = tile[lane][c];
+        if (c0 + c < to_rows && r0 + lane < to_cols) to[(long long)(c0 + c) * to_cols + r0 + lane] = tile[lane][c];
 }
+
+// ---- rows in whole pieces ------------------------------------------------------------------------------------------------
+//
+// The tiled product wants rows that begin and end with a 16-byte piece.  For a batch that it serves, matrices whose rows do not are
+// copied, filled up with zeros (16001 x 767 x 765 bf16, 64 slots of rank 33: 398 us without the copies, 106 with them).
+struct Pad {
+    const void* from[4];
+    void* to[4];
+    long long ld[4];                            // between rows of `from`, whose matrices follow each other
+    int rows[4], cols[4], to_rows[4], to_cols[4];
+    unsigned first[5];                          // first piece of each kind
+};
 template <typename T>
-__global__ __launch_bounds__(256) void turn_kernel(Turn j) {
-    __shared__ T tile[64][66];
-    turn_tile<T, 4>(j, blockIdx.x, tile);
+__global__ __launch_bounds__(256) void pad_kernel(Pad j) {
+    constexpr int E = Mma<T>::E;
+    for (unsigned at = blockIdx.x * 256 + threadIdx.x; at < j.first[4]; at += gridDim.x * 256) {
+        int kind = 0;
+        while (kind < 3 && at >= j.first[kind + 1]) ++kind;
+        const unsigned i = at - j.first[kind], pieces = j.to_cols[kind] / E, row = i / pieces, m = row / j.to_rows[kind], r = row % j.to_rows[kind];
+        const int cols = j.cols[kind], col = (int)(i % pieces) * E;
+        u32x4 v = {0, 0, 0, 0};
+        if (r < (unsigned)j.rows[kind]) {
+            const T* from = static_cast<const T*>(j.from[kind]) + ((long long)m * j.rows[kind] + r) * j.ld[kind];
+            if (col + E <= cols) {
+                __builtin_memcpy(&v, from + col, 16);
+            } else {
+                T e[E] = {};
+                for (int k = 0; k < E; ++k)
+                    if (col + k < cols) e[k] = from[col + k];
+                __builtin_memcpy(&v, e, 16);
+            }
+        }
+        *reinterpret_cast<u32x4*>(static_cast<T*>(j.to[kind]) + (long long)i * E) = v;
+    }
 }
 
 // All of it in one workgroup: sixteen waves, sixteen chunks, counts in LDS.
-constexpr int SMALL_BINS = 1026, SMALL_N = 16384;
+constexpr int SMALL_BINS = 1026, SMALL_N = 4096;
 __device__ __forceinline__ void order_small(const Sort& s, int* lds) {
     const int bins = s.n_slots + 2, wave = threadIdx.x >> 6;
     int* counts = lds;                 // 16 x bins
@@ -231,7 +264,7 @@ __device__ __forceinline__ void order_small(const Sort& s, int* lds) {
         totals[b] = sum;
     }
     __syncthreads();
-    starts_and_items(s, totals, tmp);
+    starts_and_items(s, totals, tmp, true);
     for (int j = threadIdx.x; j < 16 * bins; j += 1024) counts[j] += totals[j % bins];
     __syncthreads();
     place_chunk(s, wave, counts + wave * bins);
@@ -242,6 +275,24 @@ __global__ __launch_bounds__(1024) void prepare_kernel(Sort s, Turn j) {
     extern __shared__ __align__(16) int prepare_lds[];
     if (blockIdx.x == 0) order_small(s, prepare_lds);
     else turn_tile<T, 16>(j, blockIdx.x - 1, reinterpret_cast<T(*)[66]>(prepare_lds));
+}
+// More requests: chunks counted by a wave each, beside the turning; place_kernel follows (16001 requests of 64 slots:
+// one workgroup 30 us, the two launches 22).
+template <typename T>
+__global__ __launch_bounds__(256) void count_kernel(Sort s, Turn j, unsigned groups) {
+    extern __shared__ __align__(16) int count_lds[];
+    if (blockIdx.x >= groups) {
+        turn_tile<T, 4>(j, blockIdx.x - groups, reinterpret_cast<T(*)[66]>(count_lds));
+        return;
+    }
+    const int bins = s.n_slots + 2, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 4 + wave;
+    int* counts = count_lds + wave * bins;
+    for (int b = lane; b < bins; b += 64) counts[b] = 0;
+    __syncthreads();
+    if (c < s.chunks) count_chunk(s, c, counts);
+    __syncthreads();
+    if (c < s.chunks)
+        for (int b = lane; b < bins; b += 64) s.counts[(long long)c * bins + b] = counts[b];
 }
 
 // ---- gradients of the bank -----------------------------------------------------------------------------------------------
@@ -257,6 +308,7 @@ struct SlotGrad {
     long long ldx, lddy;
     float *da, *db, *part;   // part: partials x rank x (d_in + d_out)
     int d_in, d_out, rank, rp;
+    int row_x, row_dy;       // values in a row of x and dy: d_in and d_out, or with zeros up to a whole piece
     bool vec_x, vec_dy;
 };
 // Four waves share an item and a unit, 64 requests at a time each; their sums meet in LDS.  (They take the same branches:
@@ -271,7 +323,8 @@ __device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit,
     const Item it = live ? g.s.items[item] : Item{0, 0, 0, -1};
     const bool is_b = unit >= cols_a * rcs;
     if (is_b) unit -= cols_a * rcs;
-    const int r0 = unit % rcs * RT * 16, c0 = unit / rcs * 16 * E + li * E, d = is_b ? g.d_out : g.d_in, begin = begin_of<E>(c0, d);
+    const int r0 = unit % rcs * RT * 16, c0 = unit / rcs * 16 * E + li * E, d = is_b ? g.d_out : g.d_in;
+    const int row_d = is_b ? g.row_dy : g.row_x, begin = begin_of<E>(c0, row_d);
     const T* src = static_cast<const T*>(is_b ? g.dy : g.x);
     const long long ld = is_b ? g.lddy : g.ldx;
     const float* cf = (is_b ? g.u : g.v) + r0;
@@ -291,7 +344,7 @@ __device__ __forceinline__ void slot_grad(const SlotGrad& g, int item, int unit,
             for (int j = 0; j < LOT; ++j) {
                 const int t = t0 + (s0 + j) * 4 + kl;
                 const T* row = src + (long long)__shfl(mine, min((s0 + j) * 4 + kl, 63)) * ld;
-                xv[j] = vec ? whole_piece<true>(row, begin, d) : whole_piece<false>(row, begin, d);
+                xv[j] = vec ? whole_piece<true>(row, begin, row_d) : whole_piece<false>(row, begin, row_d);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) a[j][r] = cf[(long long)min(t, it.end - 1) * g.rp + min(r * 16 + li, g.rp - 1 - r0)];
             }
@@ -342,10 +395,10 @@ __global__ __launch_bounds__(256) void slot_grad_kernel(SlotGrad g) {
 // other's last workgroups.
 template <typename T, int RT, bool VEC>
 __global__ __launch_bounds__(512) void up_and_slot_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y, long long ldy,
-                                                          bool vec_out, unsigned up_groups, SlotGrad g, unsigned unit_groups) {
+                                                          unsigned up_groups, SlotGrad g, unsigned unit_groups) {
     __shared__ float part[2][4][4][256];
     if (blockIdx.x < up_groups) {
-        up_direct<T, 1, 2, 8, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, blockIdx.x);
+        up_direct<T, 1, 2, 8, VEC>(k, ord, xv, ldx, u, y, ldy, blockIdx.x);
         return;
     }
     const unsigned b = blockIdx.x - up_groups, half = threadIdx.x >> 8;
@@ -368,9 +421,20 @@ __global__ __launch_bounds__(256) void slot_join_kernel(SlotGrad g) {
 // ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
     bool sorted, each;
+    bool pad;                // rows filled up to whole pieces
     int rp, chunk, chunks, len, max_items, max_parts;
-    size_t u, v, perm, slot_at, counts, start, parts, n_items, items, wt, at, bt, part, bytes;
+    int in, out, rank;       // row lengths then: d_in, d_out, rank otherwise
+    size_t xp, wp, ap, bp, dyp, u, v, perm, slot_at, counts, parts, n_items, items, wt, at, bt, part, bytes;
 };
+
+constexpr long long MAX_THREADS = 1ll << 31;      // of a launch (the runtime refuses 2^32)
+
+// Positions of a workgroup of the tiled product, or 0: too few of them to fill the card, the direct one takes it.
+int tiled_positions(long long n, long long ldx, int d_out, size_t esz) {
+    if ((unsigned long long)n * ldx * esz >= (1ull << 32)) return 0;      // (rows are found by 32-bit offsets)
+    const long long outs = (d_out + TILED_OUTS - 1) / TILED_OUTS;
+    return (n + 255) / 256 * outs >= 128 ? 256 : (n + 63) / 64 * outs >= 128 ? 64 : 0;
+}
 
 Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int rank, bool grad) {
     Plan p{};
@@ -389,14 +453,31 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
     // Then nothing needs an order, and it costs a launch, 7 us for 1000 requests; nor do one or two slots.
     p.sorted = grad || (n > 64 && n_slots > 2 && !p.each);
     p.u = take((size_t)n * p.rp * 4);
+    const int e = (int)(16 / esz), in = (d_in + e - 1) / e * e, out = (d_out + e - 1) / e * e, whole_rank = (rank + e - 1) / e * e;
+    p.pad = (in > d_in || whole_rank > rank || (grad && out > d_out)) &&
+            (grad ? tiled_positions(n, out, d_in, esz) : tiled_positions(n, in, d_out, esz)) > 0;
+    p.in = p.pad ? in : d_in;
+    p.out = p.pad ? out : d_out;
+    p.rank = p.pad ? whole_rank : rank;
+    if (p.pad) {
+        p.xp = take((size_t)n * in * esz);
+        p.ap = take((size_t)n_slots * whole_rank * in * esz);
+        if (grad) {
+            p.dyp = take((size_t)n * out * esz);
+        } else {
+            p.wp = take((size_t)d_out * in * esz);
+            p.bp = take((size_t)n_slots * d_out * whole_rank * esz);
+        }
+    }
     if (p.sorted) {
         const bool small = n <= SMALL_N && n_slots + 2 <= SMALL_BINS;
-        p.chunk = small ? (int)((n + 16 * 64 - 1) / (16 * 64) * 64) : (int)std::max<long long>(512, ((n + 127) / 128 + 63) / 64 * 64);
+        // (every workgroup of place_kernel reads all counts: fewer chunks where there are many bins)
+        const long long most = n_slots + 2 <= SMALL_BINS ? 256 : 64;
+        p.chunk = small ? (int)((n + 16 * 64 - 1) / (16 * 64) * 64) : (int)std::max<long long>(256, ((n + most - 1) / most + 63) / 64 * 64);
         p.chunks = small ? 0 : (int)((n + p.chunk - 1) / p.chunk);
         p.perm = take((size_t)n * 4);
         p.slot_at = take((size_t)n * 4);
         p.counts = take((size_t)p.chunks * (n_slots + 2) * 4);
-        p.start = take((size_t)(n_slots + 3) * 4);
     }
     if (grad) {
         p.len = (int)std::max<long long>(512, (n + 255) / 256);
@@ -406,9 +487,9 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
         p.parts = take((size_t)n_slots * sizeof(int2));
         p.n_items = take(4);
         p.items = take((size_t)p.max_items * sizeof(Item));
-        p.wt = take((size_t)d_in * d_out * esz);
-        p.at = take((size_t)n_slots * rank * d_in * esz);
-        p.bt = take((size_t)n_slots * rank * d_out * esz);
+        p.wt = take((size_t)d_in * p.out * esz);
+        p.at = take((size_t)n_slots * d_in * p.rank * esz);
+        p.bt = take((size_t)n_slots * p.rank * p.out * esz);
         p.part = take((size_t)p.max_parts * rank * ((size_t)d_in + d_out) * 4);
     }
     return p;
@@ -441,7 +522,6 @@ int run_order(const Call& c, const Plan& p, Sort* out, const Turn* turn) {      
     s.perm = reinterpret_cast<int*>(c.ws + p.perm);
     s.slot_at = reinterpret_cast<int*>(c.ws + p.slot_at);
     s.counts = reinterpret_cast<int*>(c.ws + p.counts);
-    s.start = reinterpret_cast<int*>(c.ws + p.start);
     if (turn) {
         s.parts = reinterpret_cast<int2*>(c.ws + p.parts);
         s.n_items = reinterpret_cast<int*>(c.ws + p.n_items);
@@ -458,16 +538,39 @@ int run_order(const Call& c, const Plan& p, Sort* out, const Turn* turn) {      
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
-    count_kernel<<<(unsigned)p.chunks, 64, bins * 4, c.st>>>(s);
+    const int waves = c.n_slots + 2 <= SMALL_BINS ? 16 : 4;
+    const unsigned groups = (unsigned)(p.chunks + 3) / 4;
+    const size_t count_lds = std::max<size_t>(4 * bins * 4, 64 * 66 * sizeof(T)), place_lds = ((waves + 1) * bins + 2048) * 4;
+    if (count_lds > 48 * 1024)
+        RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(count_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)count_lds));
+    if (place_lds > 48 * 1024)
+        RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)place_lds));
+    count_kernel<T><<<groups + tiles, 256, count_lds, c.st>>>(s, turn ? *turn : Turn{}, groups);
     RAG_HIP(hipGetLastError());
-    scan_kernel<<<1, 1024, (bins + 1024) * 4, c.st>>>(s);
+    place_kernel<<<(unsigned)((p.chunks + waves - 1) / waves), 1024, place_lds, c.st>>>(s, waves);
     RAG_HIP(hipGetLastError());
-    place_kernel<<<(unsigned)p.chunks, 64, bins * 4, c.st>>>(s);
+    return RAG_OK;
+}
+
+// One matrix more to copy: `count` of rows x cols, or of to_rows x to_cols.
+template <typename T>
+void pad_more(Pad* j, int* kinds, const void* from, long long ld, void* to, long long count, int rows, int cols, int to_rows, int to_cols) {
+    const int i = (*kinds)++;
+    j->from[i] = from;
+    j->to[i] = to;
+    j->ld[i] = ld;
+    j->rows[i] = rows;
+    j->cols[i] = cols;
+    j->to_rows[i] = to_rows;
+    j->to_cols[i] = to_cols;
+    // (below 2^31: rows of n are within 4 GiB, the bank within 4096 x 128 x 8192)
+    for (int k = i; k < 4; ++k) j->first[k + 1] = j->first[i] + (unsigned)(count * to_rows * (to_cols / Mma<T>::E));
+}
+template <typename T>
+int launch_pad(const Pad& j, hipStream_t st) {
+    if (j.first[4] == 0) return RAG_OK;
+    pad_kernel<T><<<(unsigned)std::min<long long>((j.first[4] + 255) / 256, (long long)num_cus() * 32), 256, 0, st>>>(j);
     RAG_HIP(hipGetLastError());
-    if (tiles > 0) {
-        turn_kernel<T><<<tiles, 256, 0, c.st>>>(*turn);
-        RAG_HIP(hipGetLastError());
-    }
     return RAG_OK;
 }
 
@@ -489,26 +592,16 @@ int launch_down(const Plan& p, const Down& d, const Order& o, unsigned kinds, hi
     return RAG_OK;
 }
 
-constexpr long long MAX_THREADS = 1ll << 31;      // of a launch (the runtime refuses 2^32)
-
-// Positions of a workgroup of the tiled product, or 0: too few of them to fill the card, the direct one takes it.
-int tiled_positions(const Bank& k, const Order& o, long long ldx, size_t esz) {
-    if ((unsigned long long)o.n * ldx * esz >= (1ull << 32)) return 0;      // (rows are found by 32-bit offsets)
-    const long long outs = (k.d_out + TILED_OUTS - 1) / TILED_OUTS;
-    return (o.n + 255) / 256 * outs >= 128 ? 256 : (o.n + 63) / 64 * outs >= 128 ? 64 : 0;
-}
-
 template <typename T, bool VEC>
 int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const float* u, void* y, long long ldy, hipStream_t st) {
-    const bool vec_out = ldy % 4 == 0 && ((uintptr_t)y & 15) == 0;
-    const int pos = VEC ? tiled_positions(k, o, ldx, sizeof(T)) : 0;
+    const int pos = VEC ? tiled_positions(o.n, ldx, k.d_out, sizeof(T)) : 0;
     if (pos > 0) {
         const unsigned tiles = (unsigned)((o.n + pos - 1) / pos * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
         const bool short_rank = k.rank <= 4 * Mma<T>::E;
         auto fn = pos == 256 ? (short_rank ? up_tiled_kernel<T, 1, 256> : up_tiled_kernel<T, 2, 256>)
                              : (short_rank ? up_tiled_kernel<T, 1, 64> : up_tiled_kernel<T, 2, 64>);
         RAG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, tiled_lds_bytes(pos)));
-        fn<<<tiles, 512, tiled_lds_bytes(pos), st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy, vec_out);
+        fn<<<tiles, 512, tiled_lds_bytes(pos), st>>>(k, o, x, ldx, (unsigned)((unsigned long long)o.n * ldx * sizeof(T)), u, y, ldy);
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
@@ -516,7 +609,7 @@ int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const
     auto launch = [&](auto fn, int ot, int tt, int threads) {
         const long long groups = grid(ot, tt), most = MAX_THREADS / threads;
         for (long long first = 0; first < groups; first += most)
-            fn<<<(unsigned)std::min(most, groups - first), threads, 0, st>>>(k, o, x, ldx, u, y, ldy, vec_out, (int)first);
+            fn<<<(unsigned)std::min(most, groups - first), threads, 0, st>>>(k, o, x, ldx, u, y, ldy, (int)first);
     };
     if (grid(2, 4) >= 1024) launch(up_direct_kernel<T, 2, 4, 4, VEC>, 2, 4, 256);
     else if (grid(1, 4) >= 512) launch(up_direct_kernel<T, 1, 4, 8, VEC>, 1, 4, 512);
@@ -528,9 +621,9 @@ int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const
 
 Bank make_bank(const Call& c, const Plan& p, const void* w, const void* a, const void* b, int d_in, int d_out) {
     const int e = c.dtype == RAG_DTYPE_BF16 ? 8 : 4;
-    Bank k{w, a, b, c.scale, d_in, d_out, c.n_slots, c.rank, p.rp, false, false};
+    Bank k{w, a, b, c.scale, d_in, d_out, c.n_slots, p.rank, p.rp, false, false};
     k.vec_in = d_in % e == 0 && (((uintptr_t)w | (uintptr_t)a) & 15) == 0;
-    k.vec_rank = c.rank % e == 0 && ((uintptr_t)b & 15) == 0;
+    k.vec_rank = p.rank % e == 0 && ((uintptr_t)b & 15) == 0;
     return k;
 }
 
@@ -544,15 +637,36 @@ int run_apply(const Call& c, const Plan& p) {
         o.perm = s.perm;
         o.slot_at = s.slot_at;
     }
-    const Bank k = make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out);
+    const void *x = c.x, *w = c.w, *a = c.a, *b = c.b;
+    long long ldx = c.ldx;
+    if (p.pad) {
+        Pad j{};
+        int kinds = 0;
+        pad_more<T>(&j, &kinds, a, c.d_in, c.ws + p.ap, c.n_slots, c.rank, c.d_in, p.rank, p.in);
+        a = c.ws + p.ap;
+        if (p.in > c.d_in) {
+            pad_more<T>(&j, &kinds, x, ldx, c.ws + p.xp, 1, (int)c.n, c.d_in, (int)c.n, p.in);
+            pad_more<T>(&j, &kinds, w, c.d_in, c.ws + p.wp, 1, c.d_out, c.d_in, c.d_out, p.in);
+            x = c.ws + p.xp;
+            w = c.ws + p.wp;
+            ldx = p.in;
+        }
+        if (p.rank > c.rank) {
+            pad_more<T>(&j, &kinds, b, c.rank, c.ws + p.bp, c.n_slots, c.d_out, c.rank, c.d_out, p.rank);
+            b = c.ws + p.bp;
+        }
+        const int rc = launch_pad<T>(j, c.st);
+        if (rc) return rc;
+    }
+    const Bank k = make_bank(c, p, w, a, b, p.in, c.d_out);
     float* u = reinterpret_cast<float*>(c.ws + p.u);
-    const Down d{{k, k}, {c.x, nullptr}, {c.ldx, 0}, {u, nullptr}};
-    if (k.vec_in && aligned16(c.x, c.ldx, sizeof(T))) {
+    const Down d{{k, k}, {x, nullptr}, {ldx, 0}, {u, nullptr}};
+    if (k.vec_in && aligned16(x, ldx, sizeof(T))) {
         const int rc = launch_down<T, true>(p, d, o, 1, c.st);
-        return rc ? rc : launch_up<T, true>(k, o, c.x, c.ldx, u, c.y, c.ldy, c.st);
+        return rc ? rc : launch_up<T, true>(k, o, x, ldx, u, c.y, c.ldy, c.st);
     }
     const int rc = launch_down<T, false>(p, d, o, 1, c.st);
-    return rc ? rc : launch_up<T, false>(k, o, c.x, c.ldx, u, c.y, c.ldy, c.st);
+    return rc ? rc : launch_up<T, false>(k, o, x, ldx, u, c.y, c.ldy, c.st);
 }
 
 template <typename T>
@@ -567,7 +681,9 @@ int run_grad(const Call& c, const Plan& p) {
         t.to[i] = to[i];
         t.rows[i] = rows[i];
         t.cols[i] = cols[i];
-        t.first[i + 1] = t.first[i] + (c.n > 0 && (i == 0 || c.dx) ? count[i] * ((rows[i] + 63) / 64) * ((cols[i] + 63) / 64) : 0);
+        t.to_rows[i] = i == 0 ? p.rank : c.d_in;
+        t.to_cols[i] = i == 2 ? p.rank : p.out;
+        t.first[i + 1] = t.first[i] + (c.n > 0 && (i == 0 || c.dx) ? count[i] * ((t.to_rows[i] + 63) / 64) * ((t.to_cols[i] + 63) / 64) : 0);
     }
     Sort s;
     int rc = run_order<T>(c, p, &s, &t);
@@ -576,20 +692,40 @@ int run_grad(const Call& c, const Plan& p) {
     const Order o{s.perm, s.slot_at, c.slots, c.n, c.n_slots};
     float* u = reinterpret_cast<float*>(c.ws + p.u);
     float* v = reinterpret_cast<float*>(c.ws + p.v);
-    const SlotGrad g{s, u, v, c.x, c.dy, c.ldx, c.lddy, c.da, c.db, reinterpret_cast<float*>(c.ws + p.part), c.d_in, c.d_out, c.rank, p.rp,
-                     c.d_in % E == 0 && aligned16(c.x, c.ldx, sizeof(T)), c.d_out % E == 0 && aligned16(c.dy, c.lddy, sizeof(T))};
-    const Bank fore = make_bank(c, p, c.w, c.a, c.b, c.d_in, c.d_out), back = make_bank(c, p, to[1], to[0], to[2], c.d_out, c.d_in);
+    const void *x = c.x, *a = c.a, *dy = c.dy;
+    long long ldx = c.ldx, lddy = c.lddy;
+    if (p.pad) {
+        Pad j{};
+        int kinds = 0;
+        pad_more<T>(&j, &kinds, a, c.d_in, c.ws + p.ap, c.n_slots, c.rank, c.d_in, p.rank, p.in);
+        a = c.ws + p.ap;
+        if (p.in > c.d_in) {
+            pad_more<T>(&j, &kinds, x, ldx, c.ws + p.xp, 1, (int)c.n, c.d_in, (int)c.n, p.in);
+            x = c.ws + p.xp;
+            ldx = p.in;
+        }
+        if (p.out > c.d_out) {
+            pad_more<T>(&j, &kinds, dy, lddy, c.ws + p.dyp, 1, (int)c.n, c.d_out, (int)c.n, p.out);
+            dy = c.ws + p.dyp;
+            lddy = p.out;
+        }
+        rc = launch_pad<T>(j, c.st);
+        if (rc) return rc;
+    }
+    const SlotGrad g{s, u, v, x, dy, ldx, lddy, c.da, c.db, reinterpret_cast<float*>(c.ws + p.part), c.d_in, c.d_out, c.rank, p.rp,
+                     p.in, p.out, p.in % E == 0 && aligned16(x, ldx, sizeof(T)), p.out % E == 0 && aligned16(dy, lddy, sizeof(T))};
+    const Bank fore = make_bank(c, p, c.w, a, c.b, p.in, c.d_out), back = make_bank(c, p, to[1], to[0], to[2], p.out, c.d_in);
     const bool vec = fore.vec_in && g.vec_x && back.vec_in && g.vec_dy;
     if (c.n > 0) {
-        const Down d{{fore, back}, {c.x, c.dy}, {c.ldx, c.lddy}, {u, v}};
+        const Down d{{fore, back}, {x, dy}, {ldx, lddy}, {u, v}};
         rc = vec ? launch_down<T, true>(p, d, o, 2, c.st) : launch_down<T, false>(p, d, o, 2, c.st);
         if (rc) return rc;
     }
     const long long ups = (long long)((c.d_in + 15) / 16) * ((c.n + 31) / 32);
-    const bool together = c.n > 0 && c.dx && !(vec && tiled_positions(back, o, c.lddy, sizeof(T)) > 0) && ups * 512 <= MAX_THREADS;
+    const bool together = c.n > 0 && c.dx && !(vec && tiled_positions(c.n, lddy, c.d_in, sizeof(T)) > 0) && ups * 512 <= MAX_THREADS;
     if (c.n > 0 && c.dx && !together) {
-        rc = vec ? launch_up<T, true>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, c.st)
-                 : launch_up<T, false>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, c.st);
+        rc = vec ? launch_up<T, true>(back, o, dy, lddy, v, c.dx, c.lddx, c.st)
+                 : launch_up<T, false>(back, o, dy, lddy, v, c.dx, c.lddx, c.st);
         if (rc) return rc;
     }
     auto launch = [&](auto rt) {
@@ -600,9 +736,8 @@ int run_grad(const Call& c, const Plan& p) {
             return;
         }
         const unsigned groups = (unsigned)((units + 1) / 2);
-        const bool vec_out = c.lddx % 4 == 0 && ((uintptr_t)c.dx & 15) == 0;
         auto fn = vec ? up_and_slot_kernel<T, RT, true> : up_and_slot_kernel<T, RT, false>;
-        fn<<<(unsigned)ups + (unsigned)p.max_items * groups, 512, 0, c.st>>>(back, o, c.dy, c.lddy, v, c.dx, c.lddx, vec_out, (unsigned)ups, g, groups);
+        fn<<<(unsigned)ups + (unsigned)p.max_items * groups, 512, 0, c.st>>>(back, o, dy, lddy, v, c.dx, c.lddx, (unsigned)ups, g, groups);
     };
     if (c.rank <= 16) launch(std::integral_constant<int, 1>());
     else if (c.rank <= 32) launch(std::integral_constant<int, 2>());

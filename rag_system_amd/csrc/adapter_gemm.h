@@ -305,15 +305,16 @@ __device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, 
 
 // A tile of Y^T to memory: lane = position, four columns.
 template <typename T>
-__device__ __forceinline__ void put(const Bank& k, void* y, long long ldy, long long request, int o, int slot, f32x4 v, bool vec) {
+__device__ __forceinline__ void put(const Bank& k, void* y, long long ldy, long long request, int o, int slot, f32x4 v) {
     T* to = static_cast<T*>(y) + request * ldy + o;
     if (slot == -2) v = f32x4{NAN, NAN, NAN, NAN};
-    if (vec && o + 4 <= k.d_out) {
+    if (o + 4 <= k.d_out) {             // (of any alignment)
         if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<f32x4*>(to) = v;
+            __builtin_memcpy(to, &v, 16);
         } else {
             typedef u16 u16x4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<u16x4*>(to) = u16x4{f_to_bf(v[0]), f_to_bf(v[1]), f_to_bf(v[2]), f_to_bf(v[3])};
+            typedef unsigned long long any64 __attribute__((aligned(2), may_alias));
+            *reinterpret_cast<any64*>(to) = __builtin_bit_cast(unsigned long long, u16x4{f_to_bf(v[0]), f_to_bf(v[1]), f_to_bf(v[2]), f_to_bf(v[3])});
         }
         return;
     }
@@ -325,7 +326,7 @@ __device__ __forceinline__ void put(const Bank& k, void* y, long long ldy, long 
 // straight from memory (each byte is used by one wave, LDS would only add a trip); their sums meet in LDS, a wave finishes a tile.
 template <typename T, int OT, int TT, int WAVES, bool VEC>
 __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const void* xv, long long ldx, const float* u, void* y,
-                                          long long ldy, bool vec_out, int block) {
+                                          long long ldy, int block) {
     typedef Mma<T> M;
     constexpr int E = M::E;
     __shared__ float part[WAVES][OT * TT][256];
@@ -389,14 +390,14 @@ __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const
         const int o = o0 + j / TT * 16;
         const long long pos = p0 + j % TT * 16 + li;
         const int slot = pos < ord.n ? ord.slot(pos) : -3;
-        if (pos < ord.n && o + 4 * kl < k.d_out) put<T>(k, y, ldy, ord.request(pos), o + 4 * kl, slot, sum, vec_out);
+        if (pos < ord.n && o + 4 * kl < k.d_out) put<T>(k, y, ldy, ord.request(pos), o + 4 * kl, slot, sum);
     }
 }
 
 template <typename T, int OT, int TT, int WAVES, bool VEC>
 __global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y,
-                                                               long long ldy, bool vec_out, int first) {
-    up_direct<T, OT, TT, WAVES, VEC>(k, ord, xv, ldx, u, y, ldy, vec_out, first + (int)blockIdx.x);
+                                                               long long ldy, int first) {
+    up_direct<T, OT, TT, WAVES, VEC>(k, ord, xv, ldx, u, y, ldy, first + (int)blockIdx.x);
 }
 
 // Y for many requests: a workgroup has 128 output columns x POS positions (256, or 64 where that would leave CUs idle), each of
@@ -408,7 +409,7 @@ constexpr int TILED_OUTS = 128;
 constexpr int tiled_lds_bytes(int pos) { return 3 * (TILED_OUTS + pos) * 128; }
 template <typename T, int RS, int POS>
 __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, const void* xv, long long ldx, unsigned x_bytes, const float* u, void* y,
-                                                          long long ldy, bool vec_out) {
+                                                          long long ldy) {
     typedef Mma<T> M;
     constexpr int E = M::E, ESZ = sizeof(T), ROWS = TILED_OUTS + POS, STAGE = ROWS * 128, LOADS = ROWS / 8 / 8;
     constexpr int WP = POS / 64 >= 4 ? 4 : 2, WO = 8 / WP, TO = 8 / WO, TP = POS / 16 / WP;   // waves, and tiles of a wave
@@ -580,7 +581,7 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
         if (slot > -3) {
 #pragma unroll
             for (int o = 0; o < TO; ++o)
-                if (ob + o * 16 + 4 * kl < k.d_out) put<T>(k, y, ldy, request, ob + o * 16 + 4 * kl, slot, v[o], vec_out);
+                if (ob + o * 16 + 4 * kl < k.d_out) put<T>(k, y, ldy, request, ob + o * 16 + 4 * kl, slot, v[o]);
         }
     }
 }

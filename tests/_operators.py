@@ -13,38 +13,50 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def split_rest(dtype):
+    """What a float32 factor of a product with bfloat16 weights may lose: it is multiplied as its bfloat16 h, off by up to half
+    a step (2^-8 of the value), and the bfloat16 of the difference, off by half a step of that: 2^-8 * 2^-8 of the value.  (Where
+    the sums are long, their own allowance hides it: 768 products 2^-13.4; it is more than that of 5 products, 2^-19.8.)"""
+    return half_step(dtype) ** 2 if dtype == torch.bfloat16 else 0.0
+
+
 def adapters_ref(x, W, A, B, scale, slots):
     """(y, allow) in 64 bits; slots: list of ints, -1 = none."""
+    rest = split_rest(x.dtype)
     x, W, A, B, scale = (t.detach().cpu().double() for t in (x, W, A, B, scale))
     y, mag = x @ W.t(), x.abs() @ W.abs().t()
+    low = torch.zeros_like(mag)                 # of the adapters alone
     for t, s in enumerate(slots):
         if s >= 0:
             y[t] += scale[s] * (B[s] @ (A[s] @ x[t]))
-            mag[t] += scale[s].abs() * (B[s].abs() @ (A[s].abs() @ x[t].abs()))
+            low[t] = scale[s].abs() * (B[s].abs() @ (A[s].abs() @ x[t].abs()))
     # a product of A passes its own sum over d_in, the scaling, the product with B and the sum over d_in + rank
-    return y, (2 * W.shape[1] + A.shape[1] + 6) * U32 * mag
+    return y, (2 * W.shape[1] + A.shape[1] + 6) * U32 * (mag + low) + rest * low
 
 
 def adapters_grad_ref(x, W, A, B, scale, slots, dy):
     """{dx, dA, dB: (value, allow)}"""
+    rest = split_rest(x.dtype)
     x, W, A, B, scale, dy = (t.detach().cpu().double() for t in (x, W, A, B, scale, dy))
     n, (d_out, d_in), (S, R, _) = x.shape[0], W.shape, A.shape
     out = {}
     for sign in (False, True):
         f = torch.abs if sign else (lambda t: t)
         dx, dA, dB = f(dy) @ f(W), torch.zeros_like(A), torch.zeros_like(B)
+        low = torch.zeros_like(dx)
         for t, s in enumerate(slots):
             if s < 0:
                 continue
             u = f(scale[s]) * (f(A[s]) @ f(x[t]))
             v = f(scale[s]) * (f(B[s]).t() @ f(dy[t]))
-            dx[t] += f(A[s]).t() @ v
+            low[t] = f(A[s]).t() @ v
+            dx[t] += low[t]
             dA[s] += torch.outer(v, f(x[t]))
             dB[s] += torch.outer(f(dy[t]), u)
         for k, t in (("dx", dx), ("dA", dA), ("dB", dB)):
             out.setdefault(k, []).append(t)
     steps = {"dx": 2 * d_out + R + 6, "dA": d_out + n + 6, "dB": d_in + n + 6}
-    return {k: (v, steps[k] * U32 * m) for k, (v, m) in out.items()}
+    return {k: (v, steps[k] * U32 * m + (rest * low if k == "dx" else 0.0)) for k, (v, m) in out.items()}
 
 
 def distill_ref(q, X, ids, scores, tau, tau_t, metric, over, weights=None):

@@ -291,3 +291,30 @@ def test_more_workgroups_than_a_launch_takes():
     ref = adapters_grad_ref(x[some], W, A, B, bank.scale, slots[some].tolist(), dy[some])["dx"]
     assert_within(dx[some], *ref, "dx")
     assert not dB.any()                 # (x is zero)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,d_in,d_out,S,R", [(2100, 71, 515, 7, 13), (2100, 72, 515, 7, 13), (2100, 71, 515, 7, 16), (4200, 257, 33, 5, 9),
+                                              (4200, 264, 33, 5, 16), (4200, 257, 259, 70, 1), (4097, 5, 900, 3, 2)])
+def test_rows_of_no_whole_pieces(n, d_in, d_out, S, R, dtype):
+    """Large batches whose rows, ranks or both do not end with a 16-byte piece."""
+    check(*make(n, d_in, d_out, S, R, dtype, seed=31))
+
+
+@pytest.mark.parametrize("n,S", [(4096, 1024), (4097, 1024), (4097, 1025), (5003, 4096), (9000, 1), (20001, 3), (40000, 130)])
+def test_order_of_many_requests(n, S):
+    """Requests over one chunk and many, few bins and many, with slots that nobody has and slots outside the bank."""
+    bank, x, slots, dy = make(n, 8, 12, S, 2, seed=32)
+    slots[slots % 5 == 3] = -1
+    slots[n // 2] = S
+    y_ref, y_allow = adapters_ref(x, bank.weight, bank.A, bank.B, bank.scale, slots.where(slots < S, -1).tolist())
+    y = bank.apply(x, slots)
+    assert torch.isnan(y[n // 2]).all()
+    y_ref[n // 2] = float("nan")
+    assert_within(y, y_ref, y_allow, "y")
+    ok = slots.where(slots < S, -1)
+    g_ref = adapters_grad_ref(x, bank.weight, bank.A, bank.B, bank.scale, ok.tolist(), dy)
+    dx, dA, dB = bank.grad(x, slots, dy)
+    g_ref["dx"][0][n // 2] = float("nan")
+    for name, got in (("dx", dx), ("dA", dA), ("dB", dB)):
+        assert_within(got, *g_ref[name], name)
