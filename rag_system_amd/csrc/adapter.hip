@@ -659,9 +659,17 @@ int run_apply(const Call& c, const Plan& p) {
         if (rc) return rc;
     }
     const Bank k = make_bank(c, p, w, a, b, p.in, c.d_out);
+    const bool vec = k.vec_in && aligned16(x, ldx, sizeof(T));
+    if (c.n <= 16 && c.n * c.rank * c.d_in <= WHOLE_PRODUCTS) {
+        const unsigned groups = (unsigned)(c.d_out + 15) / 16;
+        if (vec) whole_kernel<T, true><<<groups, 512, 0, c.st>>>(k, o, x, ldx, c.y, c.ldy);
+        else whole_kernel<T, false><<<groups, 512, 0, c.st>>>(k, o, x, ldx, c.y, c.ldy);
+        RAG_HIP(hipGetLastError());
+        return RAG_OK;
+    }
     float* u = reinterpret_cast<float*>(c.ws + p.u);
     const Down d{{k, k}, {x, nullptr}, {ldx, 0}, {u, nullptr}};
-    if (k.vec_in && aligned16(x, ldx, sizeof(T))) {
+    if (vec) {
         const int rc = launch_down<T, true>(p, d, o, 1, c.st);
         return rc ? rc : launch_up<T, true>(k, o, x, ldx, u, c.y, c.ldy, c.st);
     }

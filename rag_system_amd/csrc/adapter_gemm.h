@@ -207,12 +207,37 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Down d, Order ord
     }
 }
 
-// U where slots have few requests each: a workgroup per position, a wave per row of A_s.
+// Four values of U from r0 on of one position (in lanes 0 to 3): one wave, 16 bytes a lane of x and of each of A's four rows.
+template <typename T, bool VEC>
+__device__ __forceinline__ float down_rows(const Bank& k, const T* x, int s, int r0) {
+    constexpr int E = Mma<T>::E;
+    const int lane = threadIdx.x & 63;
+    const T* a = static_cast<const T*>(k.a) + (long long)s * k.rank * k.d_in;
+    float acc[4] = {};
+    for (int c = lane * E; c < k.d_in; c += 64 * E) {
+        const u32x4 xp = piece<VEC>(x, c, k.d_in);
+        u32x4 ap[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ap[r] = piece<VEC>(a + (long long)min(r0 + r, k.rank - 1) * k.d_in, c, k.d_in);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float xe = element<T>(xp, e);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = fmaf(element<T>(ap[r], e), xe, acc[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        for (int o = 32; o > 0; o >>= 1) acc[r] += __shfl_xor(acc[r], o);
+    const float v = lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3];
+    return r0 + lane < k.rank ? v * k.scale[s] : 0.f;
+}
+
+// U where slots have few requests each: a workgroup per position, a wave per four rows of A_s.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void down_each_kernel(Down d, Order ord) {
     const Bank& k = d.bank[blockIdx.y];
     float* u = d.u[blockIdx.y];
-    constexpr int E = Mma<T>::E;
     const long long p = blockIdx.x;
     const int s = ord.slot(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (s < 0) {
@@ -220,29 +245,9 @@ __global__ __launch_bounds__(256) void down_each_kernel(Down d, Order ord) {
         return;
     }
     const T* x = static_cast<const T*>(d.x[blockIdx.y]) + ord.request(p) * d.ldx[blockIdx.y];
-    const T* a = static_cast<const T*>(k.a) + (long long)s * k.rank * k.d_in;
-    const float scale = k.scale[s];
     for (int r0 = wave * 4; r0 < k.rp; r0 += 16) {
-        float acc[4] = {};
-        for (int c = lane * E; c < k.d_in; c += 64 * E) {
-            const u32x4 xp = piece<VEC>(x, c, k.d_in);
-            u32x4 ap[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) ap[r] = piece<VEC>(a + (long long)min(r0 + r, k.rank - 1) * k.d_in, c, k.d_in);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float xe = element<T>(xp, e);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[r] = fmaf(element<T>(ap[r], e), xe, acc[r]);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            for (int o = 32; o > 0; o >>= 1) acc[r] += __shfl_xor(acc[r], o);
-        if (lane < 4) {
-            const float v = lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3];
-            u[p * k.rp + r0 + lane] = r0 + lane < k.rank ? v * scale : 0.f;
-        }
+        const float v = down_rows<T, VEC>(k, x, s, r0);
+        if (lane < 4) u[p * k.rp + r0 + lane] = v;
     }
 }
 
@@ -324,9 +329,10 @@ __device__ __forceinline__ void put(const Bank& k, void* y, long long ldy, long 
 
 // Y for a few requests: a workgroup has OT x 16 output columns and TT x 16 positions, its waves every WAVES-th step along d_in,
 // straight from memory (each byte is used by one wave, LDS would only add a trip); their sums meet in LDS, a wave finishes a tile.
-template <typename T, int OT, int TT, int WAVES, bool VEC>
+// WHOLE: U too, by each workgroup for itself, into `own` in LDS (at most 16 requests).
+template <typename T, int OT, int TT, int WAVES, bool VEC, bool WHOLE = false>
 __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const void* xv, long long ldx, const float* u, void* y,
-                                          long long ldy, int block) {
+                                          long long ldy, int block, float* own = nullptr) {
     typedef Mma<T> M;
     constexpr int E = M::E;
     __shared__ float part[WAVES][OT * TT][256];
@@ -372,6 +378,16 @@ __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const
     for (int o = 0; o < OT; ++o)
 #pragma unroll
         for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4*>(&part[wave][o * TT + t][lane * 4]) = acc[o][t];
+    if (WHOLE) {
+        const int quads = k.rp / 4;
+        for (int j = wave; j < (int)ord.n * quads; j += WAVES) {
+            const int p = j / quads, s = ord.slot(p), r0 = j % quads * 4;
+            const float v = s >= 0 && r0 < k.rank ? down_rows<T, VEC>(k, x + ord.request(p) * ldx, s, r0) : 0.f;
+            if (lane < 4) own[p * k.rp + r0 + lane] = v;
+        }
+        u = own;
+        __syncthreads();
+    }
     // the adapters' side: the waves of a tile share the steps of the rank
     constexpr int TILES = OT * TT, SHARES = WAVES > TILES ? WAVES / TILES : 1;
     static_assert(WAVES % TILES == 0 || TILES % WAVES == 0, "waves of a tile");
@@ -398,6 +414,15 @@ template <typename T, int OT, int TT, int WAVES, bool VEC>
 __global__ __launch_bounds__(64 * WAVES) void up_direct_kernel(Bank k, Order ord, const void* xv, long long ldx, const float* u, void* y,
                                                                long long ldy, int first) {
     up_direct<T, OT, TT, WAVES, VEC>(k, ord, xv, ldx, u, y, ldy, first + (int)blockIdx.x);
+}
+
+// Both products of a few requests in one launch, while what every workgroup does again is little (768 wide, rank 16: 8 requests 15.5 us
+// with two launches, 12.6 with one; 16 requests 15, 17.8).
+constexpr long long WHOLE_PRODUCTS = 100000;
+template <typename T, bool VEC>
+__global__ __launch_bounds__(512) void whole_kernel(Bank k, Order ord, const void* xv, long long ldx, void* y, long long ldy) {
+    __shared__ __align__(16) float own[16 * 128];
+    up_direct<T, 1, 1, 8, VEC, true>(k, ord, xv, ldx, nullptr, y, ldy, blockIdx.x, own);
 }
 
 // Y for many requests: a workgroup has 128 output columns x POS positions (256, or 64 where that would leave CUs idle), each of
