@@ -598,7 +598,7 @@ template <typename T, bool VEC>
 int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const float* u, void* y, long long ldy, hipStream_t st) {
     const int pos = VEC ? tiled_positions(o.n, ldx, k.d_out, sizeof(T)) : 0;
     if (pos > 0) {
-        const unsigned tiles = (unsigned)((o.n + pos - 1) / pos * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
+        const unsigned tiles = (unsigned)(((o.n + pos - 1) / pos + 7) / 8 * 8 * ((k.d_out + TILED_OUTS - 1) / TILED_OUTS));
         const bool short_rank = k.rank <= 4 * Mma<T>::E;
         auto fn = pos == 256 ? (short_rank ? up_tiled_kernel<T, 1, 256> : up_tiled_kernel<T, 2, 256>)
                              : (short_rank ? up_tiled_kernel<T, 1, 64> : up_tiled_kernel<T, 2, 64>);

@@ -441,8 +441,11 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
     extern __shared__ __align__(16) char tiled_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, kl = lane >> 4;
     const int outs = (k.d_out + TILED_OUTS - 1) / TILED_OUTS;
-    const long long p0 = (long long)(blockIdx.x / outs) * POS;
-    const int o0 = blockIdx.x % outs * TILED_OUTS;
+    // the workgroups of the same positions follow each other on ONE of the eight dies, whose L2 then has their rows
+    const unsigned turn = blockIdx.x >> 3;
+    const long long p0 = (long long)((blockIdx.x & 7) + 8 * (turn / outs)) * POS;
+    const int o0 = turn % outs * TILED_OUTS;
+    if (p0 >= ord.n) return;
     const int stages = (k.d_in * ESZ + 127) / 128;
     const int lr = lane >> 3, lp = (lane & 7) ^ lr;
     // a wave's instructions: every eighth group of eight rows, W's first

@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_kernel(TileCall c) {
     const long long qi = ((long long)q_tile * WQ + wq) * 16 + li;
     const T* x = static_cast<const T*>(c.x);
     // where a row's pieces are: place of piece p of row r = p ^ turn(r)
-    auto turn = [](int r) __attribute__((always_inline)) { return BF ? ((r & 3) << 1) | ((r >> 2) & 1) : r & 7; };
+    auto turn = [](int r) __attribute__((always_inline)) { return BF ? (((r & 3) << 1) | ((r >> 2) & 1)) ^ ((r >> 1) & 2) : r & 7; };
 
     // queries: B operand of S^T, piece kl of every four (a lane without a query takes the first one's: its results are
     // not stored); zero behind the row's end
