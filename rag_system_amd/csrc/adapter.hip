@@ -585,7 +585,7 @@ int launch_down(const Plan& p, const Down& d, const Order& o, unsigned kinds, hi
         RAG_HIP(hipGetLastError());
         return RAG_OK;
     }
-    const dim3 groups((unsigned)((o.n + DOWN_TOKENS - 1) / DOWN_TOKENS), kinds);
+    const dim3 groups((unsigned)(((o.n + DOWN_TOKENS - 1) / DOWN_TOKENS + 7) / 8 * 8), kinds);
     if (k.rp <= 16) down_kernel<T, 1, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(d, o);
     else if (k.rp <= 32) down_kernel<T, 2, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(d, o);
     else if (k.rp <= 64) down_kernel<T, 4, VEC><<<groups, 64 * DOWN_WAVES, 0, st>>>(d, o);

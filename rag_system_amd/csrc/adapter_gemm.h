@@ -86,24 +86,31 @@ __device__ __forceinline__ u32x4 whole_piece(const T* row, int begin, int end) {
     }
     return r;
 }
-// That piece of `row`; zeros in the place of values before `col` and behind the end.  Two rows' pieces at the same place hold
-// matching values, which is all that a sum over them needs.  VEC: rows are 16-byte aligned and end with a piece.
+// That piece of `row`: what is in memory, and kept of it: zeros in the place of values before `col` and behind the end.  Two rows'
+// pieces at the same place hold matching values, which is all that a sum over them needs.  VEC: rows are 16-byte aligned and end
+// with a piece.  (Apart, since a loop that loads ahead may not touch the values until it uses them: it would wait for them.)
 template <bool VEC, typename T>
-__device__ __forceinline__ u32x4 piece(const T* row, int col, int end) {
+__device__ __forceinline__ u32x4 raw_piece(const T* row, int col, int end) {
     constexpr int E = Mma<T>::E;
+    return whole_piece<VEC>(row, VEC ? min(col, end - E) : begin_of<E>(col, end), end);
+}
+template <bool VEC, int E>
+__device__ __forceinline__ u32x4 kept(u32x4 r, int col, int end) {
     if (VEC) {
-        const u32x4 v = whole_piece<true>(row, min(col, end - E), end);
         const unsigned keep = col < end ? ~0u : 0u;
-        return u32x4{v[0] & keep, v[1] & keep, v[2] & keep, v[3] & keep};
+        return u32x4{r[0] & keep, r[1] & keep, r[2] & keep, r[3] & keep};
     }
     const int begin = begin_of<E>(col, end), skip = col - begin, stop = end - begin;
-    u32x4 r = whole_piece<false>(row, begin, end);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         if (E == 8) r[e] &= (2 * e >= skip && 2 * e < stop ? 0xffffu : 0u) | (2 * e + 1 >= skip && 2 * e + 1 < stop ? 0xffff0000u : 0u);
         else r[e] &= e >= skip && e < stop ? ~0u : 0u;
     }
     return r;
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ u32x4 piece(const T* row, int col, int end) {
+    return kept<VEC, Mma<T>::E>(raw_piece<VEC>(row, col, end), col, end);
 }
 // U's values that go with piece<VEC, T>(b, col, rank), E of them.  (Behind the rank U holds zeros.)
 template <bool VEC, int E>
@@ -141,7 +148,9 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Down d, Order ord
     constexpr int E = M::E;
     __shared__ float part[DOWN_WAVES][2 * RT][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, kl = lane >> 4;
-    const long long p0 = (long long)blockIdx.x * DOWN_TOKENS;
+    // neighbours, which share a slot's A, on ONE of the eight dies (65536 requests of 256 slots x 64 x 768 bf16: 300 -> 134 MB read)
+    const long long p0 = ((long long)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) * DOWN_TOKENS;
+    if (p0 >= ord.n) return;
     const T* x = static_cast<const T*>(d.x[blockIdx.y]);
     const T* row[2];
 #pragma unroll
@@ -166,14 +175,22 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Down d, Order ord
 #pragma unroll
             for (int r = 0; r < RT; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
         u32x4 xp[2][2], ap[2][RT];
-        auto load = [&](int st, u32x4* xt, u32x4* at) __attribute__((always_inline)) {      // (behind the end: zeros)
+        auto load = [&](int st, u32x4* xt, u32x4* at) __attribute__((always_inline)) {
             const int col = (st * 4 + kl) * E;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) xt[t] = piece<VEC>(row[t], col, k.d_in);
+            for (int t = 0; t < 2; ++t) xt[t] = raw_piece<VEC>(row[t], col, k.d_in);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) at[r] = piece<VEC>(a + (long long)min(r * 16 + li, k.rank - 1) * k.d_in, col, k.d_in);
+            for (int r = 0; r < RT; ++r) at[r] = raw_piece<VEC>(a + (long long)min(r * 16 + li, k.rank - 1) * k.d_in, col, k.d_in);
+            __builtin_amdgcn_sched_barrier(0);
         };
-        auto use = [&](const u32x4* xt, const u32x4* at) __attribute__((always_inline)) {
+        auto use = [&](int st, u32x4* xt, u32x4* at) __attribute__((always_inline)) {
+            if ((st + 1) * 4 * E > k.d_in) {         // (uniform; behind the end: zeros)
+                const int col = (st * 4 + kl) * E;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) xt[t] = kept<VEC, E>(xt[t], col, k.d_in);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) at[r] = kept<VEC, E>(at[r], col, k.d_in);
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -182,9 +199,9 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Down d, Order ord
         load(wave, xp[0], ap[0]);
         for (int st = wave; st < steps; st += 2 * DOWN_WAVES) {
             load(st + DOWN_WAVES, xp[1], ap[1]);
-            use(xp[0], ap[0]);
+            use(st, xp[0], ap[0]);
             load(st + 2 * DOWN_WAVES, xp[0], ap[0]);
-            use(xp[1], ap[1]);
+            use(st + DOWN_WAVES, xp[1], ap[1]);
         }
         __syncthreads();
 #pragma unroll
@@ -354,14 +371,22 @@ __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const
         for (int t = 0; t < TT; ++t) acc[o][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int steps = (k.d_in + 4 * E - 1) / (4 * E);
     u32x4 xp[2][TT], wp[2][OT];
-    auto load = [&](int st, u32x4* xt, u32x4* wt) __attribute__((always_inline)) {      // (behind the end: zeros)
+    auto load = [&](int st, u32x4* xt, u32x4* wt) __attribute__((always_inline)) {
         const int col = (st * 4 + kl) * E;
 #pragma unroll
-        for (int t = 0; t < TT; ++t) xt[t] = piece<VEC>(row[t], col, k.d_in);
+        for (int t = 0; t < TT; ++t) xt[t] = raw_piece<VEC>(row[t], col, k.d_in);
 #pragma unroll
-        for (int o = 0; o < OT; ++o) wt[o] = piece<VEC>(w[o], col, k.d_in);
+        for (int o = 0; o < OT; ++o) wt[o] = raw_piece<VEC>(w[o], col, k.d_in);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    auto use = [&](const u32x4* xt, const u32x4* wt) __attribute__((always_inline)) {
+    auto use = [&](int st, u32x4* xt, u32x4* wt) __attribute__((always_inline)) {
+        if ((st + 1) * 4 * E > k.d_in) {             // (uniform; behind the end: zeros)
+            const int col = (st * 4 + kl) * E;
+#pragma unroll
+            for (int t = 0; t < TT; ++t) xt[t] = kept<VEC, E>(xt[t], col, k.d_in);
+#pragma unroll
+            for (int o = 0; o < OT; ++o) wt[o] = kept<VEC, E>(wt[o], col, k.d_in);
+        }
 #pragma unroll
         for (int o = 0; o < OT; ++o)
 #pragma unroll
@@ -370,9 +395,9 @@ __device__ __forceinline__ void up_direct(const Bank& k, const Order& ord, const
     load(wave, xp[0], wp[0]);
     for (int st = wave; st < steps; st += 2 * WAVES) {
         load(st + WAVES, xp[1], wp[1]);
-        use(xp[0], wp[0]);
+        use(st, xp[0], wp[0]);
         load(st + 2 * WAVES, xp[0], wp[0]);
-        use(xp[1], wp[1]);
+        use(st + WAVES, xp[1], wp[1]);
     }
 #pragma unroll
     for (int o = 0; o < OT; ++o)
@@ -505,7 +530,7 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
 #pragma unroll
         for (int a = 0; a < LOADS; ++a) fetch1(b < stages ? b : 0, b, a);
     // what the adapters need of the wave's positions, on its way beside the products
-    int slot0, request0, kept = -1;
+    int slot0, request0, b_slot = -1;
     auto look = [&](int p, int* slot, int* request) __attribute__((always_inline)) {
         const long long pos = p0 + wp + p * 16 + li;
         *slot = pos < ord.n ? ord.slot(pos) : -3;
@@ -522,14 +547,14 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
             for (int h = 0; h < E / 4; ++h) to[r][h] = *reinterpret_cast<const f32x4*>(ur + min((r * 4 + kl) * E + 4 * h, k.rp - 4));
     };
     auto load_b = [&](int s) __attribute__((always_inline)) {
-        if (s == kept) return;                  // (uniform)
+        if (s == b_slot) return;                  // (uniform)
         const T* bs = static_cast<const T*>(k.b) + (long long)s * k.d_out * k.rank;
 #pragma unroll
         for (int o = 0; o < TO; ++o)
 #pragma unroll
             for (int r = 0; r < RS; ++r)
                 bv[o][r] = piece<true>(bs + (long long)min(ob + o * 16 + li, k.d_out - 1) * k.rank, (r * 4 + kl) * E, k.rank);
-        kept = s;
+        b_slot = s;
     };
     auto narrow = [&](const f32x4 (*from)[E / 4], u32x4* hi, u32x4* lo) __attribute__((always_inline)) {
 #pragma unroll
