@@ -159,11 +159,11 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Down d, Order ord
     unsigned todo = (unsigned)__ballot(mine >= 0);
     const int steps = (k.d_in + 4 * E - 1) / (4 * E);
     // positions without an adapter: zeros, outside the bank: NaN
-    for (int j = threadIdx.x; j < DOWN_TOKENS * k.rp; j += 64 * DOWN_WAVES) {
-        const long long p = p0 + j / k.rp;
-        const int s = p < ord.n ? ord.slot(p) : 0;
-        if (s < 0) u[p * k.rp + j % k.rp] = s == -2 ? NAN : 0.f;
-    }
+    if (__ballot(mine == -1 || mine == -2))            // (rp is a multiple of 16: every lane goes round as often)
+        for (int j = threadIdx.x; j < DOWN_TOKENS * k.rp; j += 64 * DOWN_WAVES) {
+            const int s = __shfl(mine, j / k.rp);
+            if (s == -1 || s == -2) u[(p0 + j / k.rp) * k.rp + j % k.rp] = s == -2 ? NAN : 0.f;
+        }
     while (todo) {                    // (uniform over the workgroup: every wave has the same slots)
         const int s = __shfl(mine, __ffs(todo) - 1);
         const unsigned with = (unsigned)__ballot(mine == s) & todo;
