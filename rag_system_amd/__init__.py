@@ -6,6 +6,9 @@ Drop-in layers (same names and semantics as the reference's rag_system package):
   tfidf          TF-IDF cosine scorer                                   (search_engine.py:284-285,330-331)
   vector_storage VectorStorage, VectorStorageManager                    (vector_storage.py:58,314)
   search_engine  SearchEngine, detect_knee                              (search_engine.py:37,51)
+Beside them (not in the reference):
+  adapters       QueryAdapters: low-rank adapters of many requests beside a shared projection, with gradients
+  faiss_compat   IndexFlat.distill: a teacher's top list distilled over the whole index, with the queries' gradient
 
 All arithmetic runs in librag_mi355x.so (hand-written HIP for gfx950, C ABI in
 include/rag_mi355x.h).  Importing the package does not touch the GPU; the first numeric call

@@ -5,6 +5,7 @@
 // their way while these are used), multiply it with the queries' registers, add the LPR parts with DPP, and put the row
 // straight into their own columns of the row sum.  Every group of LPR lanes keeps its own maximum, sum and row sum
 // (rows of one group: some hundred, so no sum is long); they are joined once, at the end.
+// Measured, 1 query, 1M x 384 float32: 229 us = 6.7 TB/s, 241 with the join (the search's stream of the same bytes: 7.2 TB/s).
 #pragma once
 #include "distill_tile.h"
 
