@@ -94,6 +94,8 @@ int rag_flat_reserve(rag_flat_t* h, int64_t n_capacity);
 int rag_flat_add(rag_flat_t* h, int64_t n, const float* x);
 /* Same as rag_flat_add but the rows are already in HBM (n*d float32). */
 int rag_flat_add_dev(rag_flat_t* h, int64_t n, const float* x_dev, void* stream);
+/* The same for bfloat16 rows of an index that stores bfloat16: they are kept as they are.  No counterpart in the reference. */
+int rag_flat_add_bf16_dev(rag_flat_t* h, int64_t n, const void* x_dev, void* stream);
 /* Append n synthetic L2-normalised rows generated on the device by the
  * counter-based generator of oracle/flat_ref.c:synth_row() (bit-identical),
  * keyed by (seed, first_global_row + i).  Benchmark / test input only; no

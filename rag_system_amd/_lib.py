@@ -61,6 +61,7 @@ SIGNATURES = {
     "rag_flat_reserve": (C.c_int, [_p, _i64]),
     "rag_flat_add": (C.c_int, [_p, _i64, _p]),
     "rag_flat_add_dev": (C.c_int, [_p, _i64, _p, _p]),
+    "rag_flat_add_bf16_dev": (C.c_int, [_p, _i64, _p, _p]),
     "rag_flat_add_synthetic": (C.c_int, [_p, _i64, C.c_uint64, _i64]),
     "rag_flat_ntotal": (_i64, [_p]),
     "rag_flat_dim": (C.c_int, [_p]),

@@ -1911,6 +1911,27 @@ int rag_flat_add_dev(rag_flat_t* h, int64_t n, const float* x_dev, void* stream)
     return RAG_OK;
 }
 
+int rag_flat_add_bf16_dev(rag_flat_t* h, int64_t n, const void* x_dev, void* stream) {
+    RAG_REQUIRE_INIT();
+    if (!h || n < 0 || (n > 0 && !x_dev)) return fail(RAG_ERR_INVALID_ARG, "bad handle, n or x_dev");
+    if (h->dtype != RAG_DTYPE_BF16) return fail(RAG_ERR_INVALID_ARG, "rag_flat_add_bf16_dev: the index stores float32");
+    if (n == 0) return RAG_OK;
+    std::lock_guard<std::mutex> lk(h->mu);
+    int rc = flush_staged(h);
+    if (rc) return rc;
+    rc = ensure_capacity(h, h->ndev + n);
+    if (rc) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    char* dst = h->x + (size_t)h->ndev * h->ld * h->esz;
+    const size_t row = (size_t)h->d * h->esz;
+    if (h->ld == h->d) RAG_HIP(hipMemcpyAsync(dst, x_dev, (size_t)n * row, hipMemcpyDeviceToDevice, st));
+    else RAG_HIP(hipMemcpy2DAsync(dst, (size_t)h->ld * h->esz, x_dev, row, row, (size_t)n, hipMemcpyDeviceToDevice, st));
+    RAG_HIP(hipStreamSynchronize(st));
+    h->ndev += n;
+    h->ntotal += n;
+    return RAG_OK;
+}
+
 int rag_flat_add_synthetic(rag_flat_t* h, int64_t n, uint64_t seed, int64_t first_global_row) {
     RAG_REQUIRE_INIT();
     if (!h || n < 0) return fail(RAG_ERR_INVALID_ARG, "bad handle or n");

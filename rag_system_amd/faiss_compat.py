@@ -54,9 +54,9 @@ class _HipFlatBackend:
         _lib.check(self._lib.rag_flat_add(self._h, x.shape[0], _lib.ptr(x)), self._lib)
 
     def add_dev(self, x):
-        """x: contiguous float32 torch tensor in HBM; on torch's current stream, complete on return."""
-        _lib.check(self._lib.rag_flat_add_dev(self._h, x.shape[0], C.c_void_p(x.data_ptr()), C.c_void_p(dt.stream_of(x))),
-                   self._lib)
+        """x: contiguous torch tensor in HBM, float32 or (bfloat16 storage) bfloat16; on torch's current stream, complete on return."""
+        add = self._lib.rag_flat_add_bf16_dev if x.element_size() == 2 else self._lib.rag_flat_add_dev
+        _lib.check(add(self._h, x.shape[0], C.c_void_p(x.data_ptr()), C.c_void_p(dt.stream_of(x))), self._lib)
 
     def distill(self, q, ids, scores, temperature, teacher_temperature, over, weights, grad):
         q, ldq = dt.rows(q)
@@ -190,8 +190,12 @@ class IndexFlat:
             if x.dim() != 2 or x.shape[1] != self.d or x.dtype not in (torch.float32, torch.bfloat16):
                 raise ValueError("add expects a (n, %d) float32 or bfloat16 tensor, got %s of %s"
                                  % (self.d, tuple(x.shape), x.dtype))
-            for part in torch.split(x.detach(), max(1, (1 << 28) // self.d)) if x.shape[0] else ():
-                self._b.add_dev(part.float().contiguous())
+            x = x.detach()
+            if x.dtype == torch.float32 or self.storage == "bf16":      # (all at once: the index grows once)
+                self._b.add_dev(x.contiguous())
+            else:
+                for part in torch.split(x, max(1, (1 << 28) // self.d)) if x.shape[0] else ():
+                    self._b.add_dev(part.float().contiguous())
             return
         x = np.ascontiguousarray(x, dtype=np.float32)
         if x.ndim != 2 or x.shape[1] != self.d:

@@ -396,3 +396,25 @@ def test_longest_lists(M, d, storage):
     index, X, q, ids, scores = make(M, 900, d, 1024, storage, 0, seed=22)
     for over in ("list", "index"):
         check(index, X, q, ids, scores, over, 0)
+
+
+@pytest.mark.parametrize("d", [64, 99])
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_added_from_hbm_are_those_added_from_the_host(d, storage, dtype):
+    g = torch.Generator(device="cuda").manual_seed(d)
+    x = torch.randn(1500, 2 * d, generator=g, device="cuda").to(TYPE[dtype])
+    a, b = (faiss.IndexFlat(d, 0, storage=storage) for _ in range(2))
+    for part in (x[:700, :d], x[700:701, d:], x[:0, :d], x[701:, :d]):      # rows apart from each other, one, none
+        a.add(part)
+        b.add(part.float().cpu().numpy())
+    assert a.ntotal == b.ntotal == 1500
+    assert np.array_equal(a.reconstruct_n(0, 1500), b.reconstruct_n(0, 1500))
+    q = np.random.default_rng(0).standard_normal((3, d)).astype(np.float32)
+    for u, v in zip(a.search(q, 5), b.search(q, 5)):
+        assert np.array_equal(u, v)
+    if storage == "f32":
+        assert a._b._lib.rag_flat_add_bf16_dev(a._b._h, 1, x.data_ptr(), None) == _lib.RAG_ERR_INVALID_ARG
+    for bad in (x[:, :d - 1], x[:, :d].double(), x[0, :d]):
+        with pytest.raises(ValueError):
+            a.add(bad)
