@@ -295,7 +295,8 @@ def test_more_workgroups_than_a_launch_takes():
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n,d_in,d_out,S,R", [(2100, 71, 515, 7, 13), (2100, 72, 515, 7, 13), (2100, 71, 515, 7, 16), (4200, 257, 33, 5, 9),
-                                              (4200, 264, 33, 5, 16), (4200, 257, 259, 70, 1), (4097, 5, 900, 3, 2)])
+                                              (4200, 264, 33, 5, 16), (4200, 257, 259, 70, 1), (4097, 5, 900, 3, 2), (2100, 71, 515, 100, 13),
+                                              (1100, 515, 1030, 100, 5)])
 def test_rows_of_no_whole_pieces(n, d_in, d_out, S, R, dtype):
     """Large batches whose rows, ranks or both do not end with a 16-byte piece."""
     check(*make(n, d_in, d_out, S, R, dtype, seed=31))
