@@ -32,7 +32,7 @@ __device__ __forceinline__ void store1(u16* p, float v) { *p = f_to_bf(v); }
 struct Bank {
     const void *w, *a, *b;      // d_out x d_in, slots x rank x d_in, slots x d_out x rank
     const float* scale;         // slots
-    int d_in, d_out, slots, rank, rp;   // rp: row length of U
+    int d_in, d_out, rank, rp;  // rp: row length of U
     bool vec_in, vec_rank;      // 16-byte loads along d_in (x, W, A) and along rank (B)
 };
 struct Order {

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 namespace rag {
 namespace distill {
@@ -93,14 +94,13 @@ bool tile_plan(long long m, int ld, bool bf16, bool grad, TilePlan* p) {
     // as many shares as leave the fewest places for a workgroup idle in the last round; more shares cost their row
     // sums (written once, read once by the join), so the fewest of equals
     const int places = num_cus() * resident(bf16, grad, best);
-    double best_time = 0;
-    for (int s = 1; s <= places; ++s) {
-        const long long groups = (long long)s * p->q_tiles, rounds = (groups + places - 1) / places;
-        if (groups > 4LL * places && s > 1) break;
-        const double time = (double)rounds / s;
-        if (p->splits == 0 || time < best_time - 1e-12) {
-            best_time = time;
-            p->splits = s;
+    p->splits = 1;
+    double best_time = INFINITY;
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+        const long long s = std::min<long long>(places, (long long)rounds * places / p->q_tiles);   // the most that these rounds take
+        if (s > 0 && (double)rounds / s < best_time - 1e-12) {
+            best_time = (double)rounds / s;
+            p->splits = (int)s;
         }
     }
     return true;

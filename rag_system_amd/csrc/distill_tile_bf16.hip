@@ -21,11 +21,11 @@ const Variant GRAD[] = {
     grad<T, 8, 1, 384, 64>(),
 };
 // The loss alone needs no row sum: without O a wave holds its queries' whole rows, and nothing is exchanged between waves (256
-// queries x 768, 1M rows: 916 us with two waves to a query, 593 with one).
+// queries x 768, 1M rows: 916 us with two waves to a query, 593 with one).  Up to 64 queries the rows' bytes
+// bound it, and rows of up to 384 values have no smaller group (16 x 384, 1M rows: 136 us with a group of 16, 137 with one of 64).
 const Variant LOSS[] = {
-    loss<T, 1, 1, 64, 32>(), loss<T, 1, 1, 128, 32>(), loss<T, 1, 1, 192, 32>(), loss<T, 1, 1, 256, 32>(), loss<T, 1, 1, 384, 32>(),
     loss<T, 1, 4, 128, 32>(), loss<T, 1, 4, 192, 32>(), loss<T, 1, 4, 256, 32>(), loss<T, 1, 4, 384, 32>(),
-    loss<T, 2, 2, 64, 32>(), loss<T, 2, 2, 128, 32>(), loss<T, 2, 2, 192, 32>(), loss<T, 2, 4, 128, 32>(), loss<T, 2, 4, 192, 32>(),
+    loss<T, 2, 4, 128, 32>(), loss<T, 2, 4, 192, 32>(),
     loss<T, 2, 4, 256, 32>(), loss<T, 2, 4, 384, 32>(),
     loss<T, 4, 1, 64, 32>(), loss<T, 4, 1, 128, 32>(), loss<T, 4, 1, 192, 32>(), loss<T, 4, 1, 256, 32>(), loss<T, 4, 1, 384, 64>(),
     loss<T, 8, 1, 64, 64>(), loss<T, 8, 1, 128, 32>(), loss<T, 8, 1, 192, 64>(), loss<T, 8, 1, 256, 32>(), loss<T, 8, 1, 384, 32>(),
