@@ -319,3 +319,24 @@ def test_order_of_many_requests(n, S):
     g_ref["dx"][0][n // 2] = float("nan")
     for name, got in (("dx", dx), ("dA", dA), ("dB", dB)):
         assert_within(got, *g_ref[name], name)
+
+
+@pytest.mark.parametrize("n,d_in,d_out,S,R", [(2, 100, 60, 3, 4), (5003, 71, 515, 9, 5), (5003, 72, 512, 9, 16)])
+def test_captured_calls_of_every_size(n, d_in, d_out, S, R):
+    """Forward and backward in one graph, replayed with new requests, with eager calls between the replays."""
+    bank, x, slots, dy = make(n, d_in, d_out, S, R, "bf16", seed=41)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        bank.apply(x, slots), bank.grad(x, slots, dy)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = (bank.apply(x, slots),) + bank.grad(x, slots, dy)
+    for turn in range(4):
+        _, x2, slots2, dy2 = make(n, d_in, d_out, S, R, "bf16", seed=42 + turn)
+        x.copy_(x2), slots.copy_(slots2), dy.copy_(dy2)
+        want = (bank.apply(x2, slots2),) + bank.grad(x2, slots2, dy2)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)

@@ -418,3 +418,21 @@ def test_rows_added_from_hbm_are_those_added_from_the_host(d, storage, dtype):
     for bad in (x[:, :d - 1], x[:, :d].double(), x[0, :d]):
         with pytest.raises(ValueError):
             a.add(bad)
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("M", [3, 20, 70, 130])
+def test_bad_queries_stay_alone(M, storage):
+    """A query of NaN or infinities gives NaN, and not a bit of the others changes (each is a lane of its own in every product)."""
+    index, X, q, ids, scores = make(M, 3000, 64, 6, storage, 0, seed=23, ragged=False)
+    for over in ("list", "index"):
+        for grad in (True, False):
+            want = index.distill(q, ids, scores, over=over, grad=grad)
+            bad = q.clone()
+            bad[1], bad[M - 1] = float("nan"), float("inf")
+            got = index.distill(bad, ids, scores, over=over, grad=grad)
+            keep = [i for i in range(M) if i not in (1, M - 1)]
+            assert torch.isnan(got[0][[1, M - 1]]).all()
+            assert torch.equal(got[0][keep], want[0][keep])
+            if grad:
+                assert torch.isnan(got[1][[1, M - 1]]).all() and torch.equal(got[1][keep], want[1][keep])
