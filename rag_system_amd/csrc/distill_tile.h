@@ -8,8 +8,9 @@
 // per-lane, and the registers of S^T already are the B operand of the second product -- register i of a lane group kl holds
 // row 4 kl + i of the query, so the A operand takes the same rows of X^T.  P never leaves its registers.  (bfloat16: 32
 // rows a product, eight of a lane: four of each half of the tile; X^T comes by the transposing LDS read.  The weights are
-// split into a bfloat16 and the bfloat16 of what is left, two products: one alone, 2^-9 off, is more than the gradient
-// keeps where student and teacher agree and sum_j P x and sum_k p x nearly cancel.)
+// float32: each is the sum of three bfloat16, its bfloat16 and twice that of what is left, which holds all 24 bits, and
+// has three products.  Where student and teacher agree, sum_j P x and sum_k p x nearly cancel, and fewer bits show: two
+// parts, 2^-17 off, took 1.25 ms for 256 queries x 768, 1M rows, against 1.45.)
 // WD waves share a group of 16 queries, each with CW of the columns (the row sum O and the queries of 384 columns
 // fill half of what a wave has with two on a SIMD); their parts of S^T meet in LDS, added in the same order by each.
 // The products add to O a few rows at a time, each rounded at O's last place; a sum over many rows of which one has
@@ -27,9 +28,9 @@
 // of pieces of eight rows) touch every bank once (counted: no conflicts, in either type).
 //
 // Bound by the matrix pipes from 64 queries on, below by the rows' bytes.  Measured, loss and gradient, 1M rows: 1024 queries x 384
-// float32 10.95 ms = 144 TFLOP/s (a large library product: 154; the pipes are busy for 93 % of the time); 256 x 768 bfloat16 1.17 ms
-// = 670 TFLOP/s of the formula's products, 1005 with the second product of the split weights (a large library product: 1261); 16 x
-// 384 float32 302 us = 5.1 TB/s.
+// float32 10.95 ms = 144 TFLOP/s (a large library product: 154; the pipes are busy for 93 % of the time); 256 x 768 bfloat16 1.45 ms
+// with the join = 541 TFLOP/s of the formula's products, 1080 with the two more of the weights' parts (a large library product: 1261);
+// 16 x 384 float32 302 us = 5.1 TB/s.
 #pragma once
 #include "common.h"
 
@@ -268,19 +269,22 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_kernel(TileCall c) {
     // sixteen rows (bfloat16: 32).
     constexpr int STEPS = BF ? SUBS / 2 : SUBS, AHEAD = 2, MID = WD > 1 ? NCT / 2 * STEPS : 0;
     auto add_rows = [&](const char* xs, const f32x4* p, int t, bool next) __attribute__((always_inline)) {
-        u32x4 b[AHEAD + 1], hi[BF ? STEPS : 1], lo[BF ? STEPS : 1];
+        u32x4 b[AHEAD + 1], part[BF ? STEPS : 1][3];       // bfloat16: the weights' parts, the largest first
         if constexpr (BF) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k) {
-                bf16x8 h, r;
+                bf16x8 h[3];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float v = p[2 * k + (e >> 2)][e & 3];
-                    h[e] = (__bf16)v;
-                    r[e] = (__bf16)(v - (float)h[e]);
+                    float v = p[2 * k + (e >> 2)][e & 3];
+#pragma unroll
+                    for (int a = 0; a < 3; ++a) {        // (what is left is exact, and the last part holds all of it)
+                        h[a][e] = (__bf16)v;
+                        v -= (float)h[a][e];
+                    }
                 }
-                hi[k] = __builtin_bit_cast(u32x4, h);
-                lo[k] = __builtin_bit_cast(u32x4, r);
+#pragma unroll
+                for (int a = 0; a < 3; ++a) part[k][a] = __builtin_bit_cast(u32x4, h[a]);
             }
         }
         auto read = [&](int st, u32x4* to) __attribute__((always_inline)) {
@@ -308,8 +312,9 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_kernel(TileCall c) {
             __builtin_amdgcn_sched_barrier(0);
             const u32x4 a = b[st % (AHEAD + 1)];
             if constexpr (BF) {
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, lo[k]), o[j], 0, 0, 0);
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, hi[k]), o[j], 0, 0, 0);
+#pragma unroll
+                for (int w = 2; w >= 0; --w)
+                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, part[k][w]), o[j], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), p[k][i], o[j], 0, 0, 0);

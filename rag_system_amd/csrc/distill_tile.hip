@@ -60,7 +60,7 @@ int resident(bool bf16, bool grad, int v) {
 }
 
 // TFLOP/s that a group of 16, 32, 64, 128 queries reaches (1M rows of 384, float32 and bfloat16, the loss alone and with its gradient).
-constexpr double RATE[2][2][4] = {{{48, 71, 118, 131}, {80, 113, 129, 143}}, {{91, 170, 430, 640}, {171, 306, 600, 840}}};
+constexpr double RATE[2][2][4] = {{{48, 71, 118, 131}, {80, 113, 129, 143}}, {{91, 170, 430, 640}, {171, 276, 535, 710}}};
 
 }  // namespace
 
