@@ -24,10 +24,18 @@ def _hip_rrf(ids, lens, k_const):
     return out_ids[:n_out.value], out_scores[:n_out.value]
 
 
-def _hip_mmr(cand, q, lam, top_k, byte_len, max_bytes):
-    lib = _lib.engine()
-    cand = np.ascontiguousarray(cand, dtype=np.float32)
+def query_of_width(q, d):
+    """The query as the MMR kernels read one: d floats.  They take its length from the candidates, so another is refused here."""
     q = np.ascontiguousarray(q, dtype=np.float32).reshape(-1)
+    if len(q) != d:
+        raise ValueError("the query has %d values, the candidates' vectors have %d" % (len(q), d))
+    return q
+
+
+def _hip_mmr(cand, q, lam, top_k, byte_len, max_bytes):
+    cand = np.ascontiguousarray(cand, dtype=np.float32)
+    q = query_of_width(q, cand.shape[1])
+    lib = _lib.engine()
     byte_len = np.ascontiguousarray(byte_len, dtype=np.int64)
     n, d = cand.shape
     order = np.empty(max(n, 1), dtype=np.int32)
@@ -38,9 +46,9 @@ def _hip_mmr(cand, q, lam, top_k, byte_len, max_bytes):
 
 
 def _hip_mmr_stored(index_backend, rows, q, lam, top_k, byte_len, max_bytes):
+    q = query_of_width(q, index_backend.d)
     lib = _lib.engine()
     rows = np.ascontiguousarray(rows, dtype=np.int64)
-    q = np.ascontiguousarray(q, dtype=np.float32).reshape(-1)
     byte_len = np.ascontiguousarray(byte_len, dtype=np.int64)
     n = len(rows)
     order = np.empty(max(n, 1), dtype=np.int32)
@@ -88,6 +96,7 @@ def mmr_select(cand_emb, query_vec, byte_lens, lambda_param=0.5, top_k=None, max
     if cand_emb.ndim != 2 or cand_emb.shape[0] == 0:
         return []
     top_k = cand_emb.shape[0] if top_k is None else top_k
+    query_vec = query_of_width(query_vec, cand_emb.shape[1])
     return _mmr_impl(cand_emb, query_vec, lambda_param, top_k, byte_lens, max_context_bytes)
 
 
@@ -100,4 +109,5 @@ def mmr_select_stored(index, rows, query_vec, byte_lens, lambda_param=0.5, top_k
         return []
     backend = getattr(index, "_b", index)
     top_k = len(rows) if top_k is None else top_k
+    query_vec = query_of_width(query_vec, index.d)
     return _mmr_stored_impl(backend, rows, query_vec, lambda_param, top_k, byte_lens, max_context_bytes)

@@ -135,12 +135,15 @@ class SearchEngine:
         norm = np.linalg.norm(out, axis=1, keepdims=True)
         return out / np.where(norm < 1e-9, 1.0, norm).astype(np.float32)
 
+    def _needs_bank(self, adapter):
+        if adapter is not None and self.query_adapters is None:
+            raise ValueError("adapter=%r, but this SearchEngine has no query_adapters" % (adapter,))
+
     def _query_vector(self, query, adapter=None, embedding_manager=None):
         """The vector the dense index is searched with."""
+        self._needs_bank(adapter)
         v = (embedding_manager or self.embedding_manager).embed_query(query)
         if self.query_adapters is None:
-            if adapter is not None:
-                raise ValueError("adapter=%r, but this SearchEngine has no query_adapters" % (adapter,))
             return v
         return self._adapted(np.asarray(v, dtype="float32").reshape(1, -1), [adapter]).reshape(np.asarray(v).shape[:-1] + (-1,))
 
@@ -641,17 +644,21 @@ class SearchEngine:
         skipped.  Identical to the default whenever the stored rows equal the re-encodings up to a
         positive factor -- MMR normalises -- which holds for rows added through embed_text / add_vector
         and for a saved index.  Document-mode candidates (joined texts, no single row)
-        fall back to re-encoding."""
+        fall back to re-encoding.
+
+        With query_adapters, stored rows are compared with the adapted query, which the index is searched with, and
+        texts encoded again with the model's own: the vectors that MMR compares are of one space (and width)."""
+        self._needs_bank(adapter)
         if not results:
             return results
         top_k = top_k if top_k is not None else len(results)
         texts = [r.get("chunk", r.get("text", "")) for r in results]
-        q = np.asarray(self._query_vector(query, adapter, embedding_manager), dtype="float32").reshape(-1)
         byte_lens = [len(t.encode("utf-8")) for t in texts]
         if reuse_index_vectors:
             rows = self._chunk_rows(results)
             if rows is not None:
                 index = self.vector_storage.index
+                q = np.asarray(self._query_vector(query, adapter, embedding_manager), dtype="float32").reshape(-1)
                 if getattr(index, "sharded", False):
                     # a row-sharded index: the candidates' rows come from the ranks that hold them (one all-gather
                     # of C x d floats), then the same selection kernel on every rank
@@ -661,6 +668,7 @@ class SearchEngine:
                     order = candidates.mmr_select_stored(index, rows, q, byte_lens, lambda_param, top_k,
                                                          max_context_bytes)
                 return [results[i] for i in order]
+        q = np.asarray(embedding_manager.embed_query(query), dtype="float32").reshape(-1)
         emb = np.array(embedding_manager.model.encode(texts), dtype="float32")
         order = candidates.mmr_select(emb, q, byte_lens, lambda_param, top_k, max_context_bytes)
         return [results[i] for i in order]

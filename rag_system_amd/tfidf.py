@@ -20,6 +20,7 @@ import threading
 import numpy as np
 
 from . import bm25 as _bm25
+from .candidates import query_of_width
 
 
 class TfidfScorer:
@@ -221,6 +222,8 @@ class TfidfScorer:
         if backend is not None and not hasattr(backend, "_h"):
             backend = None
         try:
+            if backend is not None and q is not None:
+                q = query_of_width(q, backend.d)
             out = fn(backend, dense_docs, bm25_docs, k_const, top_k, -float("inf") if threshold is None else threshold,
                      use_knee, q, lam, max_bytes)
         except BaseException:
