@@ -595,10 +595,10 @@ class SearchEngine:
         """One training step's gradients of the query adapters (not in the reference): the cross-encoder, which the
         strategies ask to re-rank a list (:362-394), teaches the dense score to rank like it.
 
-        The queries are embedded and sent through the bank, the index' top_k chunks for them scored by
-        cross_encoder.predict, and the KL divergence of its softmax(scores / teacher_temperature) from the dense
-        softmax(scores / temperature) -- over every row of the index, or over the list alone (over="list") -- taken back
-        to the adapters.  Returns (loss per query, dA, dB), torch tensors in HBM, gradients of the mean loss; the caller's
+        The queries are embedded, sent through the bank and brought to unit length as the strategies search with them, the
+        index' top_k chunks for them scored by cross_encoder.predict, and the KL divergence of its
+        softmax(scores / teacher_temperature) from the dense softmax(scores / temperature) -- over every row of the index,
+        or over the list alone (over="list") -- taken back through the length to the adapters.  Returns (loss per query, dA, dB), torch tensors in HBM, gradients of the mean loss; the caller's
         optimiser applies them to query_adapters.A / .B in place."""
         bank, index = self.query_adapters, self.vector_storage.index
         if bank is None or self.cross_encoder is None:
@@ -617,16 +617,23 @@ class SearchEngine:
         torch = dt.torch_module()
         slots = bank.slots_tensor([None] * n if adapters is None else adapters, n)
         x = torch.from_numpy(np.ascontiguousarray(self._embed_queries(queries), dtype="float32")).to(bank.device).to(bank.dtype)
-        y = bank.apply(x, slots)
-        _, ids = index.search(y.float().cpu().numpy(), min(int(top_k), index.ntotal))
+        y = bank.apply(x, slots).float()
+        norm = y.norm(dim=1, keepdim=True)
+        length = torch.where(norm < 1e-9, 1.0, norm)         # (as _adapted: a length of zero counts as 1)
+        served = y / length
+        _, ids = index.search(served.cpu().numpy(), min(int(top_k), index.ntotal))
         scores = np.full(ids.shape, -np.inf, dtype=np.float32)
         chunks = self.vector_storage.chunks_data
         at = [(i, j) for i in range(n) for j in range(ids.shape[1]) if ids[i, j] >= 0]
         scores[tuple(zip(*at))] = np.asarray(
             self.cross_encoder.predict([(queries[i], chunks[ids[i, j]]["chunk"]) for i, j in at]), dtype=np.float32).reshape(-1)
-        loss, dy = index.distill(y.to(torch.bfloat16 if index.storage == "bf16" else torch.float32),
+        loss, dq = index.distill(served.to(torch.bfloat16 if index.storage == "bf16" else torch.float32),
                                  torch.from_numpy(ids).to(bank.device), torch.from_numpy(scores).to(bank.device), temperature,
                                  teacher_temperature, over, weights=torch.full((n,), 1.0 / n, device=bank.device))
+        # back through y / |y|: what lies along the query changes its length alone, which no score sees
+        dq = dq.float()
+        along = torch.where(norm < 1e-9, 0.0, (served * dq).sum(1, keepdim=True))
+        dy = (dq - served * along) / length
         _, dA, dB = bank.grad(x, slots, dy.to(bank.dtype), input_grad=False)
         return loss, dA, dB
 
