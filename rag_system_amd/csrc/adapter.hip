@@ -623,7 +623,7 @@ int launch_up(const Bank& k, const Order& o, const void* x, long long ldx, const
 
 Bank make_bank(const Call& c, const Plan& p, const void* w, const void* a, const void* b, int d_in, int d_out) {
     const int e = c.dtype == RAG_DTYPE_BF16 ? 8 : 4;
-    Bank k{w, a, b, c.scale, d_in, d_out, p.rank, p.rp, false, false};
+    Bank k{w, a, b, c.scale, d_in, d_out, p.rank, p.rp, c.rank, false, false};
     k.vec_in = d_in % e == 0 && (((uintptr_t)w | (uintptr_t)a) & 15) == 0;
     k.vec_rank = p.rank % e == 0 && ((uintptr_t)b & 15) == 0;
     return k;

@@ -33,6 +33,7 @@ struct Bank {
     const void *w, *a, *b;      // d_out x d_in, slots x rank x d_in, slots x d_out x rank
     const float* scale;         // slots
     int d_in, d_out, rank, rp;  // rp: row length of U
+    int live;                   // of the rank: rows of A behind it are filled-up copies, whose U is zero whatever x and scale are
     bool vec_in, vec_rank;      // 16-byte loads along d_in (x, W, A) and along rank (B)
 };
 struct Order {
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void down_kernel(Down d, Order ord
             const int t = j / RT, r0 = j % RT * 16 + 4 * kl;
             if ((with >> (t * 16 + li)) & 1) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] = r0 + i < k.rank ? sum[i] * scale : 0.f;
+                for (int i = 0; i < 4; ++i) sum[i] = r0 + i < k.live ? sum[i] * scale : 0.f;
                 if (r0 < k.rp) *reinterpret_cast<f32x4*>(u + (p0 + t * 16 + li) * k.rp + r0) = sum;
             }
         }
@@ -248,7 +249,7 @@ __device__ __forceinline__ float down_rows(const Bank& k, const T* x, int s, int
     for (int r = 0; r < 4; ++r)
         for (int o = 32; o > 0; o >>= 1) acc[r] += __shfl_xor(acc[r], o);
     const float v = lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3];
-    return r0 + lane < k.rank ? v * k.scale[s] : 0.f;
+    return r0 + lane < k.live ? v * k.scale[s] : 0.f;
 }
 
 // U where slots have few requests each: a workgroup per position, a wave per four rows of A_s.
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
     }
     const unsigned w_bytes = (unsigned)k.d_out * k.d_in * ESZ;
     auto fetch1 = [&](int t, int b, int a) __attribute__((always_inline)) {
-        const int col = min(t * 128 + lp * 16, k.d_in * ESZ - 16);       // (behind the end: masked in W)
+        const int col = min(t * 128 + lp * 16, k.d_in * ESZ - 16);       // (behind the end: masked)
         distill::lds_dma16(a * 64 < TILED_OUTS ? k.w : xv, a * 64 < TILED_OUTS ? w_bytes : x_bytes, from[a] + col,
                            tiled_lds + b * STAGE + (a * 8 + wave) * 1024);
     };
@@ -508,10 +509,12 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
             for (int o = 0; o < TO; ++o) a[h][o] = *reinterpret_cast<const u32x4*>(ws + o * 2048 + off[h]);
 #pragma unroll
             for (int p = 0; p < TP; ++p) v[h][p] = *reinterpret_cast<const u32x4*>(xs + p * 2048 + off[h]);
-            if (tail) {
+            if (tail) {                     // (both: an infinity times zero is none)
                 const unsigned keep = t * 128 + (h * 4 + kl) * 16 < k.d_in * ESZ ? ~0u : 0u;
 #pragma unroll
                 for (int o = 0; o < TO; ++o) a[h][o] = u32x4{a[h][o][0] & keep, a[h][o][1] & keep, a[h][o][2] & keep, a[h][o][3] & keep};
+#pragma unroll
+                for (int p = 0; p < TP; ++p) v[h][p] = u32x4{v[h][p][0] & keep, v[h][p][1] & keep, v[h][p][2] & keep, v[h][p][3] & keep};
             }
         };
         read(0);

@@ -1,0 +1,35 @@
+"""Query adapters and distillation at the edges of what they admit."""
+import pytest
+import torch
+
+from rag_system_amd.adapters import QueryAdapters
+
+pytestmark = pytest.mark.gpu
+TYPE = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _positive(n, d_in, d_out, S, R, dtype, seed=0):
+    """A bank and requests of positive values: an infinity among them stays one in every sum."""
+    g = torch.Generator(device="cuda").manual_seed(seed + n + d_in + d_out + S + R)
+    r = lambda *s: (0.1 + torch.rand(*s, generator=g, device="cuda")).to(TYPE[dtype])     # noqa: E731
+    bank = QueryAdapters(r(d_out, d_in), r(S, R, d_in), r(S, d_out, R), torch.rand(S, generator=g, device="cuda") + 0.5)
+    return bank, r(n, d_in), torch.randint(-1, S, (n,), generator=g, device="cuda"), r(n, d_out)
+
+
+@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("n,d_in,d_out,S,R", [(3, 70, 40, 2, 13), (50, 72, 515, 3, 5), (520, 72, 1904, 3, 16), (2100, 71, 515, 7, 13), (2100, 72, 2000, 7, 13),
+                                              (2100, 100, 2000, 3, 70), (4200, 257, 33, 5, 9), (4200, 2000, 72, 5, 16)])
+def test_infinite_values_give_infinities(n, d_in, d_out, S, R, dtype):
+    """An infinite value in the last places of x (of dy) gives infinities, as the sum does that leaves out what is only filled up or
+    read twice, and NaN in no other request."""
+    bank, x, slots, dy = _positive(n, d_in, d_out, S, R, dtype)
+    at = torch.tensor([0, 1, n // 2, n - 1], device="cuda").unique()
+    y, (dx, _, _) = bank.apply(x, slots), bank.grad(x, slots, dy)
+    for back in (1, 2, 9):
+        for value in (float("inf"), float("-inf")):
+            x2, dy2 = x.clone(), dy.clone()
+            x2[at, d_in - min(back, d_in)], dy2[at, d_out - min(back, d_out)] = value, value
+            want_y, want_dx = y.clone(), dx.clone()
+            want_y[at], want_dx[at] = value, value
+            assert torch.equal(bank.apply(x2, slots), want_y)
+            assert torch.equal(bank.grad(x2, slots, dy2)[0], want_dx)
