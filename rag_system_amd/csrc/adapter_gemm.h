@@ -7,8 +7,8 @@
 //     down:  U^T = c A_s X^T      (rank x requests)       float32, in sorted order, rank padded to Rp with zeros
 //     up:    Y^T = W X^T + B_s U^T
 // The backward is the same two with the transposed matrices: V = c B_s^T dY, dX = dY W + V A_s.
-// U keeps float32: for bfloat16 weights its product is made of two, with U's bfloat16 and the bfloat16 of what that leaves
-// (a single one would add an error of y's own rounding).
+// U keeps float32: for bfloat16 weights its product is made of three, with the three bfloat16 that hold U's 24 bits (two would lose up
+// to 2^-16 of it, which shows where y is small beside what W and the adapter add to it).
 #pragma once
 #include "distill_tile.h"
 
@@ -312,14 +312,10 @@ __device__ __forceinline__ f32x4 up(const Bank& k, const float* u, long long p, 
                 __builtin_memcpy(&uv, v, 16);
                 sum = M::mma(bv, uv, sum);
             } else {
-                bf16x8 hi, lo;
+                u32x4 part[3];
+                distill::three_parts<true>(v, part);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    hi[e] = (__bf16)v[e];
-                    lo[e] = (__bf16)(v[e] - (float)hi[e]);
-                }
-                sum = M::mma(bv, __builtin_bit_cast(u32x4, lo), sum);
-                sum = M::mma(bv, __builtin_bit_cast(u32x4, hi), sum);
+                for (int a = 2; a >= 0; --a) sum = M::mma(bv, part[a], sum);
             }
         }
         if ((with >> li) & 1) acc += sum;
@@ -562,26 +558,19 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
                 bv[o][r] = piece<true>(bs + (long long)min(ob + o * 16 + li, k.d_out - 1) * k.rank, (r * 4 + kl) * E, k.rank);
         b_slot = s;
     };
-    auto narrow = [&](const f32x4 (*from)[E / 4], u32x4* hi, u32x4* lo) __attribute__((always_inline)) {
+    constexpr int PARTS = E == 8 ? 3 : 1;
+    auto narrow = [&](const f32x4 (*from)[E / 4], u32x4 (*part)[PARTS]) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < RS; ++r) {
             if constexpr (E == 4) {
-                hi[r] = __builtin_bit_cast(u32x4, from[r][0]);
+                part[r][0] = __builtin_bit_cast(u32x4, from[r][0]);
             } else {
-                bf16x8 h, l;
+                float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h[e] = (__bf16)from[r][e >> 2][e & 3];
-                    l[e] = (__bf16)(from[r][e >> 2][e & 3] - (float)h[e]);
-                }
-                hi[r] = __builtin_bit_cast(u32x4, h);
-                lo[r] = __builtin_bit_cast(u32x4, l);
+                for (int e = 0; e < 8; ++e) v[e] = from[r][e >> 2][e & 3];
+                distill::three_parts<true>(v, part[r]);
             }
         }
-    };
-    auto times_u = [&](u32x4 bp, u32x4 hi, u32x4 lo, f32x4 c) __attribute__((always_inline)) {
-        if constexpr (E == 8) c = M::mma(bp, lo, c);
-        return M::mma(bp, hi, c);
     };
     load_u(0, un);
     int b = 0;
@@ -607,8 +596,8 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
     for (int p = 0; p < TP; ++p) {
         const long long q = p0 + wp + p * 16;
         const int slot = next_slot, request = next_request;
-        u32x4 uh[RS], ul[RS];
-        narrow(un, uh, ul);
+        u32x4 part[RS][PARTS];
+        narrow(un, part);
         if (p < TP - 1) {
             look(p + 1, &next_slot, &next_request);
             load_u(p + 1, un);
@@ -627,7 +616,9 @@ __global__ __launch_bounds__(512, 1) void up_tiled_kernel(Bank k, Order ord, con
                 for (int o = 0; o < TO; ++o) {
                     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int r = 0; r < RS; ++r) sum = times_u(bv[o][r], uh[r], ul[r], sum);
+                    for (int r = 0; r < RS; ++r)
+#pragma unroll
+                        for (int a = PARTS - 1; a >= 0; --a) sum = M::mma(bv[o][r], part[r][a], sum);
                     if ((with >> li) & 1) v[o] += sum;          // (others' lanes keep what they have)
                 }
             }

@@ -8,8 +8,7 @@
 // per-lane, and the registers of S^T already are the B operand of the second product -- register i of a lane group kl holds
 // row 4 kl + i of the query, so the A operand takes the same rows of X^T.  P never leaves its registers.  (bfloat16: 32
 // rows a product, eight of a lane: four of each half of the tile; X^T comes by the transposing LDS read.  The weights are
-// float32: each is the sum of three bfloat16, its bfloat16 and twice that of what is left, which holds all 24 bits, and
-// has three products.  Where student and teacher agree, sum_j P x and sum_k p x nearly cancel, and fewer bits show: two
+// float32: each is the sum of three bfloat16, which holds all 24 bits, and has three products.  Where student and teacher agree, sum_j P x and sum_k p x nearly cancel, and fewer bits show: two
 // parts, 2^-17 off, took 1.25 ms for 256 queries x 768, 1M rows, against 1.45.)
 // WD waves share a group of 16 queries, each with CW of the columns (the row sum O and the queries of 384 columns
 // fill half of what a wave has with two on a SIMD); their parts of S^T meet in LDS, added in the same order by each.
@@ -89,6 +88,29 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// Eight float32 values as the sums of three bfloat16 each, the largest first: the upper 16 bits, of what that leaves the upper 16
+// bits, and the rest, eight bits each, so all three are exact.  (Cut off, not rounded: the largest float32 would round to infinity.)
+// INF: infinities too, whose rest is zero.
+template <bool INF>
+__device__ __forceinline__ void three_parts(const float* v, u32x4* part) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned h[2][3];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float rest = v[2 * e + i];
+#pragma unroll
+            for (int a = 0; a < 3; ++a) {
+                h[i][a] = __float_as_uint(rest) & 0xffff0000u;
+                const float top = __uint_as_float(h[i][a]);
+                rest = INF && a == 0 && rest == top ? 0.f : rest - top;
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < 3; ++a) part[a][e] = h[0][a] >> 16 | h[1][a];
+    }
+}
 
 constexpr int WINDOW = 64;      // tiles
 constexpr float LIFT = 40.f;    // powers of two
@@ -273,18 +295,10 @@ __global__ __launch_bounds__(64 * WQ * WD, 1) void tile_kernel(TileCall c) {
         if constexpr (BF) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k) {
-                bf16x8 h[3];
+                float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float v = p[2 * k + (e >> 2)][e & 3];
-#pragma unroll
-                    for (int a = 0; a < 3; ++a) {        // (what is left is exact, and the last part holds all of it)
-                        h[a][e] = (__bf16)v;
-                        v -= (float)h[a][e];
-                    }
-                }
-#pragma unroll
-                for (int a = 0; a < 3; ++a) part[k][a] = __builtin_bit_cast(u32x4, h[a]);
+                for (int e = 0; e < 8; ++e) v[e] = p[2 * k + (e >> 2)][e & 3];
+                three_parts<false>(v, part[k]);          // (no weight is infinite)
             }
         }
         auto read = [&](int st, u32x4* to) __attribute__((always_inline)) {

@@ -16,7 +16,7 @@ def _positive(n, d_in, d_out, S, R, dtype, seed=0):
     return bank, r(n, d_in), torch.randint(-1, S, (n,), generator=g, device="cuda"), r(n, d_out)
 
 
-@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n,d_in,d_out,S,R", [(3, 70, 40, 2, 13), (50, 72, 515, 3, 5), (520, 72, 1904, 3, 16), (2100, 71, 515, 7, 13), (2100, 72, 2000, 7, 13),
                                               (2100, 100, 2000, 3, 70), (4200, 257, 33, 5, 9), (4200, 2000, 72, 5, 16)])
 def test_infinite_values_give_infinities(n, d_in, d_out, S, R, dtype):
