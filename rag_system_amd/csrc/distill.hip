@@ -388,7 +388,9 @@ __global__ __launch_bounds__(THREADS) void list_any_kernel(Call c) {
 
 // Any row length: one workgroup per (split of the rows, query), 32 rows at a time; a wave computes eight dot products,
 // then every thread adds its columns of the 32 rows.  For rows that the other kernels' registers do not hold (over 1536 values):
-// the rows are read twice, the second time from L2.
+// the rows are read twice, the second time from L2.  As in the matrix form, m is a reference that moves when a logit lies more than
+// 2^LIFT above it, and the sums are put down then and every WINDOW steps: added to the share's part in HBM, and begun again.  (All rows of a
+// large batch's one share in one float32 lost 2^-7 of the sum at 300000 rows.)
 constexpr int ANY_ROWS = 32;
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
@@ -402,7 +404,30 @@ __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
     for (int j = tid; j < c.ld; j += THREADS) qs[j] = j < c.d ? load1(q + j) : 0.f;
     __syncthreads();
     float m = -INFINITY, l = 0.f, o[COLS][E] = {};
-    for (long long r = r0; r < r1; r += ANY_ROWS) {
+    float m_part = 0.f, l_part = 0.f;      // of what is put down
+    bool fresh = true;
+    const long long at = blockIdx.x * c.m + i;
+    auto put_down = [&]() {
+        const float before = fresh ? 0.f : expf((m_part - (m == -INFINITY ? 0.f : m)) * c.beta);
+        l_part = fmaf(l_part, before, l);
+        l = 0.f;
+        m_part = m;
+        if (GRAD)
+            for (int b = 0; b < COLS; ++b) {
+                const int j = (b * THREADS + tid) * E;
+                if (j >= c.ld) break;
+                for (int e = 0; e < E; e += 4) {
+                    f32x4* to = reinterpret_cast<f32x4*>(c.part_o + at * c.ld + j + e);
+                    f32x4 v = {o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]};
+                    if (!fresh) v += *to * before;
+                    *to = v;
+                    for (int k = 0; k < 4; ++k) o[b][e + k] = 0.f;
+                }
+            }
+        fresh = false;
+    };
+    int step = 0;
+    for (long long r = r0; r < r1; r += ANY_ROWS, ++step) {
         for (int a = wave; a < ANY_ROWS; a += WAVES) {
             float acc = 0.f;
             if (r + a < r1) {
@@ -420,16 +445,14 @@ __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
             if (lane == 0) s_of[a] = acc;
         }
         __syncthreads();
-        float t = m;
+        float t = -INFINITY;
         for (int a = 0; a < ANY_ROWS; ++a) t = fmaxf(t, s_of[a]);
-        const float scale = t == -INFINITY ? 1.f : expf((m - t) * c.beta);
-        m = t;
-        l *= scale;
-        if (GRAD)
-            for (int b = 0; b < COLS; ++b)
-                for (int e = 0; e < E; ++e) o[b][e] *= scale;
+        const bool lift = (t - m) * c.beta > distill::LIFT * 0.69314718f;      // (uniform; m = -inf: nothing has been added)
+        if ((lift && m != -INFINITY) || (step > 0 && step % distill::WINDOW == 0)) put_down();
+        if (lift) m = t;
+        const float base = m == -INFINITY ? 0.f : m;
         for (int a = 0; a < ANY_ROWS && r + a < r1; ++a) {
-            const float p = s_of[a] == -INFINITY ? 0.f : expf((s_of[a] - m) * c.beta);
+            const float p = expf((s_of[a] - base) * c.beta);
             l += p;
             if (!GRAD) continue;
             for (int b = 0; b < COLS; ++b) {
@@ -442,16 +465,10 @@ __global__ __launch_bounds__(THREADS) void index_any_kernel(Call c) {
         }
         __syncthreads();
     }
-    const long long at = blockIdx.x * c.m + i;
+    put_down();
     if (tid == 0) {
-        c.part_ml[2 * at] = m;
-        c.part_ml[2 * at + 1] = l;
-    }
-    if (!GRAD) return;
-    for (int b = 0; b < COLS; ++b) {
-        const int j = (b * THREADS + tid) * E;
-        if (j < c.ld)
-            for (int e = 0; e < E; ++e) c.part_o[at * c.ld + j + e] = o[b][e];
+        c.part_ml[2 * at] = m_part;
+        c.part_ml[2 * at + 1] = l_part;
     }
 }
 
