@@ -454,7 +454,11 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
     p.sorted = grad || (n > 64 && n_slots > 2 && !p.each);
     p.u = take((size_t)n * p.rp * 4);
     const int e = (int)(16 / esz), in = (d_in + e - 1) / e * e, out = (d_out + e - 1) / e * e, whole_rank = (rank + e - 1) / e * e;
-    p.pad = (in > d_in || whole_rank > rank || (grad && out > d_out)) &&
+    // pieces of all copies (pad_kernel counts them in 32 bits: a backward with a long x and a short dy has more, and does without)
+    const long long pieces = ((long long)n_slots * whole_rank * in + (in > d_in ? n * in : 0) +
+                              (grad ? (out > d_out ? n * out : 0)
+                                    : (in > d_in ? (long long)d_out * in : 0) + (whole_rank > rank ? (long long)n_slots * d_out * whole_rank : 0))) / e;
+    p.pad = (in > d_in || whole_rank > rank || (grad && out > d_out)) && pieces < 1ll << 31 &&
             (grad ? tiled_positions(n, out, d_in, esz) : tiled_positions(n, in, d_out, esz)) > 0;
     p.in = p.pad ? in : d_in;
     p.out = p.pad ? out : d_out;
@@ -565,7 +569,7 @@ void pad_more(Pad* j, int* kinds, const void* from, long long ld, void* to, long
     j->cols[i] = cols;
     j->to_rows[i] = to_rows;
     j->to_cols[i] = to_cols;
-    // (below 2^31: rows of n are within 4 GiB, the bank within 4096 x 128 x 8192)
+    // (below 2^31 in all: make_plan)
     for (int k = i; k < 4; ++k) j->first[k + 1] = j->first[i] + (unsigned)(count * to_rows * (to_cols / Mma<T>::E));
 }
 template <typename T>

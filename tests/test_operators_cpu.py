@@ -89,3 +89,17 @@ def test_adapter_reference_against_autograd():
     ref = adapters_grad_ref(x, W, A, B, c, slots, dy)
     for name, t in (("dx", x), ("dA", A), ("dB", B)):
         assert float((ref[name][0] - t.grad).abs().max()) < 1e-12
+
+
+@pytest.mark.parametrize("dtype,d_in,d_out", [(1, 8191, 8), (0, 4095, 4), (1, 8190, 16)])
+@pytest.mark.parametrize("n", [1 << 21, 1 << 22, (1 << 22) + 77, 1 << 23, 1 << 24])
+def test_no_filled_up_copies_of_more_pieces_than_are_counted(n, dtype, d_in, d_out):
+    """The copies' 16-byte pieces are counted in 32 bits: a backward whose x has 2^31 or more of them is served without copies (a
+    workspace with no room for one of x)."""
+    lib, out = _lib.load_library(), C.c_int64()
+    e, size = (8, 2) if dtype == 1 else (4, 4)
+    whole = (d_in + e - 1) // e * e
+    pieces = n * (whole // e)
+    assert lib.rag_adapter_ws_bytes(dtype, n, d_in, d_out, 2, 1, 1, C.byref(out)) == 0
+    if pieces >= 1 << 31:
+        assert out.value < n * whole * size
