@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from _operators import adapters_grad_ref, adapters_ref, assert_within
 from rag_system_amd.adapters import QueryAdapters
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +34,22 @@ def test_infinite_values_give_infinities(n, d_in, d_out, S, R, dtype):
             want_y[at], want_dx[at] = value, value
             assert torch.equal(bank.apply(x2, slots), want_y)
             assert torch.equal(bank.grad(x2, slots, dy2)[0], want_dx)
+
+
+@pytest.mark.parametrize("n", [1500001, 2800033])
+def test_offsets_behind_two_and_four_gib(n):
+    """Rows of x and dy that begin behind 2 GiB (32-bit offsets of the tiled product) and behind 4 (no tiled product): rows of every
+    part of the batch."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free memory")
+    g = torch.Generator(device="cuda").manual_seed(n)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()     # noqa: E731
+    big, slots = r(n, 768), torch.randint(-1, 3, (n,), generator=g, device="cuda")
+    some = torch.cat([torch.tensor([0, 1, n - 2, n - 1]), torch.arange(0, n, n // 37)]).unique().cuda()
+    W, A, B = r(24, 768), r(3, 12, 768), r(3, 24, 12)
+    y = QueryAdapters(W, A, B).apply(big, slots)
+    want, allow = adapters_ref(big[some], W, A, B, torch.ones(3), slots[some].tolist())
+    assert_within(y[some], want, allow, "y")
+    W, A, B = r(768, 24), r(3, 12, 24), r(3, 768, 12)
+    dx, _, _ = QueryAdapters(W, A, B).grad(y, slots, big)
+    assert_within(dx[some], *adapters_grad_ref(y[some], W, A, B, torch.ones(3), slots[some].tolist(), big[some])["dx"], "dx")
