@@ -47,6 +47,12 @@ __device__ __forceinline__ int place_in_wave(int bits, int bin, bool live, int* 
     *of = __popcll(with);
     return __popcll(with & ((1ull << (threadIdx.x & 63)) - 1));
 }
+// What a lane has written is there for the others of its wave, and is not written before they have read what was.
+__device__ __forceinline__ void wave_meets() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 // f(request, bin, live) for 64 requests of the chunk at a time, eight lots of slots on their way at once.
 template <typename F>
 __device__ __forceinline__ void each_of_chunk(const Sort& s, int c, F f) {
@@ -59,6 +65,7 @@ __device__ __forceinline__ void each_of_chunk(const Sort& s, int c, F f) {
         for (int j = 0; j < 8; ++j) {
             if (t0 + j * 64 >= end) break;      // (uniform)
             f(t0 + j * 64 + lane, bin[j], t0 + j * 64 + lane < end);
+            wave_meets();
         }
     }
 }
@@ -75,6 +82,7 @@ __device__ __forceinline__ void place_chunk(const Sort& s, int c, int* next) {
         int of = 0;
         const int at = place_in_wave(s.bits, bin, live, &of);
         const int to = live ? next[bin] + at : 0;
+        wave_meets();
         if (live && at == of - 1) next[bin] = to + 1;
         if (live) {
             s.perm[to] = t;
