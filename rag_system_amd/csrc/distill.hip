@@ -616,9 +616,9 @@ int launch(Ctx& x) {
             else list_rows_kernel<T, lpr.value, np.value, false><<<(unsigned)c.m, 64 * waves, bytes, x.st>>>(c);
             return true;
         };
-        const bool served = rows(Int<16>(), Int<1>()) || rows(Int<16>(), Int<2>()) || rows(Int<32>(), Int<2>()) ||
-                            rows(Int<32>(), Int<3>()) || rows(Int<32>(), Int<4>()) ||
-                            (E == 4 && (rows(Int<32>(), Int<6>()) || rows(Int<32>(), Int<8>())));
+        bool served = rows(Int<16>(), Int<1>()) || rows(Int<16>(), Int<2>()) || rows(Int<32>(), Int<2>()) || rows(Int<32>(), Int<3>()) ||
+                      rows(Int<32>(), Int<4>());
+        if constexpr (E == 4) served = served || rows(Int<32>(), Int<6>()) || rows(Int<32>(), Int<8>());
         if (!served) list_any_kernel<T><<<(unsigned)c.m, THREADS, ((size_t)c.ld + 2 * c.k) * sizeof(float), x.st>>>(c);
         RAG_HIP(hipGetLastError());
         return RAG_OK;

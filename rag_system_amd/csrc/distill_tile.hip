@@ -44,7 +44,7 @@ const Variants& variants(bool bf16, bool grad) { return (bf16 ? VARIANTS_BF16 : 
 
 // Workgroups of a variant that a CU holds (its LDS and registers; asked of the runtime once per variant).
 int resident(bool bf16, bool grad, int v) {
-    static std::atomic<int> known[2][2][64];
+    static std::atomic<int> known[2][2][MAX_VARIANTS];
     int n = known[bf16][grad][v];
     if (n == 0) {
         const Variant& a = variants(bf16, grad).all[v];

@@ -32,7 +32,7 @@ const Variant LOSS[] = {
     loss<T, 8, 1, 512, 32>(), loss<T, 8, 1, 768, 32>(),
 };
 }  // namespace
-const Variants VARIANTS_BF16[2] = {{LOSS, sizeof LOSS / sizeof LOSS[0]}, {GRAD, sizeof GRAD / sizeof GRAD[0]}};
+const Variants VARIANTS_BF16[2] = {list_of(LOSS), list_of(GRAD)};
 
 }  // namespace distill
 }  // namespace rag

@@ -35,7 +35,7 @@ const Variant LOSS[] = {
     loss<T, 8, 1, 64, 32>(), loss<T, 8, 1, 128, 32>(), loss<T, 8, 1, 192, 32>(), loss<T, 8, 1, 256, 32>(), loss<T, 8, 1, 384, 32>(),
 };
 }  // namespace
-const Variants VARIANTS_F32[2] = {{LOSS, sizeof LOSS / sizeof LOSS[0]}, {GRAD, sizeof GRAD / sizeof GRAD[0]}};
+const Variants VARIANTS_F32[2] = {list_of(LOSS), list_of(GRAD)};
 
 }  // namespace distill
 }  // namespace rag

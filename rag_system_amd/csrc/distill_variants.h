@@ -17,6 +17,12 @@ struct Variants {
     int n;
 };
 extern const Variants VARIANTS_F32[2], VARIANTS_BF16[2];   // [grad]
+constexpr int MAX_VARIANTS = 64;      // of a type and form
+template <int N>
+constexpr Variants list_of(const Variant (&all)[N]) {
+    static_assert(N <= MAX_VARIANTS, "what is known of each variant (distill_tile.hip) has no more places");
+    return Variants{all, N};
+}
 
 constexpr int LDS_MAX = 160 * 1024;
 constexpr int exch_bytes(int wq, int wd, int rt) { return wd > 1 ? wq * wd * (rt / 16) * 1024 : 0; }
