@@ -69,6 +69,7 @@ class SearchEngine:
                              adapter: int = None) -> List[Dict[str, Any]]:
         strategy = strategy.lower().strip()
         retrieval_mode = retrieval_mode.lower().strip()
+        self._needs_bank(adapter)
         self._debug("search_with_strategy strategy=%s top_k=%s mode=%s threshold=%s"
                     % (strategy, top_k, retrieval_mode, threshold))
         if strategy == "faiss":

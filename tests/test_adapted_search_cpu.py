@@ -118,3 +118,13 @@ def test_fused_tail_refuses_a_query_of_another_width():
     assert Csc.calls == 0
     scorer.hybrid_tail(("begun",), Flat(), [0], [0], 2, q=np.ones(8, np.float32))
     assert Csc.calls == 1
+
+
+@pytest.mark.parametrize("strategy", ["faiss", "bm25", "hybrid", "multi", "rrf"])
+def test_an_adapter_without_a_bank_is_refused(strategy):
+    """By every strategy, bm25 too: the caller's adapter would be lost without a word."""
+    with oracle_backends():
+        em, vs = _store(DIM)
+        with pytest.raises(ValueError, match="query_adapters"):
+            SearchEngine(vs, em).search_with_strategy(QUERY, strategy, 5, adapter=1)
+        assert SearchEngine(vs, em, query_adapters=_Bank(DIM)).search_with_strategy(QUERY, "bm25", 5, adapter=1)
