@@ -72,14 +72,16 @@ class SearchEngine:
         self._needs_bank(adapter)
         self._debug("search_with_strategy strategy=%s top_k=%s mode=%s threshold=%s"
                     % (strategy, top_k, retrieval_mode, threshold))
+        # (only where one is asked for: a subclass may override these methods with the arguments they have without adapters)
+        own = {} if adapter is None else {"adapter": adapter}
         if strategy == "faiss":
-            results = self.search_faiss(query, top_k, retrieval_mode, adapter=adapter)
+            results = self.search_faiss(query, top_k, retrieval_mode, **own)
         elif strategy == "bm25":
             results = self.search_bm25(query, top_k, retrieval_mode)
         elif strategy in ("ibrido", "hybrid"):
-            results = self.search_hybrid(query, top_k, retrieval_mode, adapter=adapter)
+            results = self.search_hybrid(query, top_k, retrieval_mode, **own)
         elif strategy == "multi":
-            results = self.search_multi_representation(query, top_k, "document", adapter=adapter)
+            results = self.search_multi_representation(query, top_k, "document", **own)
         elif strategy == "rrf":
             # everything behind the three rankings -- fusion, sort, cut, knee, threshold and (with
             # mmr_reuse_index_vectors) MMR -- in one engine call when it is served (rag_hybrid_rrf_mmr)
@@ -97,7 +99,7 @@ class SearchEngine:
                     return [kept[i] for i in order]
                 return self.mmr_selection(query, kept, self.embedding_manager, lambda_param=mmr_lambda, top_k=top_k,
                                           max_context_bytes=max_context_bytes, reuse_index_vectors=mmr_reuse_index_vectors,
-                                          adapter=adapter)
+                                          **own)
         else:
             raise ValueError(f"Unknown retrieval strategy: {strategy}")
         results.sort(key=_rank_key, reverse=True)
@@ -108,7 +110,7 @@ class SearchEngine:
         if use_mmr and kept:
             kept = self.mmr_selection(query, kept, self.embedding_manager, lambda_param=mmr_lambda, top_k=top_k,
                                       max_context_bytes=max_context_bytes, reuse_index_vectors=mmr_reuse_index_vectors,
-                                      adapter=adapter)
+                                      **own)
         return kept
 
     # ------------------------------------------------------------------ helpers

@@ -128,3 +128,32 @@ def test_an_adapter_without_a_bank_is_refused(strategy):
         with pytest.raises(ValueError, match="query_adapters"):
             SearchEngine(vs, em).search_with_strategy(QUERY, strategy, 5, adapter=1)
         assert SearchEngine(vs, em, query_adapters=_Bank(DIM)).search_with_strategy(QUERY, "bm25", 5, adapter=1)
+
+
+@pytest.mark.parametrize("strategy", ["faiss", "hybrid", "multi", "rrf"])
+def test_subclasses_of_before_the_adapters(strategy):
+    """Methods that a subclass overrides with the arguments they had are called with those, unless an adapter is asked for."""
+    seen = []
+
+    class Mine(SearchEngine):
+        def search_faiss(self, query, top_k=10, retrieval_mode="chunk"):
+            seen.append("faiss")
+            return super().search_faiss(query, top_k, retrieval_mode)
+
+        def search_hybrid(self, query, top_k=10, retrieval_mode="chunk"):
+            seen.append("hybrid")
+            return super().search_hybrid(query, top_k, retrieval_mode)
+
+        def search_multi_representation(self, query, top_k=10, retrieval_mode="document"):
+            seen.append("multi")
+            return super().search_multi_representation(query, top_k, retrieval_mode)
+
+        def mmr_selection(self, query, results, embedding_manager, lambda_param=0.5, top_k=None, max_context_bytes=None,
+                          reuse_index_vectors=False):
+            seen.append("mmr")
+            return super().mmr_selection(query, results, embedding_manager, lambda_param, top_k, max_context_bytes, reuse_index_vectors)
+    with oracle_backends():
+        em, vs = _store(DIM)
+        got = Mine(vs, em).search_with_strategy(QUERY, strategy, 5, threshold=-10.0, use_mmr=True)
+        assert got == SearchEngine(vs, em).search_with_strategy(QUERY, strategy, 5, threshold=-10.0, use_mmr=True)
+    assert seen == ([strategy] if strategy != "rrf" else []) + ["mmr"]
