@@ -601,8 +601,9 @@ class SearchEngine:
         The queries are embedded, sent through the bank and brought to unit length as the strategies search with them, the
         index' top_k chunks for them scored by cross_encoder.predict, and the KL divergence of its
         softmax(scores / teacher_temperature) from the dense softmax(scores / temperature) -- over every row of the index,
-        or over the list alone (over="list") -- taken back through the length to the adapters.  Returns (loss per query, dA, dB), torch tensors in HBM, gradients of the mean loss; the caller's
-        optimiser applies them to query_adapters.A / .B in place."""
+        or over the list alone (over="list") -- taken back through the length to the adapters.  Returns (loss per query, dA,
+        dB), torch tensors in HBM, gradients of the mean loss; the caller's optimiser applies them to query_adapters.A / .B
+        in place."""
         bank, index = self.query_adapters, self.vector_storage.index
         if bank is None or self.cross_encoder is None:
             raise ValueError("distill_step needs query_adapters and a cross_encoder")
@@ -628,6 +629,8 @@ class SearchEngine:
         scores = np.full(ids.shape, -np.inf, dtype=np.float32)
         chunks = self.vector_storage.chunks_data
         at = [(i, j) for i in range(n) for j in range(ids.shape[1]) if ids[i, j] >= 0]
+        if not at:
+            raise ValueError("distill_step: no query finds a row of the index (embeddings of NaN?)")
         scores[tuple(zip(*at))] = np.asarray(
             self.cross_encoder.predict([(queries[i], chunks[ids[i, j]]["chunk"]) for i, j in at]), dtype=np.float32).reshape(-1)
         loss, dq = index.distill(served.to(torch.bfloat16 if index.storage == "bf16" else torch.float32),

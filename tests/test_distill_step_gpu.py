@@ -134,3 +134,28 @@ def test_types_of_bank_and_index(storage, bank_type):
     got = se.distill_step(QUERIES, SLOTS, top_k=60, temperature=1.0)
     for a, b in zip(got, want):
         assert a.dtype == torch.float32 and float((a - b).abs().max()) <= 2.0 ** -3 * float(b.abs().max())
+
+
+def test_queries_without_a_vector():
+    """An embedding of NaN finds no row: the teacher is not asked about it, its loss is 0, and NaN reaches its own slot alone.  Where no
+    query finds a row there is nothing to learn from, and the call says so."""
+    se, bank, _ = _engine(24, 0)
+    embed = se.embedding_manager.model.encode
+    which = []
+
+    class Model:
+        def encode(self, texts):
+            v = np.array(embed(texts))
+            v[which] = np.nan
+            return v
+    se.embedding_manager.model = Model()
+    want = se.distill_step(QUERIES, [0, 1, 2, 0, 0], top_k=9, temperature=0.5)
+    which += [1]
+    loss, dA, dB = se.distill_step(QUERIES, [0, 1, 2, 0, 0], top_k=9, temperature=0.5)
+    assert len(se.cross_encoder.asked[1]) == 4 * 9 and float(loss[1]) == 0
+    for t, w in ((loss[[0, 2, 3, 4]], want[0][[0, 2, 3, 4]]), (dA[[0, 2]], want[1][[0, 2]]), (dB[[0, 2]], want[2][[0, 2]])):
+        assert torch.equal(t, w)
+    which += [0, 2, 3, 4]
+    with pytest.raises(ValueError, match="no query finds"):
+        se.distill_step(QUERIES, [0, 1, 2, 0, 0], top_k=9, temperature=0.5)
+    assert len(se.cross_encoder.asked) == 2
