@@ -4,6 +4,7 @@ import torch
 
 from _operators import adapters_grad_ref, adapters_ref, assert_within
 from rag_system_amd.adapters import QueryAdapters
+from test_distill_gpu import check, make
 
 pytestmark = pytest.mark.gpu
 TYPE = {"f32": torch.float32, "bf16": torch.bfloat16}
@@ -53,3 +54,16 @@ def test_offsets_behind_two_and_four_gib(n):
     W, A, B = r(768, 24), r(3, 12, 24), r(3, 768, 12)
     dx, _, _ = QueryAdapters(W, A, B).grad(y, slots, big)
     assert_within(dx[some], *adapters_grad_ref(y[some], W, A, B, torch.ones(3), slots[some].tolist(), big[some])["dx"], "dx")
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("M", [2, 3, 4])
+@pytest.mark.parametrize("d", [100, 200, 384, 500, 768, 1000, 1024])
+def test_two_to_four_queries(d, M, metric, storage):
+    """Every width class of the form for a few queries, with and without the gradient; equal calls give equal bits."""
+    index, X, q, ids, scores = make(M, 3001, d, 9, storage, metric, seed=41, ragged=False)
+    loss, dq = check(index, X, q, ids, scores, "index", metric)
+    again = index.distill(q, ids, scores, 0.1, 1.5)
+    assert torch.equal(loss, again[0]) and torch.equal(dq, again[1])
+    check(index, X, q, ids, scores, "index", metric, grad=False)
