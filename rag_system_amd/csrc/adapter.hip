@@ -492,9 +492,11 @@ Plan make_plan(int dtype, long long n, int d_in, int d_out, int n_slots, int ran
         p.counts = take((size_t)p.chunks * (n_slots + 2) * 4);
     }
     if (grad) {
-        // (up to 1024 requests every slot is one item, and nothing is left to join: 1024 x 384, 4 slots: 35.5 us, 37 with items of 512;
-        // with 3000, 2 slots, items of 512 are worth it: 55 us, 67 with 1024)
-        p.len = n <= 1024 ? 1024 : (int)std::max<long long>(512, (n + 255) / 256);
+        // One item a slot saves the launch that joins partials, 1.4 us; items of 512 shorten the longest chain.  So one item up to a
+        // mean of 512 a slot, and up to 2048 requests, since all of them may have the same slot (x 384 float32, items of 512 against
+        // one item: 1024 requests of one slot 37 and 48 us, of two 39 and 37, of four 33 and 32; 2000 of four 46 and 45, of sixteen 48
+        // and 47; 3000 of two 53 and 76).
+        p.len = n <= 512ll * std::min(n_slots, 4) ? (int)std::max<long long>(1, n) : (int)std::max<long long>(512, (n + 255) / 256);
         p.max_items = n_slots + (int)(n / p.len) + 1;
         p.max_parts = 2 * (int)(n / p.len) + 2;
         p.v = take((size_t)n * p.rp * 4);

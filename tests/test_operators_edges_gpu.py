@@ -67,3 +67,17 @@ def test_two_to_four_queries(d, M, metric, storage):
     again = index.distill(q, ids, scores, 0.1, 1.5)
     assert torch.equal(loss, again[0]) and torch.equal(dq, again[1])
     check(index, X, q, ids, scores, "index", metric, grad=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,S", [(511, 1), (512, 1), (513, 1), (1024, 2), (1025, 2), (2048, 4), (2049, 4), (2048, 9), (2049, 9)])
+@pytest.mark.parametrize("how", ["spread", "one slot", "none"])
+def test_gradients_around_one_item_a_slot(n, S, how, dtype):
+    """The bank's gradients where slots go from one item to several, and where one slot has every request or none has any."""
+    g = torch.Generator(device="cuda").manual_seed(n + S)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(TYPE[dtype])     # noqa: E731
+    bank, x, dy = QueryAdapters(r(12, 20), r(S, 5, 20), r(S, 12, 5)), r(n, 20), r(n, 12)
+    slots = torch.randint(0, S, (n,), generator=g, device="cuda") if how == "spread" else torch.full((n,), S - 1 if how == "one slot" else -1, device="cuda")
+    want = adapters_grad_ref(x, bank.weight, bank.A, bank.B, bank.scale, slots.tolist(), dy)
+    for name, got in zip(("dx", "dA", "dB"), bank.grad(x, slots, dy)):
+        assert_within(got, *want[name], name)
