@@ -329,7 +329,7 @@ int rag_csc_set_doc_tables(rag_csc_t* h, const int64_t* flat_row, const int64_t*
  *     y_t = W x_t + scale[s] B[s] (A[s] x_t),     s = slots[t];  -1: no adapter, y_t = W x_t
  * x n x d_in (rows ldx apart), W d_out x d_in, A n_slots x rank x d_in, B n_slots x d_out x rank (dense, row-major),
  * scale n_slots float32, slots n int64, y n x d_out (rows ldy apart).  x, W, A, B and y are of `dtype`; sums are
- * float32 and y is rounded once.  A request whose slot is outside [-1, n_slots) gets NaN.  A shorter adapter is
+ * float32 (A x too, also beside bfloat16 weights) and y is rounded once.  A request whose slot is outside [-1, n_slots) gets NaN.  A shorter adapter is
  * one whose last rows of A and columns of B are zero (its gradients are zero there too).  Any alignment of the
  * rows of x / y; y must not overlap the inputs.  `ws_dev`: rag_adapter_ws_bytes bytes, 256-byte aligned, the
  * caller's until the call's work on `stream` is done (calls that may overlap need one each).  Asynchronous on
@@ -361,6 +361,8 @@ int rag_adapter_grad_dev(int dtype, int64_t n, int d_in, int d_out, int n_slots,
  *     dq_i = weights_i d loss_i / d q_i      (weights NULL: 1; dq_dev NULL: the loss alone)
  * q and dq (rows ldq / lddq apart) have the index' storage type, loss float32.  A query without an entry of finite
  * score has loss 0 and dq 0; one with a row number outside [-1, ntotal) gets NaN.  Any alignment.
+ * Weights and sums are float32.  L2 over the index takes its logits from products and norms, so they are off by some 2^-24
+ * (|q|^2 + |x|^2) / temperature; those of the list are sums of squared differences.
  * `ws_dev`: rag_flat_distill_ws_bytes bytes (it does not depend on the number of rows; 0 for the list), 256-byte
  * aligned, the caller's until the call's work on `stream` is done.  Asynchronous on `stream`; equal calls give equal
  * bits.  May be captured into a graph once no added row is staged on the host (L2: once the norms exist), that is

@@ -26,10 +26,11 @@
 // that the 16-byte reads of S (8 rows, one piece) and the reads of O (float32: 4 pieces of rows r and r + 4; bfloat16: a pair
 // of pieces of eight rows) touch every bank once (counted: no conflicts, in either type).
 //
-// Bound by the matrix pipes from 64 queries on, below by the rows' bytes.  Measured, loss and gradient, 1M rows: 1024 queries x 384
-// float32 10.95 ms = 144 TFLOP/s (a large library product: 154; the pipes are busy for 93 % of the time); 256 x 768 bfloat16 1.45 ms
-// with the join = 541 TFLOP/s of the formula's products, 1080 with the two more of the weights' parts (a large library product: 1261);
-// 16 x 384 float32 302 us = 5.1 TB/s.
+// Measured with the join, loss and gradient, 1M rows.  Up to 16 queries the rows' bytes bound it: 16 x 384 float32 302 us = 5.1 TB/s.
+// float32 from 64 queries on, the matrix pipes: 1024 x 384 11.05 ms = 142 TFLOP/s (a large library product: 154), busy for 93 % of the
+// time.  bfloat16: 256 x 768 1.40 to 1.45 ms = 560 TFLOP/s of the formula's products, twice that with the two more of the weights'
+// parts (a large library product: 1261).  The pipes are busy for 54 % of the time: each group of 16 queries reads every tile from LDS
+// for S and again for O, and the weights' parts are made between the two.
 #pragma once
 #include "common.h"
 

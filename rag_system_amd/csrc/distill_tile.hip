@@ -91,8 +91,9 @@ bool tile_plan(long long m, int ld, bool bf16, bool grad, TilePlan* p) {
     p->kind = best;
     p->rows = a.rt;
     p->q_tiles = (int)((m + 16 * a.wq - 1) / (16 * a.wq));
-    // as many shares as leave the fewest places for a workgroup idle in the last round; more shares cost their row
-    // sums (written once, read once by the join), so the fewest of equals
+    // as many shares as leave the fewest places for a workgroup idle in the last round, as if a workgroup could have any place; more
+    // shares cost their row sums (written once, read once by the join), so the fewest of equals.  (The workgroups of a share stay on
+    // one die: fewer than eight shares, from 4096 float32 queries x 384 on, leave dies idle.)
     const int places = num_cus() * resident(bf16, grad, best);
     p->splits = 1;
     double best_time = INFINITY;

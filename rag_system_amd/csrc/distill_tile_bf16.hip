@@ -13,10 +13,10 @@ const Variant GRAD[] = {
     // 32 at a time
     grad<T, 2, 2, 64, 32>(), grad<T, 2, 2, 128, 32>(), grad<T, 2, 2, 192, 32>(), grad<T, 2, 4, 128, 32>(),
     grad<T, 2, 4, 192, 32>(), grad<T, 2, 4, 256, 32>(), grad<T, 2, 4, 384, 32>(),
-    // 64 at a time; 64 rows a tile where the ring still has two (256 queries x 512, 1M rows: 901 us with 32 rows, 846 with 64)
+    // 64 at a time; 64 rows a tile where the ring still has two (256 queries x 512, 1M rows: 1181 us with 32 rows, 1097 with 64)
     grad<T, 4, 2, 64, 64>(), grad<T, 4, 2, 128, 64>(), grad<T, 4, 2, 192, 64>(), grad<T, 4, 2, 256, 64>(),
     grad<T, 4, 2, 384, 32>(),
-    // 128 at a time (1024 queries x 384, 1M rows: 2117 us with tiles of 32 rows, 1838 with 64)
+    // 128 at a time (1024 queries x 384, 1M rows: 2440 us with tiles of 32 rows, 2230 with 64)
     grad<T, 8, 1, 64, 64>(), grad<T, 8, 1, 128, 64>(), grad<T, 8, 1, 192, 64>(), grad<T, 8, 1, 256, 64>(),
     grad<T, 8, 1, 384, 64>(),
 };
