@@ -452,8 +452,8 @@ __global__ __launch_bounds__(512) void whole_kernel(Bank k, Order ord, const voi
 // eight waves 64 x 64 (an operand read for every two products; 32 x 32: for every one), 128 bytes of every row a stage, three stages
 // by LDS-DMA.  (Two waves on a SIMD, since an LDS-DMA instruction holds its wave for 60 to 180 cycles: four waves of 64 x 128 read
 // less and took 30 us more.)  Rows of 16-byte pieces only.
-// 65536 x 768 x 768 bf16, rank 64: 147 us = 526 TFLOP/s (the library's product alone, without adapters: 67), matrix pipes busy for 32 %.  One workgroup fits on a
-// CU, so what it does before its first and behind its last product, some 10 us of each 23, is not hidden by another's products.
+// 65536 x 768 x 768 bf16, rank 64: 147 us = 526 TFLOP/s (the library's product alone, without adapters: 67), matrix pipes busy for
+// 32 % of the time.  One workgroup fits on a CU, so what it does before its first and behind its last product, some 10 us of each 23, is not hidden by another's products.
 // RS: 64-byte steps of the rank that a wave keeps of its slot's B rows while neighbours share the slot.
 constexpr int TILED_OUTS = 128;
 constexpr int tiled_lds_bytes(int pos) { return 3 * (TILED_OUTS + pos) * 128; }

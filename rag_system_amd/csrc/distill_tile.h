@@ -8,8 +8,9 @@
 // per-lane, and the registers of S^T already are the B operand of the second product -- register i of a lane group kl holds
 // row 4 kl + i of the query, so the A operand takes the same rows of X^T.  P never leaves its registers.  (bfloat16: 32
 // rows a product, eight of a lane: four of each half of the tile; X^T comes by the transposing LDS read.  The weights are
-// float32: each is the sum of three bfloat16, which holds all 24 bits, and has three products.  Where student and teacher agree, sum_j P x and sum_k p x nearly cancel, and fewer bits show: two
-// parts, 2^-17 off, took 1.25 ms for 256 queries x 768, 1M rows, against 1.45.)
+// float32: each is the sum of three bfloat16, which holds all 24 bits, and has three products.  Where student and teacher agree,
+// sum_j P x and sum_k p x nearly cancel, and fewer bits show: two parts, 2^-17 off, took 1.25 ms for 256 queries x 768, 1M rows,
+// against 1.40.)
 // WD waves share a group of 16 queries, each with CW of the columns (the row sum O and the queries of 384 columns
 // fill half of what a wave has with two on a SIMD); their parts of S^T meet in LDS, added in the same order by each.
 // The products add to O a few rows at a time, each rounded at O's last place; a sum over many rows of which one has

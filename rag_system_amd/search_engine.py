@@ -640,7 +640,7 @@ class SearchEngine:
         dq = dq.float()
         along = torch.where(norm < 1e-9, 0.0, (served * dq).sum(1, keepdim=True))
         dy = (dq - served * along) / length
-        _, dA, dB = bank.grad(x, slots, dy.to(bank.dtype), input_grad=False)
+        _, dA, dB = bank.grad(x, slots, dy.to(bank.dtype), input_grad=False)     # (y's gradient is of y's type)
         return loss, dA, dB
 
     # ------------------------------------------------------------------ MMR
